@@ -341,6 +341,130 @@ int mrt_attention(const void* q_dev, int q_dtype, const int64_t* q_strides, cons
                   int64_t q_len, int64_t kv_len, int64_t qk_dim, int64_t v_dim, float scale, int causal,
                   void* stream);
 
+/* ---------------------------------------------------------------- 4-bit weights */
+
+/*
+ * Weights held in 4 bits: a code 0..15 for every element, and for every
+ * `group` (32, 64 or 128) columns of a row an FP16 scale s and a zero point z
+ * in 0..15; the weight's value is s (c - z).  K is a multiple of the group.
+ * The reference has no such form; the products stand beside mrt_gemm, for the
+ * few tokens of a decode step (FP16 weights of a prompt: mrt_weight_q4_read
+ * into a buffer and mrt_weight_upload).
+ */
+typedef struct mrt_weight_q4_s* mrt_weight_q4;
+
+/* Quantise W[N, K] (FP16, BF16 or FP32, host or device memory, dense rows) by
+ * rounding to nearest: symmetric != 0: z = 8, s = fp16(max|w| / 7) per group;
+ * else the range of the group widened to hold 0, s = fp16(range / 15), z =
+ * rint(-min / s).  s is at least 2^-24 and at most 65504; NaN becomes code 0. */
+int mrt_weight_q4_upload(const void* src, int src_dtype, int src_on_device, int64_t N, int64_t K, int64_t group,
+                         int symmetric, void* stream, mrt_weight_q4* out);
+
+/* Take codes that exist: codes [N, K / 2] bytes, the even column in the low
+ * half; scales [N, K / group] (rounded to FP16); zeros [N, K / group] bytes
+ * (their low four bits count), or NULL for 8 everywhere. */
+int mrt_weight_q4_import(const void* codes, const void* scales, int scale_dtype, const void* zeros, int src_on_device,
+                         int64_t N, int64_t K, int64_t group, void* stream, mrt_weight_q4* out);
+
+/* Attach a bias of N elements, as mrt_weight_attach_bias. */
+int mrt_weight_q4_attach_bias(mrt_weight_q4 w, const void* src, int src_dtype, int src_on_device, void* stream);
+int mrt_weight_q4_shape(mrt_weight_q4 w, int64_t* n, int64_t* k, int64_t* group);
+/* The values s (c - z), rounded to FP16, as row-major [N, K] with row stride ld. */
+int mrt_weight_q4_read(mrt_weight_q4 w, void* dst_dev, int64_t ld, void* stream);
+int mrt_weight_q4_free(mrt_weight_q4 w);
+
+/*
+ * y_dev[M, N] (row stride ldy) = x_dev[M, K] (FP16, row stride ldx) * W^T in
+ * FP32 sums.  FP16 y: rounded once, then bias (MRT_GEMM_BIAS) and residual
+ * (res_dev FP16 [M, N], row stride ldr, or NULL; y_dev may be res_dev) each
+ * added with a rounding, as mrt_gemm and mrt_gemm_residual do.  FP32 y: the
+ * sums as they are, without bias or residual.  Any M is right; tokens are
+ * taken 16 at a time, each 16 reading the weight once.  No scratch memory.
+ * An infinity or NaN in a token makes its outputs infinities or NaN. */
+int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, const void* res_dev, int64_t ldr, void* y_dev,
+                int y_dtype, int64_t ldy, int64_t M, unsigned flags, void* stream);
+
+/* ---------------------------------------------------------------- 4-bit paged cache */
+
+/*
+ * Keys and values of one layer held in 4 bits, in pages that sequences own in
+ * any order.  A (token, kv head) row of head_dim channels (64 or 128) has one
+ * FP16 scale s and one zero point z: with lo = min(0, min x) and hi = max(0,
+ * max x), s = max(fp16((hi - lo) / 15), 2^-24), z = rint(-lo / s), c =
+ * rint(x / s) + z (both kept in 0..15); the row holds s (c - z).  A row with a
+ * NaN or an infinity, or a range above 15 * 65504, reads back as NaN.  The
+ * handle owns the pages (pages * page_tokens * kv_heads * (head_dim + 8)
+ * bytes, zero at first); page_tokens is a multiple of 16.  rope_theta is that
+ * of the position rotation (pairs i, i + head_dim / 2 turned by position *
+ * rope_theta^(-2 i / head_dim)), or 0 for none.  No counterpart in the
+ * reference.
+ */
+typedef struct mrt_kv_q4_s* mrt_kv_q4;
+
+/*
+ * The sequences of one call.  Rows (tokens) q_start_dev[b] ..
+ * q_start_dev[b + 1] - 1 of q, k, v and out are sequence b's newest, at
+ * positions kv_len_dev[b] - n .. kv_len_dev[b] - 1 (n of them), kv_len_dev[b]
+ * counting the tokens held once they are appended; page table_dev[b *
+ * ld_table + p / page_tokens] holds position p.  The device arrays (INT32) are
+ * read when the kernels run, so a captured call can be replayed with other
+ * lengths and pages, within the sizes given here.  Rows behind
+ * q_start_dev[seqs] and rows at a negative position belong to nobody: they are
+ * not read, stored or written.  A sequence with no rows is skipped.  Lengths
+ * beyond max_q_len, max_kv_len or tokens, and page numbers outside the cache,
+ * are not followed: what needs them is left out, and mrt_sync then returns
+ * MRT_ERR_INVALID_ARG.
+ */
+typedef struct mrt_kv_batch {
+    int64_t seqs;               /* sequences, at most 65535 */
+    int64_t tokens;             /* rows of q, k, v, out */
+    int64_t max_q_len;          /* most rows of one sequence */
+    int64_t max_kv_len;         /* most tokens held for one sequence, at most ld_table * page_tokens */
+    const int32_t* q_start_dev; /* [seqs + 1], not decreasing */
+    const int32_t* kv_len_dev;  /* [seqs] */
+    const int32_t* table_dev;   /* [seqs, ld_table] page numbers */
+    int64_t ld_table;
+} mrt_kv_batch;
+
+int mrt_kv_q4_create(int64_t pages, int64_t page_tokens, int64_t kv_heads, int64_t head_dim, float rope_theta,
+                     mrt_kv_q4* out);
+int mrt_kv_q4_free(mrt_kv_q4 kv);
+
+/*
+ * Rotate and store: k_dev and v_dev [tokens, kv_heads, head_dim] (FP16 or
+ * BF16, heads dense, token strides ldk and ldv in elements) go into the cache,
+ * k rotated first; q_dev [tokens, heads, head_dim] (token stride ldq) is
+ * rotated into q_out_dev (token stride ldqo, which may be q_dev itself).
+ * heads = 0: no q.  All arithmetic in FP32, the angles exact for any position.
+ * Two rows of one call must not share a position of a page.
+ */
+int mrt_kv_q4_append(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype, const void* q_dev, int64_t ldq, int64_t heads,
+                     void* q_out_dev, int64_t ldqo, const void* k_dev, int64_t ldk, const void* v_dev, int64_t ldv,
+                     void* stream);
+
+/* The held values of the batch's rows, rounded to dtype (FP16 or BF16), as
+ * [tokens, kv_heads, head_dim] with token strides ldk and ldv; either of k_dev
+ * and v_dev may be NULL.  Rows that are whole sequences (n = kv_len) give
+ * mrt_attention its K and V. */
+int mrt_kv_q4_read(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype, void* k_dev, int64_t ldk, void* v_dev,
+                   int64_t ldv, void* stream);
+
+/*
+ * out_dev[t, h] = sum_p softmax_p(scale q_dev[t, h] . K[p]) V[p] over the held
+ * positions of the row's sequence: p up to its own (causal != 0) or all
+ * kv_len.  q_dev and out_dev [tokens, heads, head_dim] (FP16 or BF16, token
+ * strides ldq and ldo; out_dev may be q_dev), heads a multiple of kv_heads,
+ * query head h reading kv head h / (heads / kv_heads).  A row that sees no
+ * position gives zeros.  ws_dev: scratch of at least the bytes that
+ * mrt_kv_q4_attention_workspace says for the same batch sizes (256-byte
+ * aligned), the caller's own, so calls with scratch of their own may overlap;
+ * its contents need no clearing and mean nothing afterwards.
+ */
+int mrt_kv_q4_attention_workspace(mrt_kv_q4 kv, const mrt_kv_batch* batch, int64_t heads, size_t* bytes);
+int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype, const void* q_dev, int64_t ldq,
+                        int64_t heads, void* out_dev, int64_t ldo, float scale, int causal, void* ws_dev,
+                        size_t ws_bytes, void* stream);
+
 /* ---------------------------------------------------------------- tensor parallel */
 
 /*

@@ -88,6 +88,19 @@ _SIGS = {
     "mrt_embedding": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _int, _vp]),
     "mrt_attention": (_int, [_vp, _int, C.POINTER(_i64), _vp, _int, C.POINTER(_i64), _vp, _int, C.POINTER(_i64),
                              _vp, _int, C.POINTER(_i64), _i64, _i64, _i64, _i64, _i64, _i64, C.c_float, _int, _vp]),
+    "mrt_weight_q4_upload": (_int, [_vp, _int, _int, _i64, _i64, _i64, _int, _vp, C.POINTER(_vp)]),
+    "mrt_weight_q4_import": (_int, [_vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _vp, C.POINTER(_vp)]),
+    "mrt_weight_q4_attach_bias": (_int, [_vp, _vp, _int, _int, _vp]),
+    "mrt_weight_q4_shape": (_int, [_vp, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64)]),
+    "mrt_weight_q4_read": (_int, [_vp, _vp, _i64, _vp]),
+    "mrt_weight_q4_free": (_int, [_vp]),
+    "mrt_gemv_q4": (_int, [_vp, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _u32, _vp]),
+    "mrt_kv_q4_create": (_int, [_i64, _i64, _i64, _i64, C.c_float, C.POINTER(_vp)]),
+    "mrt_kv_q4_free": (_int, [_vp]),
+    "mrt_kv_q4_append": (_int, [_vp, _vp, _int, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "mrt_kv_q4_read": (_int, [_vp, _vp, _int, _vp, _i64, _vp, _i64, _vp]),
+    "mrt_kv_q4_attention_workspace": (_int, [_vp, _vp, _i64, C.POINTER(_sz)]),
+    "mrt_kv_q4_attention": (_int, [_vp, _vp, _int, _vp, _i64, _i64, _vp, _i64, C.c_float, _int, _vp, _sz, _vp]),
     "mrt_shard_rows": (_int, [C.POINTER(_i64), _i64, _int, _int, C.POINTER(_i64)]),
     "mrt_shard_cols": (_int, [_i64, _int, _int, C.POINTER(_i64), C.POINTER(_i64)]),
     "mrt_tp_unique_id": (_int, [_vp, _sz]),
@@ -254,6 +267,110 @@ def gemm_residual(w: Weight, x_ptr: int, ldx: int, res_ptr: int, ldr: int, y_ptr
                   bias: bool = False, stream: int | None = None) -> None:
     """y = fp16(res + fp16(x W^T (+ bias))); y may be res."""
     call("mrt_gemm_residual", w.h, x_ptr, ldx, res_ptr, ldr, y_ptr, ldy, M, GEMM_BIAS if bias else 0, stream)
+
+
+class WeightQ4:
+    """A weight held in 4 bits (mrt_weight_q4_*): codes, and a scale and a zero
+    point for every `group` columns of a row."""
+
+    def __init__(self, src_ptr: int, src_dtype: int, src_on_device: bool, N: int, K: int, group: int = 128,
+                 symmetric: bool = False, stream: int | None = None):
+        """Quantise W[N, K], rounding to nearest."""
+        h = C.c_void_p()
+        call("mrt_weight_q4_upload", src_ptr, src_dtype, int(src_on_device), N, K, group, int(symmetric), stream,
+             C.byref(h))
+        self._adopt(h)
+
+    @classmethod
+    def from_codes(cls, codes_ptr: int, scales_ptr: int, scale_dtype: int, zeros_ptr: int | None, on_device: bool,
+                   N: int, K: int, group: int, stream: int | None = None) -> "WeightQ4":
+        """Codes that exist: [N, K / 2] bytes, even columns low; scales and zeros [N, K / group]."""
+        self = cls.__new__(cls)
+        h = C.c_void_p()
+        call("mrt_weight_q4_import", codes_ptr, scales_ptr, scale_dtype, zeros_ptr, int(on_device), N, K, group, stream,
+             C.byref(h))
+        self._adopt(h)
+        return self
+
+    def _adopt(self, h: C.c_void_p) -> None:
+        self.h = h
+        n, k, g = C.c_int64(), C.c_int64(), C.c_int64()
+        call("mrt_weight_q4_shape", h, C.byref(n), C.byref(k), C.byref(g))
+        self.n, self.k, self.group = n.value, k.value, g.value
+
+    def attach_bias(self, src_ptr: int, src_dtype: int, src_on_device: bool, stream: int | None = None):
+        call("mrt_weight_q4_attach_bias", self.h, src_ptr, src_dtype, int(src_on_device), stream)
+
+    def read(self, dst_ptr: int, ld: int | None = None, stream: int | None = None) -> None:
+        """The weight's values as row-major FP16 [n, k] in a device buffer."""
+        call("mrt_weight_q4_read", self.h, dst_ptr, self.k if ld is None else ld, stream)
+
+    def free(self):
+        if getattr(self, "h", None):
+            lib().mrt_weight_q4_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def gemv_q4(w: WeightQ4, x_ptr: int, ldx: int, y_ptr: int, ldy: int, M: int, bias: bool = False,
+            res_ptr: int | None = None, ldr: int = 0, y_dtype: int = FP16, stream: int | None = None) -> None:
+    """y = x W^T for a few tokens and a 4-bit weight; y = fp16(res + ...) with res_ptr (y may be res)."""
+    call("mrt_gemv_q4", w.h, x_ptr, ldx, res_ptr, ldr, y_ptr, y_dtype, ldy, M, GEMM_BIAS if bias else 0, stream)
+
+
+class KvBatch(C.Structure):
+    """mrt_kv_batch: the sequences of one call on a paged cache."""
+
+    _fields_ = [("seqs", C.c_int64), ("tokens", C.c_int64), ("max_q_len", C.c_int64), ("max_kv_len", C.c_int64),
+                ("q_start_dev", C.c_void_p), ("kv_len_dev", C.c_void_p), ("table_dev", C.c_void_p),
+                ("ld_table", C.c_int64)]
+
+
+class KvQ4:
+    """A layer's keys and values held in 4 bits, in pages (mrt_kv_q4_*)."""
+
+    def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, rope_theta: float = 0.0):
+        h = C.c_void_p()
+        call("mrt_kv_q4_create", pages, page_tokens, kv_heads, head_dim, rope_theta, C.byref(h))
+        self.h = h
+
+    def append(self, batch: KvBatch, dtype: int, q_ptr: int | None, ldq: int, heads: int, q_out_ptr: int | None,
+               ldqo: int, k_ptr: int, ldk: int, v_ptr: int, ldv: int, stream: int | None = None) -> None:
+        """Rotate q into q_out (heads = 0: no q), rotate k, store k and v."""
+        call("mrt_kv_q4_append", self.h, C.byref(batch), dtype, q_ptr, ldq, heads, q_out_ptr, ldqo, k_ptr, ldk, v_ptr,
+             ldv, stream)
+
+    def read(self, batch: KvBatch, dtype: int, k_ptr: int | None, ldk: int, v_ptr: int | None, ldv: int,
+             stream: int | None = None) -> None:
+        """The held values of the batch's rows."""
+        call("mrt_kv_q4_read", self.h, C.byref(batch), dtype, k_ptr, ldk, v_ptr, ldv, stream)
+
+    def attention_workspace(self, batch: KvBatch, heads: int) -> int:
+        """Bytes of scratch that attention() wants for this batch's sizes."""
+        n = C.c_size_t()
+        call("mrt_kv_q4_attention_workspace", self.h, C.byref(batch), heads, C.byref(n))
+        return n.value
+
+    def attention(self, batch: KvBatch, dtype: int, q_ptr: int, ldq: int, heads: int, out_ptr: int, ldo: int,
+                  scale: float, causal: bool, ws_ptr: int | None, ws_bytes: int, stream: int | None = None) -> None:
+        call("mrt_kv_q4_attention", self.h, C.byref(batch), dtype, q_ptr, ldq, heads, out_ptr, ldo, scale, int(causal),
+             ws_ptr, ws_bytes, stream)
+
+    def free(self):
+        if getattr(self, "h", None):
+            lib().mrt_kv_q4_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
 
 
 def gemm_host(w: Weight, x_host_ptr: int, y_host_ptr: int, M: int, bias: bool = False,

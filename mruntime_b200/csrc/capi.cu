@@ -198,6 +198,9 @@ extern "C" int mrt_sync(void* stream) {
         if (c->counters != nullptr) cudaMemset(c->counters, 0, c->counters_bytes);
         if (flag == 6)  // kErrBadToken: the decoder's embedding met an id outside the vocabulary
             return set_error(MRT_ERR_INVALID_ARG, "embedding_lookup: token_id out of range (device error code 6)");
+        if (flag == 8)  // kErrBadPage
+            return set_error(MRT_ERR_INVALID_ARG,
+                             "paged cache: a page number or a sequence's length is out of bounds (device error code 8)");
         static const char* what[] = {"", "TMA producer", "MMA issuer", "epilogue", "clean-up", "wait self-test",
                                      "embedding", "peer all-reduce"};
         return set_error(MRT_ERR_TIMEOUT, std::string("a kernel wait timed out in the ") +

@@ -23,6 +23,7 @@ enum : int {
     kErrSelfTest = 5,  // mrt_selftest_wait_timeout's wait gave up (expected)
     kErrBadToken = 6,  // the decoder's embedding met a token id outside the vocabulary
     kErrPeerWait = 7,  // a cross-GPU all-reduce gave up waiting for a peer's partial
+    kErrBadPage = 8,   // a paged cache's batch names a page or a length outside its bounds
 };
 
 // Wall-clock limit of one bounded wait, in nanoseconds of %globaltimer.
