@@ -1,6 +1,8 @@
 // kv_q4_attn.cu -- softmax attention of new tokens' queries over a paged cache
 // held in 4 bits (kv_q4.h): the reference's attention op
 // (src/core/cpu_backend.cpp:171-290) over such a cache.
+#include <cuda_bf16.h>
+
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -33,78 +35,6 @@ __device__ __forceinline__ float widen(uint16_t h, int dtype) {
 __device__ __forceinline__ uint16_t narrow(float f, int dtype) {
     if (dtype == MRT_FP16) return f32_to_f16_bits(f);
     return f != f ? static_cast<uint16_t>(0x7FC0) : f32_to_bf16_bits(f);
-}
-
-// One CTA per token, one warp per query head at a time, one key at a time with
-// the running maximum and sum of the softmax.
-template <int PER>
-__global__ void __launch_bounds__(kThreads) attn_q4_rows_kernel(const AttnQ4Args a) {
-    constexpr int D = PER * 32;
-    __shared__ int s_seq;
-    griddep_wait();
-    griddep_launch_dependents();
-    const KvView& v = a.v;
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) s_seq = -1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < v.seqs; b += blockDim.x)
-        if (v.q_start[b] <= t && t < v.q_start[b + 1]) s_seq = b;
-    __syncthreads();
-    const int b = s_seq;
-    if (b < 0) return;
-    int first, n, kv;
-    if (!kv_seq(v, b, &first, &n, &kv)) {
-        if (threadIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
-        return;
-    }
-    const int keys = a.causal ? kv - n + (t - first) + 1 : kv;  // may be 0 or less: no key
-    for (int h = warp; h < a.heads; h += kThreads / 32) {
-        const int kh = h / (a.heads / v.kv_heads);
-        float q[PER], o[PER];
-        float m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            q[j] = widen(a.q[t * a.ldq + h * D + lane * PER + j], a.dtype) * a.scale;
-            o[j] = 0.0f;
-        }
-        const uint8_t* block = nullptr;
-        for (int p = 0; p < keys; ++p) {
-            const int token = p & (kKvBlock - 1);
-            if (token == 0) {
-                block = kv_block_at(v, v.table + static_cast<int64_t>(b) * v.ld_table, kh, p);
-                if (block == nullptr) {
-                    if (lane == 0) raise_error(v.err_flag, kErrBadPage);
-                    break;
-                }
-            }
-            const uint32_t ks = reinterpret_cast<const uint32_t*>(block + kv_k_scales(D))[token];
-            const uint32_t vs = reinterpret_cast<const uint32_t*>(block + kv_v_scales(D))[token];
-            const int w = lane * PER / 8;
-            const uint32_t kw = *reinterpret_cast<const uint32_t*>(block + kv_k_word(D, token, w));
-            const uint32_t vw = *reinterpret_cast<const uint32_t*>(block + kv_v_word(D, token, w));
-            float s = 0.0f;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int c = (kw >> (4 * pair_nibble((lane * PER + j) & 7))) & 15;
-                s = fmaf(q[j], static_cast<float>(c - static_cast<int>(ks >> 16)), s);
-            }
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, off);
-            s *= f16_bits_to_f32(static_cast<uint16_t>(ks));
-            const float m2 = fmaxf(m, s), fix = expf(m - m2), e = expf(s - m2);
-            const float ev = e * f16_bits_to_f32(static_cast<uint16_t>(vs));
-            l = l * fix + e;
-            m = m2;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int c = (vw >> (4 * ((lane * PER + j) & 7))) & 15;
-                o[j] = fmaf(ev, static_cast<float>(c - static_cast<int>(vs >> 16)), o[j] * fix);
-            }
-        }
-        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) a.out[t * a.ldo + h * D + lane * PER + j] = narrow(o[j] * inv, a.dtype);
-    }
 }
 
 // Four neighbouring channels of an output row (any alignment of the row).
@@ -661,6 +591,766 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const RowsArgs a
     }
 }
 
+// ------------------------------------------------------------------ many rows
+
+// TMEM accesses in MMA-fragment order, 16 lanes (rows) at a time: lane (r, c)
+// of the warp gets, of every eight 32-bit columns, columns 2c and 2c + 1 of
+// rows r and r + 8.  (A thread then meets a quarter of the columns instead of
+// all of them, so what belongs to a column is loaded a quarter as often.)
+__device__ __forceinline__ void tmem_ld_frag128(uint32_t taddr, uint32_t (&r)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x16.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, "
+        "%40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, "
+        "%59, %60, %61, %62, %63"
+        "}, [%64];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]),
+          "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
+          "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]),
+          "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]),
+          "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_frag64(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
+        "}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_st_frag64(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32"
+        "};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// 64 columns of 32 bits, one register a column and row: lane (r, c) holds, of
+// every four columns, column c of rows r and r + 8.
+__device__ __forceinline__ void tmem_st_pairs64(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32"
+        "};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem]^T.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Wait for a phase, bounded: after kWaitLimitNs, or once another thread of the
+// CTA has given up, the wait ends, and the kernel runs on to its end without
+// waiting (every access stays in bounds whatever was computed).  Unlike
+// mbar_wait it does not look at the device's error flag: a bad page of one
+// sequence must not end another's waits.
+__device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
+    if (mbar_try_wait(bar, parity)) return;
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return;
+        if ((it & 63u) == 0) {
+            if (*gave_up) return;
+            if (globaltimer_ns() - t0 > kWaitLimitNs) {
+                *gave_up = 1;
+                raise_error(flag, code);
+                return;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Many rows (prompts, chunks of prompts): tcgen05 flash attention.  A CTA
+// takes 256 rows of a (sequence, kv head) -- new tokens times the query heads
+// that share it -- as two tiles of 128, and keys 128 at a time:
+//
+//   warps 0-3, 4-7  softmax of tile 0, 1: S from TMEM, P' back into its place
+//   warps 8-11      K and V codes from the pages to 16-bit integers c - z
+//                   (exact) in the tensor cores' swizzled layout
+//   warp 12         the products: S_i = Q_i K^T, O_i += P'_i V (A from TMEM)
+//
+// so that one tile's softmax runs beside the other's products.  Scales stay
+// out of the operands: a key's multiplies its column of S, a value's goes into
+// the exponent, as in the few-rows kernel.  The running maximum m is moved only
+// when a row exceeds it by 2^8 (P' then still fits FP16 with all its bits), so
+// O in TMEM is hardly ever rescaled.  TMEM: S_0, S_1 (P' in their first half),
+// O_0, O_1.
+//
+// Units' key tiles are dealt to the CTAs in equal contiguous stretches, as in
+// the few-rows kernel, parts of units that span CTAs joined from scratch.
+constexpr int kManyRows = 256, kManyKeys = 128;
+constexpr int kManyThreads = 13 * 32;
+
+struct ManyPart {  // a unit that begins in a CTA's stretch and goes on
+    int seq, head, row0;
+    int place;     // 0 or 1: which of the CTA's two places holds its part
+    int last_cta;  // < 0: none
+};
+
+struct ManyArgs {
+    AttnQ4Args a;
+    int group, grid;
+    float* part_o;     // [2 * grid][256][D]
+    float2* part_ml;   // [2 * grid][256]
+    ManyPart* parts;   // [grid]
+};
+
+// sum_{i < n} floor((a i + b) / m), all >= 0: the lattice points under a line,
+// counted by exchanging the axes until the line is flat.
+__device__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+    int64_t sum = 0;
+    while (n > 0) {
+        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const int64_t top = a * n + b;
+        if (top < m) break;
+        n = top / m;
+        b = top % m;
+        const int64_t t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+
+// Key tiles of a sequence's row tiles.  Row tile x < count - 1 ends with token
+// (256 x + 255) / group, and causal rows see keys up to themselves.
+struct ManySeq {
+    int first, n, kv, group, causal;
+    int count;  // row tiles, 0: nothing to do
+    __device__ __forceinline__ int64_t past() const { return max(kv - n, 0); }
+    __device__ __forceinline__ int tiles(int x) const {
+        if (!causal) return max(1, (kv + kManyKeys - 1) / kManyKeys);
+        const int64_t last = min(static_cast<int64_t>(n) - 1, (static_cast<int64_t>(kManyRows) * x + kManyRows - 1) / group);
+        return static_cast<int>((past() + last) / kManyKeys) + 1;
+    }
+    // of row tiles 0 .. x - 1
+    __device__ __forceinline__ int64_t before(int x) const {
+        if (!causal) return static_cast<int64_t>(x) * tiles(0);
+        const int y = min(x, count - 1);
+        int64_t t = y + floor_sum(y, static_cast<int64_t>(kManyKeys) * group, kManyRows, kManyRows - 1 + past() * group);
+        if (x == count) t += tiles(count - 1);
+        return t;
+    }
+};
+
+__device__ __forceinline__ bool many_seq(const ManyArgs& g, int b, ManySeq* s) {
+    const bool ok = kv_seq(g.a.v, b, &s->first, &s->n, &s->kv);
+    s->group = g.group;
+    s->causal = g.a.causal;
+    s->count = ok ? static_cast<int>((static_cast<int64_t>(s->n) * g.group + kManyRows - 1) / kManyRows) : 0;
+    return ok;
+}
+
+template <int D>
+struct ManyShape {
+    static constexpr int kPanel = 128 * 128;            // 128 rows of 64 16-bit columns
+    static constexpr int kQ = 2 * (D / 64) * kPanel;
+    static constexpr int kK = (D / 64) * kPanel;        // a stage
+    static constexpr int kV = 2 * D * 128;              // V^T: two panels (64 keys) of D rows
+    static constexpr int kCols = 64 * 16 + 64 * 8;      // (ks, ks, lv, lv), (rs, rs) of each column pair
+    static constexpr int kStages = 2;
+    static constexpr int kBytes = 1024 + kQ + kStages * (kK + kV + kCols);
+};
+
+// 16 bytes (eight 16-bit columns) of row `row` in a swizzled panel of 128-byte rows.
+__device__ __forceinline__ uint32_t panel_at(uint32_t base, int row, int chunk) {
+    return base + row * 128 + ((chunk ^ (row & 7)) << 4);
+}
+
+__device__ __forceinline__ void st_shared_16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                              *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+constexpr uint32_t kSixteenth = 0x2C002C00u;  // FP16 1/16 twice
+
+// Codes at bits 0-3 / 4-7 of each half less the zero points, as FP16: z1024 =
+// the halves 1024 + z, z64 = -(64 + z).  1024 + c and (1024 + 16 c) / 16 are exact.
+__device__ __forceinline__ uint32_t nib0_f16(uint32_t w, uint32_t z1024) { return h2_sub((w & kNib0) | 0x64006400u, z1024); }
+__device__ __forceinline__ uint32_t nib1_f16(uint32_t w, uint32_t z64) {
+    return h2_fma((w & kNib1) | 0x64006400u, kSixteenth, z64);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const ManyArgs args) {
+    using S = ManyShape<D>;
+    constexpr int kPanels = D / 64;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_full[2], s_empty[2], s_scores[2], s_probs[2], s_done[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_gave_up, s_seq;
+    __shared__ int64_t s_sum[13], s_at;
+    uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    const uint32_t q_u32 = smem_u32(smem), k_u32 = q_u32 + S::kQ, v_u32 = k_u32 + S::kStages * S::kK;
+    uint8_t* cols = smem + S::kQ + S::kStages * (S::kK + S::kV);
+    const AttnQ4Args& a = args.a;
+    const KvView& v = a.v;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 128);
+            mbar_init(&s_empty[i], 1);
+            mbar_init(&s_scores[i], 1);
+            mbar_init(&s_probs[i], 4);
+            mbar_init(&s_done[i], 1);
+        }
+        s_gave_up = 0;
+        fence_barrier_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(&s_tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    griddep_launch_dependents();  // after the allocation: whoever follows may want TMEM of its own
+    griddep_wait();
+
+    // This CTA's stretch, and the unit it begins in.
+    int64_t mine = 0;
+    for (int b = threadIdx.x; b < v.seqs; b += kManyThreads) {
+        ManySeq q;
+        if (!many_seq(args, b, &q) && blockIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
+        if (q.count > 0) mine += q.before(q.count);
+    }
+    const int64_t total = block_sum<13>(mine, s_sum) * v.kv_heads;
+    const int64_t per = (total + args.grid - 1) / args.grid;
+    int64_t at = blockIdx.x * per;
+    const int64_t end = min(total, at + per), range_begin = at;
+    ManySeq sq;
+    int seq = -1, head = 0, x = 0;
+    int64_t unit_at = 0;
+    ManyPart part{0, 0, 0, 0, -1};
+    if (at < end) {
+        int64_t before = 0;
+        for (int b0 = 0; seq < 0; b0 += kManyThreads) {
+            const int b = b0 + threadIdx.x;
+            int64_t t = 0;
+            if (b < v.seqs) {
+                ManySeq q;
+                many_seq(args, b, &q);
+                if (q.count > 0) t = q.before(q.count) * v.kv_heads;
+            }
+            int64_t incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t u = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                if (lane >= o) incl += u;
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) s_seq = -1;
+            if (lane == 31) s_sum[warp] = incl;
+            __syncthreads();
+            int64_t base = before;
+            for (int w = 0; w < warp; ++w) base += s_sum[w];
+            if (at >= base + incl - t && at < base + incl) {
+                s_seq = b;
+                s_at = base + incl - t;
+            }
+            for (int w = 0; w < 13; ++w) before += s_sum[w];
+            __syncthreads();
+            seq = s_seq;
+            unit_at = s_at;
+        }
+        many_seq(args, seq, &sq);
+        const int64_t a_head = sq.before(sq.count);
+        head = static_cast<int>((at - unit_at) / a_head);
+        unit_at += head * a_head;
+        const int64_t off = at - unit_at;
+        int lo = 0, span = sq.count;  // the row tile lies in [lo, lo + span)
+        while (span > 1) {
+            const int step = (span + kManyThreads - 1) / kManyThreads;
+            const int mid = lo + threadIdx.x * step;
+            const int n = __syncthreads_count(mid < lo + span && sq.before(mid) <= off);
+            const int next = lo + (n - 1) * step;
+            span = min(step, lo + span - next);
+            lo = next;
+        }
+        x = lo;
+        unit_at += sq.before(x);
+    }
+
+    uint32_t stage_it = 0, tile_it[2] = {0, 0};  // key tiles so far: of the CTA, of each row tile
+    const uint32_t idesc_qk = idesc_f16_f32(128, kManyKeys) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+    const uint32_t idesc_pv = idesc_f16_f32(128, D);
+    while (at < end) {
+        int tiles = sq.tiles(x);
+        if (at >= unit_at + tiles) {  // the next unit
+            unit_at += tiles;
+            if (++x == sq.count) {
+                x = 0;
+                if (++head == v.kv_heads) {
+                    head = 0;
+                    do {
+                        ++seq;
+                        many_seq(args, seq, &sq);
+                    } while (sq.count == 0);
+                }
+            }
+            tiles = sq.tiles(x);
+        }
+        const int t0 = static_cast<int>(at - unit_at);
+        const int t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - at)));
+        const int row0 = x * kManyRows;
+        const int64_t all_rows = static_cast<int64_t>(sq.n) * args.group;
+        const int rows = static_cast<int>(min(static_cast<int64_t>(kManyRows), all_rows - row0));
+        const int row_tiles = rows > 128 ? 2 : 1;
+        const int count = t1 - t0;
+
+        // Q, as it is, into its panels.
+        {
+            const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.ldq & 7) == 0;
+            for (int i = threadIdx.x; i < row_tiles * 128 * (D / 8); i += kManyThreads) {
+                const int row = i / (D / 8), ch = i - row * (D / 8);
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (row < rows) {
+                    const int tok = (row0 + row) / args.group, gh = row0 + row - tok * args.group;
+                    const uint16_t* src = a.q + (sq.first + tok) * a.ldq + (head * args.group + gh) * D + ch * 8;
+                    if (vec) {
+                        w = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        w.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
+                        w.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
+                        w.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
+                        w.w = src[6] | static_cast<uint32_t>(src[7]) << 16;
+                    }
+                }
+                const uint32_t base = q_u32 + ((row >> 7) * kPanels + (ch >> 3)) * S::kPanel;
+                st_shared_16(panel_at(base, row & 127, ch & 7), w.x, w.y, w.z, w.w);
+            }
+            fence_async_smem();
+        }
+        __syncthreads();
+
+        if (warp < 8) {
+            // ---------------------------------------------------------- softmax
+            const int i = warp >> 2;
+            if (i < row_tiles) {
+                const int r = lane >> 2, c = lane & 3;
+                const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // its 32 TMEM lanes
+                const uint32_t t_s = tmem + i * 128 + lanes, t_o = tmem + 256 + i * D + lanes;
+                float m[4], l[4];
+                int limit[4], limit_min = 0x7FFFFFFF;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = i * 128 + (warp & 3) * 32 + k * 8 + r;
+                    m[k] = -INFINITY;
+                    l[k] = 0.0f;
+                    limit[k] = 0;
+                    if (row < rows) {
+                        limit[k] = a.causal ? sq.kv - sq.n + (row0 + row) / args.group + 1 : sq.kv;
+                        limit_min = min(limit_min, limit[k]);
+                    }
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
+                for (int j = 0; j < count; ++j) {
+                    const uint32_t it = stage_it + j, ti = tile_it[i] + j, st = it & 1;
+                    const uint8_t* cc = cols + st * S::kCols;
+                    const float4* kl = reinterpret_cast<const float4*>(cc) + c;
+                    const float2* rs = reinterpret_cast<const float2*>(cc + 1024) + c;
+                    const int pos0 = (t0 + j) * kManyKeys;
+                    const bool inner = pos0 + kManyKeys <= limit_min;
+                    wait_phase(&s_full[st], (it >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                    wait_phase(&s_scores[i], ti & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                    __syncwarp();
+                    tc_fence_after();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {  // rows h 16 + r, + 8
+                        uint32_t s[64];
+                        tmem_ld_frag128(t_s + (static_cast<uint32_t>(h) << 20), s);
+                        float big[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float4 w = kl[k * 4];
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                float y0 = fmaf(__uint_as_float(s[k * 4 + b * 2]), w.x, w.z);
+                                float y1 = fmaf(__uint_as_float(s[k * 4 + b * 2 + 1]), w.y, w.w);
+                                if (!inner) {
+                                    if (pos0 + k * 8 + c * 2 >= limit[h * 2 + b]) y0 = -INFINITY;
+                                    if (pos0 + k * 8 + c * 2 + 1 >= limit[h * 2 + b]) y1 = -INFINITY;
+                                }
+                                big[b] = fmaxf(big[b], fmaxf(y0, y1));
+                                s[k * 4 + b * 2] = __float_as_uint(y0);
+                                s[k * 4 + b * 2 + 1] = __float_as_uint(y1);
+                            }
+                        }
+                        bool grow = false;
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
+                            big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 2));
+                            grow |= big[b] > m[h * 2 + b] + 8.0f;  // from -inf: any
+                        }
+                        if (__any_sync(0xFFFFFFFFu, grow)) {
+                            float fix[2];
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                const float to = fmaxf(m[h * 2 + b], big[b]);
+                                fix[b] = to == -INFINITY ? 1.0f : fast_exp2(m[h * 2 + b] - to);
+                                m[h * 2 + b] = to;
+                                l[h * 2 + b] *= fix[b];
+                            }
+                            if (j > 0) {  // the scores were asked for after the last product into O had ended
+#pragma unroll
+                                for (int ch = 0; ch < D; ch += 64) {
+                                    uint32_t o[32];
+                                    const uint32_t t = t_o + (static_cast<uint32_t>(h) << 20) + ch;
+                                    tmem_ld_frag64(t, o);
+#pragma unroll
+                                    for (int k = 0; k < 32; ++k)
+                                        o[k] = __float_as_uint(__uint_as_float(o[k]) * fix[(k >> 1) & 1]);
+                                    tmem_st_frag64(t, o);
+                                }
+                            }
+                        }
+                        uint32_t p[32];
+                        float base[2];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) base[b] = m[h * 2 + b] == -INFINITY ? 0.0f : m[h * 2 + b];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float2 w = rs[k * 4];
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                const float p0 = fast_exp2(__uint_as_float(s[k * 4 + b * 2]) - base[b]);
+                                const float p1 = fast_exp2(__uint_as_float(s[k * 4 + b * 2 + 1]) - base[b]);
+                                l[h * 2 + b] = fmaf(p0, w.x, fmaf(p1, w.y, l[h * 2 + b]));
+                                const __half2 hp = __floats2half2_rn(p0, p1);
+                                p[k * 2 + b] = *reinterpret_cast<const uint32_t*>(&hp);
+                            }
+                        }
+                        tmem_st_pairs64(t_s + (static_cast<uint32_t>(h) << 20), p);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_probs[i]);
+                }
+                // The output, or the unit's part of it.
+                wait_phase(&s_done[i], (tile_it[i] + count - 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                __syncwarp();
+                tc_fence_after();
+                const bool whole = t0 == 0 && t1 == tiles;
+                const int64_t slot = blockIdx.x * 2LL + (unit_at > range_begin ? 1 : 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    l[k] += __shfl_xor_sync(0xFFFFFFFFu, l[k], 1);
+                    l[k] += __shfl_xor_sync(0xFFFFFFFFu, l[k], 2);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int ch = 0; ch < D; ch += 64) {
+                        uint32_t o[32];
+                        __syncwarp();
+                        tmem_ld_frag64(t_o + (static_cast<uint32_t>(h) << 20) + ch, o);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const int row = i * 128 + (warp & 3) * 32 + h * 16 + b * 8 + r;
+                            if (row >= rows) continue;
+                            const float sum = l[h * 2 + b];
+                            if (whole) {
+                                const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+                                const int tok = (row0 + row) / args.group, gh = row0 + row - tok * args.group;
+                                uint16_t* dst = a.out + (sq.first + tok) * a.ldo + (head * args.group + gh) * D + ch + c * 2;
+                                const bool vec = (reinterpret_cast<uintptr_t>(dst) & 3) == 0;
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    const uint16_t h0 = narrow(__uint_as_float(o[k * 4 + b * 2]) * inv, a.dtype);
+                                    const uint16_t h1 = narrow(__uint_as_float(o[k * 4 + b * 2 + 1]) * inv, a.dtype);
+                                    if (vec) {
+                                        *reinterpret_cast<uint32_t*>(dst + k * 8) = h0 | static_cast<uint32_t>(h1) << 16;
+                                    } else {
+                                        dst[k * 8] = h0;
+                                        dst[k * 8 + 1] = h1;
+                                    }
+                                }
+                            } else {
+                                float* dst = args.part_o + (slot * kManyRows + row) * D + ch + c * 2;
+#pragma unroll
+                                for (int k = 0; k < 8; ++k)
+                                    *reinterpret_cast<float2*>(dst + k * 8) =
+                                        make_float2(__uint_as_float(o[k * 4 + b * 2]), __uint_as_float(o[k * 4 + b * 2 + 1]));
+                                if (ch == 0 && c == 0) args.part_ml[slot * kManyRows + row] = make_float2(m[h * 2 + b], sum);
+                            }
+                        }
+                    }
+                tc_fence_before();
+            }
+        } else if (warp < 12) {
+            // ---------------------------------------------------------- codes to integers
+            const int tid = threadIdx.x - 256;
+            const int32_t* row_table = v.table + static_cast<int64_t>(seq) * v.ld_table;
+            const float fac = a.scale * 1.4426950408889634f;
+            // K: token tid.  V: eight tokens (a half block), a stretch of D / 8 channels:
+            // eight neighbouring lanes write eight different 16-byte columns of a panel.
+            const int v_half = (warp & 1) * 8 + (lane & 7);                        // of 16 half blocks
+            const int v_r = ((warp - 8) >> 1) * 4 + (lane >> 3);                   // channel stretch
+            uint4 kw[D / 32], vw[D / 32], vz[2];
+            uint32_t ks, vs;
+            auto load = [&](int j) {  // tile j's bytes, one tile ahead of their use
+                const int pos0 = (t0 + j) * kManyKeys;
+                const int kpos = pos0 + tid, vpos = pos0 + v_half * 8, token = kpos & (kKvBlock - 1);
+                const uint8_t *kb = nullptr, *vb = nullptr;
+                if (kpos < sq.kv) {
+                    kb = kv_block_at(v, row_table, head, kpos);
+                    if (kb == nullptr) raise_error(v.err_flag, kErrBadPage);
+                }
+                if (vpos < sq.kv) vb = kv_block_at(v, row_table, head, vpos);
+                ks = vs = 0;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) kw[k] = vw[k] = make_uint4(0, 0, 0, 0);
+                vz[0] = vz[1] = make_uint4(0, 0, 0, 0);
+                if (kb != nullptr) {
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k)
+                        kw[k] = *reinterpret_cast<const uint4*>(kb + token * (D / 2) + k * 16);
+                    ks = reinterpret_cast<const uint32_t*>(kb + kv_k_scales(D))[token];
+                    vs = reinterpret_cast<const uint32_t*>(kb + kv_v_scales(D))[token];
+                }
+                if (vb != nullptr) {
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k)
+                        vw[k] = *reinterpret_cast<const uint4*>(vb + kv_v_codes(D) + (v_half & 1) * 4 * D + v_r * (D / 2) + k * 16);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        vz[k] = *reinterpret_cast<const uint4*>(vb + kv_v_scales(D) + (v_half & 1) * 32 + k * 16);
+                }
+            };
+            load(0);
+            for (int j = 0; j < count; ++j) {
+                const uint32_t it = stage_it + j, st = it & 1;
+                if (it >= 2) wait_phase(&s_empty[st], ((it >> 1) - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+                // columns' constants
+                {
+                    const float sk = f16_bits_to_f32(static_cast<uint16_t>(ks));
+                    if ((vs & 0xFFFFu) == 0) vs |= 1u;  // never stored, or nobody's: holds zeros whatever its scale
+                    const float sv = f16_bits_to_f32(static_cast<uint16_t>(vs));
+                    uint8_t* cc = cols + st * S::kCols;
+                    float* kl = reinterpret_cast<float*>(cc) + (tid >> 1) * 4 + (tid & 1);
+                    kl[0] = sk * fac;
+                    kl[2] = fast_log2(sv);
+                    // a NaN scale reaches the rows that see it through the exponent, and no other
+                    reinterpret_cast<float*>(cc + 1024)[tid] = sv != sv ? 0.0f : fast_rcp(sv);
+                }
+                const uint32_t kst = k_u32 + st * S::kK, vst = v_u32 + st * S::kV;
+                {
+                    const uint32_t z = ks >> 16, zz = z | z << 16;
+                    const uint32_t z1024 = 0x64006400u | zz, z64 = 0xD400D400u | zz << 4, z128 = 0x43004300u | zz;
+#pragma unroll
+                    for (int k = 0; k < D / 8; ++k) {
+                        const uint4 q4 = kw[k >> 2];
+                        const uint32_t w = (k & 3) == 0 ? q4.x : (k & 3) == 1 ? q4.y : (k & 3) == 2 ? q4.z : q4.w;
+                        uint32_t e0, e1, e2, e3;
+                        if constexpr (BF16) {
+                            e0 = bf2_sub((w & kNib0) | 0x43004300u, z128);
+                            e1 = bf2_sub(((w >> 4) & kNib0) | 0x43004300u, z128);
+                            e2 = bf2_sub(((w >> 8) & kNib0) | 0x43004300u, z128);
+                            e3 = bf2_sub(((w >> 12) & kNib0) | 0x43004300u, z128);
+                        } else {
+                            e0 = nib0_f16(w, z1024);
+                            e1 = nib1_f16(w, z64);
+                            e2 = nib0_f16(w >> 8, z1024);
+                            e3 = nib1_f16(w >> 8, z64);
+                        }
+                        st_shared_16(panel_at(kst + (k >> 3) * S::kPanel, tid, k & 7), e0, e1, e2, e3);
+                    }
+                }
+                {
+                    // Token pairs' zero points; then, for each word of a token, its eight channels as rows of V^T.
+                    uint32_t z1024[4], z64[4];
+                    const uint32_t zw[8] = {vz[0].x, vz[0].y, vz[0].z, vz[0].w, vz[1].x, vz[1].y, vz[1].z, vz[1].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t zz = __byte_perm(zw[2 * k], zw[2 * k + 1], 0x7632);
+                        z1024[k] = 0x64006400u | zz;
+                        z64[k] = 0xD400D400u | zz << 4;
+                    }
+#pragma unroll
+                    for (int w = 0; w < D / 64; ++w) {
+                        uint32_t t[8];  // word w of the eight tokens
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if constexpr (D == 128) {  // 16 bytes a pair: two words of each token
+                                t[2 * k] = w ? vw[k].y : vw[k].x;
+                                t[2 * k + 1] = w ? vw[k].w : vw[k].z;
+                            } else {  // 8 bytes a pair
+                                const uint4 u = vw[k >> 1];
+                                t[2 * k] = (k & 1) ? u.z : u.x;
+                                t[2 * k + 1] = (k & 1) ? u.w : u.y;
+                            }
+                        }
+#pragma unroll
+                        for (int hi = 0; hi < 2; ++hi) {
+                            uint32_t u[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) u[k] = __byte_perm(t[2 * k], t[2 * k + 1], hi ? 0x7632 : 0x5410);
+                            const int ch = v_r * (D / 8) + w * 8 + hi * 4;
+                            const uint32_t panel = vst + (v_half >> 3) * (D * 128);
+                            const int chunk = v_half & 7;
+                            st_shared_16(panel_at(panel, ch, chunk), nib0_f16(u[0], z1024[0]), nib0_f16(u[1], z1024[1]),
+                                         nib0_f16(u[2], z1024[2]), nib0_f16(u[3], z1024[3]));
+                            st_shared_16(panel_at(panel, ch + 1, chunk), nib1_f16(u[0], z64[0]), nib1_f16(u[1], z64[1]),
+                                         nib1_f16(u[2], z64[2]), nib1_f16(u[3], z64[3]));
+                            st_shared_16(panel_at(panel, ch + 2, chunk), nib0_f16(u[0] >> 8, z1024[0]), nib0_f16(u[1] >> 8, z1024[1]),
+                                         nib0_f16(u[2] >> 8, z1024[2]), nib0_f16(u[3] >> 8, z1024[3]));
+                            st_shared_16(panel_at(panel, ch + 3, chunk), nib1_f16(u[0] >> 8, z64[0]), nib1_f16(u[1] >> 8, z64[1]),
+                                         nib1_f16(u[2] >> 8, z64[2]), nib1_f16(u[3] >> 8, z64[3]));
+                        }
+                    }
+                }
+                fence_async_smem();
+                mbar_arrive(&s_full[st]);
+                if (j + 1 < count) load(j + 1);
+            }
+        } else if (lane == 0) {
+            // ---------------------------------------------------------- products
+            auto scores = [&](int i, uint32_t st) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t qd = smem_desc_k128(q_u32 + (i * kPanels + (k >> 2)) * S::kPanel + (k & 3) * 32);
+                    const uint64_t kd = smem_desc_k128(k_u32 + st * S::kK + (k >> 2) * S::kPanel + (k & 3) * 32);
+                    tc_mma_f16(tmem + i * 128, qd, kd, idesc_qk, k > 0);
+                }
+                tc_commit(&s_scores[i]);
+            };
+            wait_phase(&s_full[stage_it & 1], (stage_it >> 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+            tc_fence_after();
+            for (int i = 0; i < row_tiles; ++i) scores(i, stage_it & 1);
+            for (int j = 0; j < count; ++j) {
+                const uint32_t st = (stage_it + j) & 1;
+                for (int i = 0; i < row_tiles; ++i) {
+                    wait_phase(&s_probs[i], (tile_it[i] + j) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < kManyKeys / 16; ++k) {
+                        const uint64_t vd = smem_desc_k128(v_u32 + st * S::kV + (k >> 2) * (D * 128) + (k & 3) * 32);
+                        tc_mma_f16_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, vd, idesc_pv, j > 0 || k > 0);
+                    }
+                    tc_commit(&s_done[i]);
+                    if (i == row_tiles - 1) tc_commit(&s_empty[st]);
+                    if (j + 1 < count) {
+                        const uint32_t it = stage_it + j + 1;
+                        wait_phase(&s_full[it & 1], (it >> 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        wait_phase(&s_done[i], (tile_it[i] + j) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        tc_fence_after();
+                        scores(i, it & 1);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        stage_it += count;
+        tile_it[0] += count;
+        if (row_tiles > 1) tile_it[1] += count;
+        if (t0 == 0 && t1 < tiles) part = ManyPart{seq, head, row0, unit_at > range_begin ? 1 : 0, static_cast<int>((unit_at + tiles - 1) / per)};
+        at += count;
+        __syncthreads();
+        tc_fence_after();
+    }
+    if (threadIdx.x == 0) args.parts[blockIdx.x] = part;
+    // Every product has ended: each role waited for the last one of its tile.
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Adds the parts of a unit that spans CTAs: one CTA per (CTA it begins in,
+// eight rows), a warp a row.
+template <int D>
+__global__ void __launch_bounds__(kThreads) attn_q4_many_join_kernel(const ManyArgs args) {
+    constexpr int PER = D / 32;
+    griddep_wait();
+    griddep_launch_dependents();
+    const ManyPart part = args.parts[blockIdx.x];
+    if (part.last_cta < 0) return;
+    const AttnQ4Args& a = args.a;
+    int first, n, kv;
+    kv_seq(a.v, part.seq, &first, &n, &kv);
+    const int row = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (part.row0 + row >= static_cast<int64_t>(n) * args.group) return;
+    float m = -INFINITY, l = 0.0f, o[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) o[j] = 0.0f;
+    for (int p = blockIdx.x; p <= part.last_cta; ++p) {
+        const int64_t at = (p * 2LL + (p == static_cast<int>(blockIdx.x) ? part.place : 0)) * kManyRows + row;
+        const float2 ml = args.part_ml[at];
+        float x[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) x[j] = args.part_o[at * D + lane * PER + j];
+        const float big = fmaxf(m, ml.x), base = big == -INFINITY ? 0.0f : big;
+        const float f0 = fast_exp2(m - base), f1 = fast_exp2(ml.x - base);
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) o[j] = o[j] * f0 + x[j] * f1;
+        m = big;
+    }
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    const int tok = (part.row0 + row) / args.group, gh = part.row0 + row - tok * args.group;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        a.out[(first + tok) * a.ldo + (part.head * args.group + gh) * D + lane * PER + j] = narrow(o[j] * inv, a.dtype);
+}
+
 }  // namespace
 }  // namespace mrt
 
@@ -680,10 +1370,11 @@ namespace {
 
 // How a call runs, by its sizes alone.
 struct Plan {
-    int few;     // 8-row tiles of the few-rows kernel, 0: more rows than it takes
-    int split;   // its units may span CTAs
+    int few;     // 8-row tiles of the few-rows kernel, 0: the many-rows kernel
+    int split;   // units may span CTAs
     int grid;
-    size_t o_bytes, ml_bytes;
+    size_t o_bytes, ml_bytes, part_bytes;  // scratch, in this order
+    size_t bytes() const { return o_bytes + ml_bytes + part_bytes; }
 };
 
 constexpr int kSplitWarps = 4, kWholeWarps = 16;
@@ -691,7 +1382,14 @@ constexpr int kSplitWarps = 4, kWholeWarps = 16;
 Plan make_plan(const KvView& v, int64_t heads, int sms) {
     Plan p{};
     const int64_t rows = heads / v.kv_heads * std::max(v.max_q_len, 1);
-    if (rows > 32) return p;
+    if (rows > 32) {
+        p.split = 1;
+        p.grid = sms;
+        p.o_bytes = static_cast<size_t>(p.grid) * 2 * kManyRows * v.head_dim * 4;
+        p.ml_bytes = static_cast<size_t>(p.grid) * 2 * kManyRows * 8;
+        p.part_bytes = static_cast<size_t>(p.grid) * sizeof(ManyPart);
+        return p;
+    }
     p.few = static_cast<int>((rows + 7) / 8);
     // Few short units: one CTA of sixteen warps each and no join.
     const int64_t units = static_cast<int64_t>(v.seqs) * v.kv_heads;
@@ -743,6 +1441,16 @@ cudaError_t launch_few(const RowsArgs& r, int few, int rows, cudaStream_t s) {
     }
 }
 
+template <int D, bool BF16>
+cudaError_t launch_many(const ManyArgs& m, cudaStream_t s) {
+    constexpr int smem = ManyShape<D>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(attn_q4_many_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = launch_pdl(attn_q4_many_kernel<D, BF16>, dim3(m.grid), kManyThreads, smem, s, m);
+    if (e == cudaSuccess)
+        e = launch_pdl(attn_q4_many_join_kernel<D>, dim3(m.grid, kManyRows / (kThreads / 32)), kThreads, 0, s, m);
+    return e;
+}
+
 }  // namespace
 }  // namespace mrt
 
@@ -756,7 +1464,7 @@ extern "C" int mrt_kv_q4_attention_workspace(mrt_kv_q4 kv, const mrt_kv_batch* b
     int sms = 0;
     if ((rc = kv_bind(kv, &v, &sms)) != MRT_OK) return rc;
     const Plan p = make_plan(v, heads, sms);
-    *bytes = p.o_bytes + p.ml_bytes;
+    *bytes = p.bytes();
     return MRT_OK;
 }
 
@@ -776,7 +1484,7 @@ extern "C" int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int 
     if ((rc = kv_bind(kv, &a.v, &sms)) != MRT_OK) return rc;
     const Plan plan = make_plan(a.v, heads, sms);
     if (plan.o_bytes > 0) {
-        if (ws_dev == nullptr || ws_bytes < plan.o_bytes + plan.ml_bytes)
+        if (ws_dev == nullptr || ws_bytes < plan.bytes())
             return set_error(MRT_ERR_INVALID_ARG, "scratch is NULL or smaller than mrt_kv_q4_attention_workspace says");
         if ((reinterpret_cast<uintptr_t>(ws_dev) & 255) != 0)
             return set_error(MRT_ERR_INVALID_ARG, "scratch must be 256-byte aligned");
@@ -802,8 +1510,17 @@ extern "C" int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int 
         const int rows = r.group * std::max(a.v.max_q_len, 1);
         e = D == 128 ? launch_few<128>(r, plan.few, rows, s) : launch_few<64>(r, plan.few, rows, s);
     } else {
-        e = D == 128 ? launch_pdl(attn_q4_rows_kernel<4>, dim3(a.v.tokens), kThreads, 0, s, a)
-                     : launch_pdl(attn_q4_rows_kernel<2>, dim3(a.v.tokens), kThreads, 0, s, a);
+        ManyArgs m{};
+        m.a = a;
+        m.group = static_cast<int>(heads / kv->kv_heads);
+        m.grid = plan.grid;
+        m.part_o = static_cast<float*>(ws_dev);
+        m.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws_dev) + plan.o_bytes);
+        m.parts = reinterpret_cast<ManyPart*>(static_cast<uint8_t*>(ws_dev) + plan.o_bytes + plan.ml_bytes);
+        if (D == 128)
+            e = dtype == MRT_BF16 ? launch_many<128, true>(m, s) : launch_many<128, false>(m, s);
+        else
+            e = dtype == MRT_BF16 ? launch_many<64, true>(m, s) : launch_many<64, false>(m, s);
     }
     return e == cudaSuccess ? MRT_OK : cuda_error(e, "4-bit attention launch");
 }
