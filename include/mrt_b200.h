@@ -392,7 +392,7 @@ int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, const void* res
  * FP16 scale s and one zero point z: with lo = min(0, min x) and hi = max(0,
  * max x), s = max(fp16((hi - lo) / 15), 2^-24), z = rint(-lo / s), c =
  * rint(x / s) + z (both kept in 0..15); the row holds s (c - z).  A row with a
- * NaN or an infinity, or a range above 15 * 65504, reads back as NaN.  The
+ * NaN, or a magnitude above 65504 once rotated, reads back as NaN.  The
  * handle owns the pages (pages * page_tokens * kv_heads * (head_dim + 8)
  * bytes, zero at first); page_tokens is a multiple of 16.  rope_theta is that
  * of the position rotation (pairs i, i + head_dim / 2 turned by position *

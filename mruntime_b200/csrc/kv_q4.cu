@@ -42,6 +42,8 @@ int kv_view(mrt_kv_q4 kv, const mrt_kv_batch* b, KvView* out) {
     v.data = kv->data;
     v.pages = static_cast<int>(kv->pages);
     v.page_tokens = static_cast<int>(kv->page_tokens);
+    const int blocks = v.page_tokens / kKvBlock;
+    v.page_shift = (blocks & (blocks - 1)) == 0 ? __builtin_ctz(blocks) : -1;
     v.kv_heads = static_cast<int>(kv->kv_heads);
     v.head_dim = static_cast<int>(kv->head_dim);
     v.seqs = static_cast<int>(b->seqs);
@@ -118,12 +120,12 @@ template <int PER>
 __device__ __forceinline__ void store_row(uint8_t* block, int token, int lane, bool value, const float (&x)[PER]) {
     constexpr int D = PER * 32;
     float lo = 0.0f, hi = 0.0f;
-    bool odd = false;  // NaN or infinity
+    bool odd = false;  // NaN, infinity, or beyond FP16
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         lo = fminf(lo, x[j]);
         hi = fmaxf(hi, x[j]);
-        odd |= !(fabsf(x[j]) <= 3.402823466e38f);
+        odd |= !(fabsf(x[j]) <= 65504.0f);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -132,7 +134,6 @@ __device__ __forceinline__ void store_row(uint8_t* block, int token, int lane, b
     }
     odd = __any_sync(0xFFFFFFFFu, odd);
     uint16_t sb = f32_to_f16_bits(fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 5.9604644775390625e-8f));
-    if ((sb & 0x7C00u) == 0x7C00u) odd = true;
     const float inv = __fdiv_rn(1.0f, f16_bits_to_f32(sb));
     const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
     uint32_t zero = static_cast<uint32_t>(z);
@@ -300,6 +301,8 @@ extern "C" int mrt_kv_q4_create(int64_t pages, int64_t page_tokens, int64_t kv_h
         return set_error(MRT_ERR_SHAPE, "pages and kv_heads must be positive");
     if (page_tokens <= 0 || page_tokens % kKvBlock != 0 || page_tokens > (1 << 20))
         return set_error(MRT_ERR_SHAPE, "page_tokens must be a multiple of 16");
+    if (static_cast<double>(pages) * kv_heads * (page_tokens / kKvBlock) > 2147483647.0)
+        return set_error(MRT_ERR_SHAPE, "pages, heads and page_tokens are too large together");
     if (head_dim != 64 && head_dim != 128) return set_error(MRT_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
     if (!(rope_theta == 0.0f || (rope_theta >= 1.0f && rope_theta <= 3.4e38f)))
         return set_error(MRT_ERR_INVALID_ARG, "rope_theta must be 0 (no rotation) or >= 1");

@@ -54,21 +54,26 @@ struct KvView {
     uint8_t* data;
     int pages, page_tokens, kv_heads, head_dim;
     int seqs, tokens, max_q_len, max_kv_len, ld_table;
+    int page_shift;  // log2 of a page's blocks, or -1
     const int32_t* q_start;
     const int32_t* kv_len;
     const int32_t* table;
     int* err_flag;
 };
 
-// The block that holds position `pos` of a sequence whose table row is given,
-// or null (raising kErrBadPage) when the row has no such page.
-__device__ __forceinline__ uint8_t* kv_block_at(const KvView& v, const int32_t* row, int head, int pos) {
-    const int slot = pos / v.page_tokens;
+// Number in the pool of the block that holds position `pos` of a sequence whose
+// table row is given, or -1 when the row names no page of the cache there.
+__device__ __forceinline__ int kv_block_number(const KvView& v, const int32_t* row, int head, int pos) {
+    const int blocks = v.page_tokens / kKvBlock, block = pos / kKvBlock;
+    const int slot = v.page_shift >= 0 ? block >> v.page_shift : block / blocks;
     const int page = slot < v.ld_table ? row[slot] : -1;
-    if (page < 0 || page >= v.pages) return nullptr;
-    const int64_t blocks = v.page_tokens / kKvBlock;
-    return v.data + ((static_cast<int64_t>(page) * v.kv_heads + head) * blocks + (pos - slot * v.page_tokens) / kKvBlock) *
-                        kv_block_bytes(v.head_dim);
+    return page < 0 || page >= v.pages ? -1 : (page * v.kv_heads + head) * blocks + (block - slot * blocks);
+}
+
+// The block itself, or null.
+__device__ __forceinline__ uint8_t* kv_block_at(const KvView& v, const int32_t* row, int head, int pos) {
+    const int n = kv_block_number(v, row, head, pos);
+    return n < 0 ? nullptr : v.data + static_cast<int64_t>(n) * kv_block_bytes(v.head_dim);
 }
 
 // New tokens and held tokens of sequence b; false (raising the error) when

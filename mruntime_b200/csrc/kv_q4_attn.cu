@@ -32,17 +32,23 @@ __device__ __forceinline__ float widen(uint16_t h, int dtype) {
     return dtype == MRT_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
 }
 
-__device__ __forceinline__ uint16_t narrow(float f, int dtype) {
-    if (dtype == MRT_FP16) return f32_to_f16_bits(f);
-    return f != f ? static_cast<uint16_t>(0x7FC0) : f32_to_bf16_bits(f);
+// Two neighbouring outputs, rounded to nearest.
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, int dtype) {
+    if (dtype == MRT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Four neighbouring channels of an output row (any alignment of the row).
-__device__ __forceinline__ void store_out4(uint16_t* dst, const AttnQ4Args& a, float4 x, float inv) {
-    dst[0] = narrow(x.x * inv, a.dtype);
-    dst[1] = narrow(x.y * inv, a.dtype);
-    dst[2] = narrow(x.z * inv, a.dtype);
-    dst[3] = narrow(x.w * inv, a.dtype);
+__device__ __forceinline__ void store2(uint16_t* dst, uint32_t v) {
+    if ((reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
+        *reinterpret_cast<uint32_t*>(dst) = v;
+    } else {
+        dst[0] = static_cast<uint16_t>(v);
+        dst[1] = static_cast<uint16_t>(v >> 16);
+    }
 }
 
 // ------------------------------------------------------------------ few rows
@@ -87,22 +93,22 @@ __device__ __forceinline__ int seq_tiles(const KvView& v, int b) {
     return max(1, (kv + kTile - 1) / kTile);
 }
 
-// Sum over the block of one 64-bit number a thread (every thread gets it).
+// Sum over the block of one number a thread (every thread gets it).
 template <int W>
-__device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* s) {
+__device__ __forceinline__ int block_sum(int x, int* s) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
     __syncthreads();
-    int64_t t = 0;
-#pragma unroll
+    int t = 0;
+#pragma unroll 1
     for (int w = 0; w < W; ++w) t += s[w];
     return t;
 }
 
-__device__ __forceinline__ int64_t tiles_a_cta(int64_t total, int grid, int warps) {
-    const int64_t per = (total + grid - 1) / grid;
+__device__ __forceinline__ int tiles_a_cta(int total, int grid, int warps) {
+    const int per = (total + grid - 1) / grid;
     return per < warps ? warps : per;
 }
 
@@ -124,9 +130,8 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
     using S = RowsShape<D, NT, W>;
     constexpr int kWords = D / 32;  // words of a lane: K row part, and V channel stretch of two tokens
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t s_sum[W];
-    __shared__ int s_seq;
-    __shared__ int64_t s_at;
+    __shared__ int s_sum[W];
+    __shared__ int s_seq, s_at;
     __shared__ float s_fac[S::kRows], s_sumq[S::kRows];
     __shared__ int s_limit[S::kRows];
     __shared__ float s_m[W][S::kRows], s_l[W][S::kRows];
@@ -141,43 +146,44 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
     griddep_launch_dependents();
 
     // This CTA's stretch of the tiles, and the sequence it begins in.
-    int64_t mine = 0;
+    int mine = 0;
     for (int b = threadIdx.x; b < v.seqs; b += W * 32) {
         mine += seq_tiles(v, b);
         int f, n, kv;
         if (!kv_seq(v, b, &f, &n, &kv) && blockIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
     }
-    const int64_t total = block_sum<W>(mine, s_sum) * v.kv_heads;
-    int64_t at, end;
-    int seq;
-    int64_t seq_at;  // tile number at which the sequence begins
+    const int total = block_sum<W>(mine, s_sum) * v.kv_heads;
+    int at, end, seq;
+    int seq_at;  // tile number at which the sequence begins
     if (args.split) {
-        const int64_t per = tiles_a_cta(total, args.grid, W);
-        at = blockIdx.x * per;
-        end = min(total, at + per);
+        const int per = tiles_a_cta(total, args.grid, W);
+        at = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(blockIdx.x) * per));
+        end = min(total - at, per) + at;
         if (at >= end) return;
-        int64_t before = 0;
+        int before = 0;
         seq = -1;
         seq_at = 0;
         for (int b0 = 0; seq < 0; b0 += W * 32) {  // ends: at < total
             const int b = b0 + threadIdx.x;
-            const int64_t t = b < v.seqs ? static_cast<int64_t>(seq_tiles(v, b)) * v.kv_heads : 0;
-            int64_t incl = t;
+            const int t = b < v.seqs ? seq_tiles(v, b) * v.kv_heads : 0;
+            int incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t u = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                const int u = __shfl_up_sync(0xFFFFFFFFu, incl, o);
                 if (lane >= o) incl += u;
             }
             __syncthreads();
             if (threadIdx.x == 0) s_seq = -1;
             if (lane == 31) s_sum[warp] = incl;
             __syncthreads();
-            int64_t base = before;
+            int base = before;
+#pragma unroll 1
             for (int w = 0; w < warp; ++w) base += s_sum[w];
             if (at >= base + incl - t && at < base + incl) {
                 s_seq = b;
                 s_at = base + incl - t;
             }
+#pragma unroll 1
             for (int w = 0; w < W; ++w) before += s_sum[w];
             __syncthreads();
             seq = s_seq;
@@ -188,23 +194,23 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
         const int t = seq_tiles(v, seq);
         if (t == 0) return;
         seq_at = 0;
-        at = static_cast<int64_t>(blockIdx.x % v.kv_heads) * t;
+        at = static_cast<int>(blockIdx.x % v.kv_heads) * t;
         end = at + t;
     }
-    const int64_t range_begin = at;
+    const int range_begin = at;
 
     while (at < end) {
         // The next unit of the stretch: tiles [t0, t1) of (seq, head).
         int tiles = seq_tiles(v, seq);
-        while (at >= seq_at + static_cast<int64_t>(tiles) * v.kv_heads) {
-            seq_at += static_cast<int64_t>(tiles) * v.kv_heads;
+        while (at >= seq_at + tiles * v.kv_heads) {
+            seq_at += tiles * v.kv_heads;
             ++seq;
             tiles = seq_tiles(v, seq);
         }
-        const int head = static_cast<int>((at - seq_at) / tiles);
-        const int64_t unit_at = seq_at + static_cast<int64_t>(head) * tiles;
-        const int t0 = static_cast<int>(at - unit_at);
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - at)));
+        const int head = (at - seq_at) / tiles;
+        const int unit_at = seq_at + head * tiles;
+        const int t0 = at - unit_at;
+        const int t1 = min(tiles, t0 + (end - at));
         int first, n, kv;
         kv_seq(v, seq, &first, &n, &kv);
         const int rows = n * args.group;  // <= 8 NT
@@ -511,9 +517,11 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
                 acc.w = fmaf(x.w, f, acc.w);
             }
             if (whole) {
-                const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+                const float inv = sum == 0.0f ? 0.0f : fast_rcp(sum);
                 const int qi = row / args.group, g = row - qi * args.group;
-                store_out4(a.out + (first + qi) * a.ldo + (head * args.group + g) * D + ch, a, acc, inv);
+                uint16_t* dst = a.out + (first + qi) * a.ldo + (head * args.group + g) * D + ch;
+                store2(dst, narrow2(acc.x * inv, acc.y * inv, a.dtype));
+                store2(dst + 2, narrow2(acc.z * inv, acc.w * inv, a.dtype));
             } else {
                 *reinterpret_cast<float4*>(args.part_o + (slot * S::kRows + row) * D + ch) = acc;
                 if (ch == 0) args.part_ml[slot * S::kRows + row] = make_float2(big, sum);
@@ -529,7 +537,7 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
 template <int D, int NT, int W>
 __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const RowsArgs args) {
     constexpr int kRows = NT * 8, PER = D / 32;
-    __shared__ int64_t s_sum[kThreads / 32];
+    __shared__ int s_sum[kThreads / 32];
     __shared__ float s_m[kThreads / 32], s_l[kThreads / 32];
     __shared__ float s_o[kThreads / 32][D];
     griddep_wait();
@@ -541,22 +549,22 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const RowsArgs a
     const int tiles = seq_tiles(v, seq);
     int first, n, kv;
     if (tiles == 0 || !kv_seq(v, seq, &first, &n, &kv) || row >= n * args.group) return;
-    int64_t all = 0, before = 0;
+    int all = 0, before = 0;
     for (int b = threadIdx.x; b < v.seqs; b += kThreads) {
         const int t = seq_tiles(v, b);
         all += t;
         if (b < seq) before += t;
     }
-    const int64_t total = block_sum<kThreads / 32>(all, s_sum) * v.kv_heads;
-    const int64_t unit_at = block_sum<kThreads / 32>(before, s_sum) * v.kv_heads + static_cast<int64_t>(head) * tiles;
-    const int64_t per = tiles_a_cta(total, args.grid, W);
-    const int64_t c0 = unit_at / per, c1 = (unit_at + tiles - 1) / per;
+    const int total = block_sum<kThreads / 32>(all, s_sum) * v.kv_heads;
+    const int unit_at = block_sum<kThreads / 32>(before, s_sum) * v.kv_heads + head * tiles;
+    const int per = tiles_a_cta(total, args.grid, W);
+    const int c0 = unit_at / per, c1 = (unit_at + tiles - 1) / per;
     if (c0 == c1) return;  // that CTA stored the output
     float m = -INFINITY, l = 0.0f, o[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) o[j] = 0.0f;
-    for (int64_t p = c0 + warp; p <= c1; p += kThreads / 32) {
-        const int64_t at = (p * 2 + (unit_at > p * per ? 1 : 0)) * kRows + row;
+    for (int p = c0 + warp; p <= c1; p += kThreads / 32) {
+        const int64_t at = (p * 2LL + (unit_at > p * per ? 1 : 0)) * kRows + row;
         const float2 ml = args.part_ml[at];
         float x[PER];
 #pragma unroll
@@ -585,9 +593,10 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const RowsArgs a
             sum = fmaf(s_l[w], f, sum);
             acc = fmaf(s_o[w][threadIdx.x], f, acc);
         }
-        const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+        const float inv = sum == 0.0f ? 0.0f : fast_rcp(sum);
         const int qi = row / args.group, g = row - qi * args.group;
-        a.out[(first + qi) * a.ldo + (head * args.group + g) * D + threadIdx.x] = narrow(acc * inv, a.dtype);
+        a.out[(first + qi) * a.ldo + (head * args.group + g) * D + threadIdx.x] =
+            static_cast<uint16_t>(narrow2(acc * inv, 0.0f, a.dtype));
     }
 }
 
@@ -597,27 +606,6 @@ __global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const RowsArgs a
 // of the warp gets, of every eight 32-bit columns, columns 2c and 2c + 1 of
 // rows r and r + 8.  (A thread then meets a quarter of the columns instead of
 // all of them, so what belongs to a column is loaded a quarter as often.)
-__device__ __forceinline__ void tmem_ld_frag128(uint32_t taddr, uint32_t (&r)[64]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x16.b32 {"
-        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, "
-        "%40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, "
-        "%59, %60, %61, %62, %63"
-        "}, [%64];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
-          "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]),
-          "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]),
-          "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]),
-          "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]),
-          "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 __device__ __forceinline__ void tmem_ld_frag64(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x8.b32 {"
@@ -633,44 +621,70 @@ __device__ __forceinline__ void tmem_ld_frag64(uint32_t taddr, uint32_t (&r)[32]
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_st_frag64(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], {"
-        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15"
+        "}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_st_frag32(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16"
         "};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
-// 64 columns of 32 bits, one register a column and row: lane (r, c) holds, of
+// 32 columns of 32 bits, one register a column and row: lane (r, c) holds, of
 // every four columns, column c of rows r and r + 8.
-__device__ __forceinline__ void tmem_st_pairs64(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st_pairs32(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {"
-        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32"
+        "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {"
+        "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16"
         "};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[tmem] (+)= A[tmem] * B[smem]^T.
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
+// The products take descriptors by their low words (address, leading offset);
+// the high word is the same for every panel here, so a step along K is one
+// 32-bit addition and nothing is worth keeping in registers.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;  // stride, version, swizzle (smem_desc_k128)
+
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr) { return (smem_addr & 0x3FFFFu) >> 4 | 1u << 16; }
+
+// D[tmem] (+)= A[smem] * B[smem]^T.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
+                                          uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+        : "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]^T.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
         : "memory");
 }
 
@@ -679,44 +693,66 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, 
 // waiting (every access stays in bounds whatever was computed).  Unlike
 // mbar_wait it does not look at the device's error flag: a bad page of one
 // sequence must not end another's waits.
-__device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
-    if (mbar_try_wait(bar, parity)) return;
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return;
-        if ((it & 63u) == 0) {
-            if (*gave_up) return;
-            if (globaltimer_ns() - t0 > kWaitLimitNs) {
-                *gave_up = 1;
-                raise_error(flag, code);
-                return;
-            }
+__device__ __forceinline__ void wait_phase_slow(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
+        if ((it & 255u) != 0) continue;  // the clock is far away: not read in a wait that ends soon
+        if (*gave_up) return;
+        if (t0 == 0) t0 = globaltimer_ns();
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            *gave_up = 1;
+            raise_error(flag, code);
+            return;
         }
     }
+}
+
+__device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
+    if (!mbar_try_wait(bar, parity)) wait_phase_slow(bar, parity, gave_up, flag, code);
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Many rows (prompts, chunks of prompts): tcgen05 flash attention.  A CTA
 // takes 256 rows of a (sequence, kv head) -- new tokens times the query heads
-// that share it -- as two tiles of 128, and keys 128 at a time:
+// that share it -- as two tiles of 128, and keys 64 at a time:
 //
-//   warps 0-3, 4-7  softmax of tile 0, 1: S from TMEM, P' back into its place
-//   warps 8-11      K and V codes from the pages to 16-bit integers c - z
-//                   (exact) in the tensor cores' swizzled layout
-//   warp 12         the products: S_i = Q_i K^T, O_i += P'_i V (A from TMEM)
+//   warps 0-7, 8-15  softmax of tile 0, 1, sixteen rows a warp: S from TMEM,
+//                    P back into its place
+//   warps 16-23      codes from the pages into the tensor cores' swizzled
+//                    layout, K as the integers c - z (exact), V as values
+//                    s (c - z) rounded to FP16; four warps the even key tiles,
+//                    four the odd ones
+//   warps 24, 25     the products of tile 0, 1: S_i = Q_i K^T, O_i += P_i V
+//                    (A from TMEM)
+//   warps 26, 27     Q into its panels
 //
-// so that one tile's softmax runs beside the other's products.  Scales stay
-// out of the operands: a key's multiplies its column of S, a value's goes into
-// the exponent, as in the few-rows kernel.  The running maximum m is moved only
-// when a row exceeds it by 2^8 (P' then still fits FP16 with all its bits), so
-// O in TMEM is hardly ever rescaled.  TMEM: S_0, S_1 (P' in their first half),
-// O_0, O_1.
+// Each role walks the CTA's units by itself and meets the others only at
+// mbarriers, and units follow one another without a stop.  TMEM: two S (P in
+// its first half) for each row tile, O_0, O_1: the scores of the next keys are
+// there while the softmax works on these, so neither waits for the other's
+// whole chain (with 128 keys and one S a tile, softmax 4000 and products 2600
+// cycles alternated).
+//
+// A key's scale multiplies its column of S, so scores are as exact as FP32; a
+// value's goes into the operand, at the price of one more rounding (2^-11 of
+// each value, independent from token to token like that of P, and averaged
+// with it), because every number that a column needs in the softmax is a
+// shared-memory read for every pair of rows, and shared memory is what bounds
+// this kernel (Q and K for S, V for O, the codes' stores, the columns'
+// scales); with the value's scale in the exponent, as in the few-rows kernel,
+// a column needed three.  The running maximum m is moved only when a row
+// exceeds it by 2^8 (P then still fits FP16 with all its bits), so O in TMEM is
+// hardly ever rescaled.  All loops are short: with the softmax unrolled over
+// its rows the kernel had 148 KB of code and every step of every role waited
+// for its instructions.
 //
 // Units' key tiles are dealt to the CTAs in equal contiguous stretches, as in
 // the few-rows kernel, parts of units that span CTAs joined from scratch.
-constexpr int kManyRows = 256, kManyKeys = 128;
-constexpr int kManyThreads = 13 * 32;
+constexpr int kManyRows = 256, kManyKeys = 64;
+constexpr int kSoftmaxWarps = 16, kCodesWarps = 8, kManyWarps = kSoftmaxWarps + kCodesWarps + 4;
+constexpr int kManyThreads = kManyWarps * 32;
+constexpr int kLoaders = 64;  // threads that bring Q
 
 struct ManyPart {  // a unit that begins in a CTA's stretch and goes on
     int seq, head, row0;
@@ -732,18 +768,34 @@ struct ManyArgs {
     ManyPart* parts;   // [grid]
 };
 
+// Key tiles of a sequence's row tiles.  Row tile x < count - 1 ends with token
+// (256 x + 255) / group, and causal rows see keys up to themselves.  (The host
+// has checked that rows and tile numbers fit in 31 bits.)
+struct ManySeq {
+    int first, n, kv, group, causal;
+    int count;  // row tiles, 0: nothing to do
+    __device__ __forceinline__ int past() const { return max(kv - n, 0); }
+    __device__ __forceinline__ int tiles(int x) const {
+        if (!causal) return max(1, (kv + kManyKeys - 1) / kManyKeys);
+        const int last = min(n - 1, (kManyRows * x + kManyRows - 1) / group);
+        return (past() + last) / kManyKeys + 1;
+    }
+};
+
 // sum_{i < n} floor((a i + b) / m), all >= 0: the lattice points under a line,
 // counted by exchanging the axes until the line is flat.
-__device__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+__device__ __noinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
     int64_t sum = 0;
+#pragma unroll 1
     while (n > 0) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
+        const int64_t qa = a / m, qb = b / m;
+        sum += n * (n - 1) / 2 * qa + n * qb;
+        a -= qa * m;
+        b -= qb * m;
         const int64_t top = a * n + b;
         if (top < m) break;
         n = top / m;
-        b = top % m;
+        b = top - n * m;
         const int64_t t = m;
         m = a;
         a = t;
@@ -751,43 +803,34 @@ __device__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
     return sum;
 }
 
-// Key tiles of a sequence's row tiles.  Row tile x < count - 1 ends with token
-// (256 x + 255) / group, and causal rows see keys up to themselves.
-struct ManySeq {
-    int first, n, kv, group, causal;
-    int count;  // row tiles, 0: nothing to do
-    __device__ __forceinline__ int64_t past() const { return max(kv - n, 0); }
-    __device__ __forceinline__ int tiles(int x) const {
-        if (!causal) return max(1, (kv + kManyKeys - 1) / kManyKeys);
-        const int64_t last = min(static_cast<int64_t>(n) - 1, (static_cast<int64_t>(kManyRows) * x + kManyRows - 1) / group);
-        return static_cast<int>((past() + last) / kManyKeys) + 1;
-    }
-    // of row tiles 0 .. x - 1
-    __device__ __forceinline__ int64_t before(int x) const {
-        if (!causal) return static_cast<int64_t>(x) * tiles(0);
-        const int y = min(x, count - 1);
-        int64_t t = y + floor_sum(y, static_cast<int64_t>(kManyKeys) * group, kManyRows, kManyRows - 1 + past() * group);
-        if (x == count) t += tiles(count - 1);
-        return t;
-    }
-};
+// Key tiles of row tiles 0 .. x - 1.
+__device__ __forceinline__ int many_before(const ManySeq& s, int x) {
+    if (x == 0) return 0;
+    if (!s.causal) return x * s.tiles(0);
+    const int y = min(x, s.count - 1);
+    int t = y + static_cast<int>(floor_sum(y, static_cast<int64_t>(kManyKeys) * s.group, kManyRows,
+                                           kManyRows - 1 + static_cast<int64_t>(s.past()) * s.group));
+    if (x == s.count) t += s.tiles(s.count - 1);
+    return t;
+}
 
 __device__ __forceinline__ bool many_seq(const ManyArgs& g, int b, ManySeq* s) {
     const bool ok = kv_seq(g.a.v, b, &s->first, &s->n, &s->kv);
     s->group = g.group;
     s->causal = g.a.causal;
-    s->count = ok ? static_cast<int>((static_cast<int64_t>(s->n) * g.group + kManyRows - 1) / kManyRows) : 0;
+    s->count = ok ? (s->n * g.group + kManyRows - 1) / kManyRows : 0;
     return ok;
 }
 
 template <int D>
 struct ManyShape {
-    static constexpr int kPanel = 128 * 128;            // 128 rows of 64 16-bit columns
+    static constexpr int kPanel = 128 * 128;                // Q: 128 rows of 64 16-bit columns
     static constexpr int kQ = 2 * (D / 64) * kPanel;
-    static constexpr int kK = (D / 64) * kPanel;        // a stage
-    static constexpr int kV = 2 * D * 128;              // V^T: two panels (64 keys) of D rows
-    static constexpr int kCols = 64 * 16 + 64 * 8;      // (ks, ks, lv, lv), (rs, rs) of each column pair
-    static constexpr int kStages = 2;
+    static constexpr int kKPanel = kManyKeys * 128;         // K: 64 rows of 64 channels
+    static constexpr int kK = (D / 64) * kKPanel;           // a stage
+    static constexpr int kV = D * 128;                      // V^T: D rows of 64 keys
+    static constexpr int kColsRow = 80, kCols = 4 * kColsRow;  // [c][k]: scales of columns 8k + 2c, + 1; rows in different banks
+    static constexpr int kStages = 4;
     static constexpr int kBytes = 1024 + kQ + kStages * (kK + kV + kCols);
 };
 
@@ -805,6 +848,11 @@ __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
     const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
                               *reinterpret_cast<const __half2*>(&c));
@@ -816,6 +864,33 @@ __device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Two FP32 values in one 64-bit register pair.
+__device__ __forceinline__ uint64_t pair2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) { return pair2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float low2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+
+__device__ __forceinline__ uint64_t mask2(uint64_t v, bool lo, bool hi) {
+    return pair2(lo ? -INFINITY : low2(v), hi ? -INFINITY : high2(v));
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 constexpr uint32_t kSixteenth = 0x2C002C00u;  // FP16 1/16 twice
 
 // Codes at bits 0-3 / 4-7 of each half less the zero points, as FP16: z1024 =
@@ -825,15 +900,52 @@ __device__ __forceinline__ uint32_t nib1_f16(uint32_t w, uint32_t z64) {
     return h2_fma((w & kNib1) | 0x64006400u, kSixteenth, z64);
 }
 
+// A CTA's stretch of the key tiles, unit by unit.
+struct ManyWalk {
+    int at, end, begin;    // tile numbers: next, end and begin of the stretch
+    int unit_at;           // where the unit begins
+    ManySeq sq;
+    int seq, head, x;      // the unit: sequence, kv head, row tile
+    int tiles, t0, count;  // its key tiles; the stretch has [t0, t0 + count) of them
+    int row0, rows;        // its first row, its rows
+
+    __device__ __forceinline__ bool next(const ManyArgs& g) {
+        if (at >= end) return false;
+        tiles = sq.tiles(x);
+        if (at >= unit_at + tiles) {
+            unit_at += tiles;
+            if (++x == sq.count) {
+                x = 0;
+                if (++head == g.a.v.kv_heads) {
+                    head = 0;
+                    do many_seq(g, ++seq, &sq);
+                    while (sq.count == 0);
+                }
+            }
+            tiles = sq.tiles(x);
+        }
+        t0 = at - unit_at;
+        count = min(tiles - t0, end - at);
+        row0 = x * kManyRows;
+        rows = min(kManyRows, sq.n * g.group - row0);
+        at += count;
+        return true;
+    }
+    __device__ __forceinline__ int row_tiles() const { return rows > 128 ? 2 : 1; }
+    __device__ __forceinline__ int place() const { return unit_at > begin ? 1 : 0; }  // where its part goes
+};
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const ManyArgs args) {
     using S = ManyShape<D>;
-    constexpr int kPanels = D / 64;
+    constexpr int kPanels = D / 64, dtype = BF16 ? MRT_BF16 : MRT_FP16;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_full[2], s_empty[2], s_scores[2], s_probs[2], s_done[2];
+    // s_full, s_empty: a stage of K, V and column scales.  Per row tile and S:
+    // s_scores: S; s_probs: P; s_done: the product that used it.  s_free: O has
+    // been read.  s_q, s_q_free: Q.
+    __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_scores[2][2], s_probs[2][2], s_done[2][2], s_free[2], s_q, s_q_free;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_gave_up, s_seq;
-    __shared__ int64_t s_sum[13], s_at;
+    __shared__ int s_gave_up, s_seq, s_at, s_sum[kManyWarps];
     uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     const uint32_t q_u32 = smem_u32(smem), k_u32 = q_u32 + S::kQ, v_u32 = k_u32 + S::kStages * S::kK;
     uint8_t* cols = smem + S::kQ + S::kStages * (S::kK + S::kV);
@@ -842,17 +954,24 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < S::kStages; ++i) {
             mbar_init(&s_full[i], 128);
-            mbar_init(&s_empty[i], 1);
-            mbar_init(&s_scores[i], 1);
-            mbar_init(&s_probs[i], 4);
-            mbar_init(&s_done[i], 1);
+            mbar_init(&s_empty[i], 2);
         }
+        for (int i = 0; i < 2; ++i) {
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&s_scores[i][b], 1);
+                mbar_init(&s_probs[i][b], 8);
+                mbar_init(&s_done[i][b], 1);
+            }
+            mbar_init(&s_free[i], 8);
+        }
+        mbar_init(&s_q, kLoaders);
+        mbar_init(&s_q_free, 2);
         s_gave_up = 0;
         fence_barrier_init();
     }
-    if (warp == 12) {
+    if (warp == kSoftmaxWarps + kCodesWarps) {
         tmem_alloc(&s_tmem, 512);
         tmem_relinquish();
     }
@@ -864,105 +983,420 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     griddep_wait();
 
     // This CTA's stretch, and the unit it begins in.
-    int64_t mine = 0;
+    int mine = 0;
     for (int b = threadIdx.x; b < v.seqs; b += kManyThreads) {
         ManySeq q;
         if (!many_seq(args, b, &q) && blockIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
-        if (q.count > 0) mine += q.before(q.count);
+        mine += many_before(q, q.count);
     }
-    const int64_t total = block_sum<13>(mine, s_sum) * v.kv_heads;
-    const int64_t per = (total + args.grid - 1) / args.grid;
-    int64_t at = blockIdx.x * per;
-    const int64_t end = min(total, at + per), range_begin = at;
-    ManySeq sq;
-    int seq = -1, head = 0, x = 0;
-    int64_t unit_at = 0;
-    ManyPart part{0, 0, 0, 0, -1};
-    if (at < end) {
-        int64_t before = 0;
-        for (int b0 = 0; seq < 0; b0 += kManyThreads) {
+    const int total = block_sum<kManyWarps>(mine, s_sum) * v.kv_heads;
+    const int per = (total + args.grid - 1) / args.grid;
+    ManyWalk u;
+    u.at = u.begin = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(blockIdx.x) * per));
+    u.end = u.at + min(total - u.at, per);
+    u.seq = -1;
+    u.head = u.x = u.unit_at = 0;
+    if (u.at < u.end) {
+        int before = 0;
+#pragma unroll 1
+        for (int b0 = 0; u.seq < 0; b0 += kManyThreads) {  // ends: u.at < total
             const int b = b0 + threadIdx.x;
-            int64_t t = 0;
+            int t = 0;
             if (b < v.seqs) {
                 ManySeq q;
                 many_seq(args, b, &q);
-                if (q.count > 0) t = q.before(q.count) * v.kv_heads;
+                t = many_before(q, q.count) * v.kv_heads;
             }
-            int64_t incl = t;
+            int incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t u = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                if (lane >= o) incl += u;
+                const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                if (lane >= o) incl += up;
             }
             __syncthreads();
             if (threadIdx.x == 0) s_seq = -1;
             if (lane == 31) s_sum[warp] = incl;
             __syncthreads();
-            int64_t base = before;
-            for (int w = 0; w < warp; ++w) base += s_sum[w];
-            if (at >= base + incl - t && at < base + incl) {
+            int base = before;
+#pragma unroll 1
+            for (int w = 0; w < kManyWarps; ++w) {
+                if (w == warp) base = before;
+                before += s_sum[w];
+            }
+            if (u.at >= base + incl - t && u.at < base + incl) {
                 s_seq = b;
                 s_at = base + incl - t;
             }
-            for (int w = 0; w < 13; ++w) before += s_sum[w];
             __syncthreads();
-            seq = s_seq;
-            unit_at = s_at;
+            u.seq = s_seq;
+            u.unit_at = s_at;
         }
-        many_seq(args, seq, &sq);
-        const int64_t a_head = sq.before(sq.count);
-        head = static_cast<int>((at - unit_at) / a_head);
-        unit_at += head * a_head;
-        const int64_t off = at - unit_at;
-        int lo = 0, span = sq.count;  // the row tile lies in [lo, lo + span)
+        many_seq(args, u.seq, &u.sq);
+        const int a_head = many_before(u.sq, u.sq.count);
+        u.head = (u.at - u.unit_at) / a_head;
+        u.unit_at += u.head * a_head;
+        const int off = u.at - u.unit_at;
+        int span = u.sq.count;  // the row tile lies in [x, x + span)
+#pragma unroll 1
         while (span > 1) {
             const int step = (span + kManyThreads - 1) / kManyThreads;
-            const int mid = lo + threadIdx.x * step;
-            const int n = __syncthreads_count(mid < lo + span && sq.before(mid) <= off);
-            const int next = lo + (n - 1) * step;
-            span = min(step, lo + span - next);
-            lo = next;
+            const int mid = u.x + threadIdx.x * step;
+            const int n = __syncthreads_count(mid < u.x + span && many_before(u.sq, min(mid, u.sq.count)) <= off);
+            const int next = u.x + (n - 1) * step;
+            span = min(step, u.x + span - next);
+            u.x = next;
         }
-        x = lo;
-        unit_at += sq.before(x);
+        u.unit_at += many_before(u.sq, u.x);
     }
+    // Key tiles so far: of the CTA, of the role's row tile.
+    uint32_t stage_it = 0, tile_it = 0;
 
-    uint32_t stage_it = 0, tile_it[2] = {0, 0};  // key tiles so far: of the CTA, of each row tile
-    const uint32_t idesc_qk = idesc_f16_f32(128, kManyKeys) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
-    const uint32_t idesc_pv = idesc_f16_f32(128, D);
-    while (at < end) {
-        int tiles = sq.tiles(x);
-        if (at >= unit_at + tiles) {  // the next unit
-            unit_at += tiles;
-            if (++x == sq.count) {
-                x = 0;
-                if (++head == v.kv_heads) {
-                    head = 0;
-                    do {
-                        ++seq;
-                        many_seq(args, seq, &sq);
-                    } while (sq.count == 0);
+    if (warp < kSoftmaxWarps) {
+        // -------------------------------------------------------------- softmax
+        const int i = warp >> 3, r = lane >> 2, c = lane & 3;
+        const int row_in = (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + r;  // this lane's rows of the tile: it and + 8
+        const uint32_t lanes = static_cast<uint32_t>(row_in - r) << 16;
+        const uint32_t t_rows = tmem + i * 128 + lanes, t_o = tmem + 256 + i * D + lanes;
+        for (; u.next(args); stage_it += u.count) {
+            if (i >= u.row_tiles()) continue;
+            float m[2];
+            uint64_t l[2];  // sums over even and over odd columns
+            int limit[2], limit_min = 0x7FFFFFFF;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int row = i * 128 + row_in + b * 8;
+                m[b] = -INFINITY;
+                l[b] = 0;
+                limit[b] = 0;
+                if (row < u.rows) {
+                    limit[b] = a.causal ? u.sq.kv - u.sq.n + (u.row0 + row) / args.group + 1 : u.sq.kv;
+                    limit_min = min(limit_min, limit[b]);
                 }
             }
-            tiles = sq.tiles(x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
+#pragma unroll 1
+            for (int j = 0; j < u.count; ++j) {
+                const uint32_t it = stage_it + j, st = it % S::kStages, t = tile_it + j, buf = t & 1;
+                const uint32_t t_s = t_rows + buf * kManyKeys;
+                const int pos0 = (u.t0 + j) * kManyKeys;
+                wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                wait_phase(&s_scores[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                __syncwarp();
+                tc_fence_after();
+                // y = scale log2(e) s_k S: [column pair][row]
+                uint64_t y[16];
+                {
+                    uint32_t s[32];
+                    tmem_ld_frag64(t_s, s);
+                    const uint8_t* kl = cols + st * S::kCols + c * S::kColsRow;
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(kl + k * 8);
+                        y[k * 2] = mul2(pair2(s[k * 4], s[k * 4 + 1]), w.x);
+                        y[k * 2 + 1] = mul2(pair2(s[k * 4 + 2], s[k * 4 + 3]), w.x);
+                        y[k * 2 + 2] = mul2(pair2(s[k * 4 + 4], s[k * 4 + 5]), w.y);
+                        y[k * 2 + 3] = mul2(pair2(s[k * 4 + 6], s[k * 4 + 7]), w.y);
+                    }
+                }
+                if (pos0 + kManyKeys > limit_min) {
+                    const int left0 = limit[0] - pos0 - c * 2, left1 = limit[1] - pos0 - c * 2;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        y[k * 2] = mask2(y[k * 2], k * 8 >= left0, k * 8 + 1 >= left0);
+                        y[k * 2 + 1] = mask2(y[k * 2 + 1], k * 8 >= left1, k * 8 + 1 >= left1);
+                    }
+                }
+                float big[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < 16; ++k) big[k & 1] = fmaxf(big[k & 1], fmaxf(low2(y[k]), high2(y[k])));
+                bool grow = false;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
+                    big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 2));
+                    grow |= big[b] > m[b] + 8.0f;  // from -inf: any
+                }
+                if (__any_sync(0xFFFFFFFFu, grow)) {
+                    float fix[2];
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const float to = fmaxf(m[b], big[b]);
+                        fix[b] = to == -INFINITY ? 1.0f : fast_exp2(m[b] - to);
+                        m[b] = to;
+                        l[b] = mul2(l[b], pair2(fix[b], fix[b]));
+                    }
+                    if (j > 0) {  // O, once the last product into it has ended
+                        wait_phase(&s_done[i][buf ^ 1], ((t - 1) >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int ch = 0; ch < D; ch += 32) {
+                            uint32_t o[16];
+                            tmem_ld_frag32(t_o + ch, o);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fix[(k >> 1) & 1]);
+                            tmem_st_frag32(t_o + ch, o);
+                        }
+                    }
+                }
+                const float n0 = m[0] == -INFINITY ? 0.0f : -m[0], n1 = m[1] == -INFINITY ? 0.0f : -m[1];
+                const uint64_t less[2] = {pair2(n0, n0), pair2(n1, n1)};
+                uint32_t p[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const uint64_t e = add2(y[k], less[k & 1]);
+                    const float p0 = fast_exp2(low2(e)), p1 = fast_exp2(high2(e));
+                    l[k & 1] = add2(l[k & 1], pair2(p0, p1));
+                    const __half2 hp = __floats2half2_rn(p0, p1);
+                    p[k] = *reinterpret_cast<const uint32_t*>(&hp);
+                }
+                tmem_st_pairs32(t_s, p);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_probs[i][buf]);
+            }
+            // The output, or the unit's part of it.
+            const uint32_t last = tile_it + u.count - 1;
+            wait_phase(&s_done[i][last & 1], (last >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+            __syncwarp();
+            tc_fence_after();
+            const bool whole = u.t0 == 0 && u.count == u.tiles;
+            const int64_t slot = blockIdx.x * 2LL + u.place();
+            float sums[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                sums[b] = low2(l[b]) + high2(l[b]);
+                sums[b] += __shfl_xor_sync(0xFFFFFFFFu, sums[b], 1);
+                sums[b] += __shfl_xor_sync(0xFFFFFFFFu, sums[b], 2);
+            }
+#pragma unroll 1
+            for (int ch = 0; ch < D; ch += 32) {
+                uint32_t o[16];
+                __syncwarp();
+                tmem_ld_frag32(t_o + ch, o);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int row = i * 128 + row_in + b * 8;
+                    if (row >= u.rows) continue;
+                    if (whole) {
+                        const float inv = sums[b] == 0.0f ? 0.0f : fast_rcp(sums[b]);
+                        const int tok = (u.row0 + row) / args.group, gh = u.row0 + row - tok * args.group;
+                        uint16_t* dst = a.out + (u.sq.first + tok) * a.ldo + (u.head * args.group + gh) * D + ch + c * 2;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            store2(dst + k * 8, narrow2(__uint_as_float(o[k * 4 + b * 2]) * inv,
+                                                        __uint_as_float(o[k * 4 + b * 2 + 1]) * inv, dtype));
+                    } else {
+                        float* dst = args.part_o + (slot * kManyRows + row) * D + ch + c * 2;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<float2*>(dst + k * 8) =
+                                make_float2(__uint_as_float(o[k * 4 + b * 2]), __uint_as_float(o[k * 4 + b * 2 + 1]));
+                        if (ch == 0 && c == 0) args.part_ml[slot * kManyRows + row] = make_float2(m[b], sums[b]);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[i]);
+            tile_it += u.count;
         }
-        const int t0 = static_cast<int>(at - unit_at);
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - at)));
-        const int row0 = x * kManyRows;
-        const int64_t all_rows = static_cast<int64_t>(sq.n) * args.group;
-        const int rows = static_cast<int>(min(static_cast<int64_t>(kManyRows), all_rows - row0));
-        const int row_tiles = rows > 128 ? 2 : 1;
-        const int count = t1 - t0;
-
-        // Q, as it is, into its panels.
-        {
-            const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.ldq & 7) == 0;
-            for (int i = threadIdx.x; i < row_tiles * 128 * (D / 8); i += kManyThreads) {
-                const int row = i / (D / 8), ch = i - row * (D / 8);
+    } else if (warp < kSoftmaxWarps + kCodesWarps) {
+        // -------------------------------------------------------------- codes to operands
+        // A group's first two warps take K, a token a lane; the others V, a lane eight
+        // tokens (a half block) of a stretch of D / 8 channels: eight neighbouring lanes
+        // write eight different 16-byte columns of V^T.
+        const int group = (warp >> 2) & 1;
+        const bool is_k = (warp & 2) == 0;
+        const int token = (warp & 1) * 32 + lane;
+        const int v_half = lane & 7, v_r = (warp & 1) * 4 + (lane >> 3);
+        const int block_in = is_k ? token >> 4 : v_half >> 1;
+        const int offset = is_k ? (token & 15) * (D / 2) : kv_v_codes(D) + (v_half & 1) * 4 * D + v_r * (D / 2);
+        const float fac = a.scale * 1.4426950408889634f;
+        ManyPart part{0, 0, 0, 0, -1};
+        for (; u.next(args); stage_it += u.count) {
+            if (u.t0 == 0 && u.count < u.tiles)
+                part = ManyPart{u.seq, u.head, u.row0, u.place(), (u.unit_at + u.tiles - 1) / per};
+            const int32_t* row_table = v.table + static_cast<int64_t>(u.seq) * v.ld_table;
+            // Lane l holds the number of block l of eight tiles (-1: none): of those under
+            // way and, fetched early, of the next eight.
+            auto locate = [&](int j) {
+                const int pos = (u.t0 + j) * kManyKeys + lane * kKvBlock;
+                return j + (lane >> 2) < u.count && pos < u.sq.kv ? kv_block_number(v, row_table, u.head, pos) : -2;
+            };
+            int blocks = locate(0), blocks_next = locate(8);
+            uint4 w[D / 32], z[2];  // the codes; K: scales of the token, V: of the eight tokens
+            auto fetch = [&](int j) {
+                if ((j & 7) < 2 && j >= 8) {  // the group's first tile of eight
+                    blocks = blocks_next;
+                    blocks_next = locate((j & ~7) + 8);
+                }
+                const int at = __shfl_sync(0xFFFFFFFFu, blocks, (j & 7) * 4 + block_in);
+                if (at == -1) raise_error(v.err_flag, kErrBadPage);
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) w[k] = make_uint4(0, 0, 0, 0);
+                z[0] = z[1] = make_uint4(0, 0, 0, 0);
+                if (at >= 0) {
+                    const uint8_t* b = v.data + static_cast<int64_t>(at) * kv_block_bytes(D);
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) w[k] = *reinterpret_cast<const uint4*>(b + offset + k * 16);
+                    if (is_k) {
+                        z[0].x = reinterpret_cast<const uint32_t*>(b + kv_k_scales(D))[token & 15];
+                        z[0].y = reinterpret_cast<const uint32_t*>(b + kv_v_scales(D))[token & 15];
+                    } else {
+                        z[0] = *reinterpret_cast<const uint4*>(b + kv_v_scales(D) + (v_half & 1) * 32);
+                        z[1] = *reinterpret_cast<const uint4*>(b + kv_v_scales(D) + (v_half & 1) * 32 + 16);
+                    }
+                }
+            };
+            const int j0 = (group ^ stage_it) & 1;
+            if (j0 < u.count) fetch(j0);
+#pragma unroll 1
+            for (int j = j0; j < u.count; j += 2) {
+                const uint32_t it = stage_it + j, st = it % S::kStages;
+                if (it >= S::kStages)
+                    wait_phase(&s_empty[st], (it / S::kStages - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+                __syncwarp();
+                if (is_k) {
+                    // The column's scale; NaN when K or V of the token is, which so reaches the
+                    // rows that see it and no other (its codes are zeros).
+                    float sk = f16_bits_to_f32(static_cast<uint16_t>(z[0].x)) * fac;
+                    if ((z[0].y & 0x7C00u) == 0x7C00u) sk = __int_as_float(0x7FFFFFFF);
+                    *reinterpret_cast<float*>(cols + st * S::kCols + ((token >> 1) & 3) * S::kColsRow + (token >> 3) * 8 +
+                                              (token & 1) * 4) = sk;
+                    const uint32_t zz = (z[0].x >> 16) * 0x10001u;
+                    const uint32_t z1024 = 0x64006400u | zz, z64 = 0xD400D400u | zz << 4, z128 = 0x43004300u | zz;
+                    const uint32_t kst = k_u32 + st * S::kK;
+#pragma unroll
+                    for (int k = 0; k < D / 8; ++k) {
+                        const uint4 q4 = w[k >> 2];
+                        const uint32_t x = (k & 3) == 0 ? q4.x : (k & 3) == 1 ? q4.y : (k & 3) == 2 ? q4.z : q4.w;
+                        uint32_t e0, e1, e2, e3;
+                        if constexpr (BF16) {
+                            e0 = bf2_sub((x & kNib0) | 0x43004300u, z128);
+                            e1 = bf2_sub(((x >> 4) & kNib0) | 0x43004300u, z128);
+                            e2 = bf2_sub(((x >> 8) & kNib0) | 0x43004300u, z128);
+                            e3 = bf2_sub(((x >> 12) & kNib0) | 0x43004300u, z128);
+                        } else {
+                            e0 = nib0_f16(x, z1024);
+                            e1 = nib1_f16(x, z64);
+                            e2 = nib0_f16(x >> 8, z1024);
+                            e3 = nib1_f16(x >> 8, z64);
+                        }
+                        st_shared_16(panel_at(kst + (k >> 3) * S::kKPanel, token, k & 7), e0, e1, e2, e3);
+                    }
+                } else {
+                    // Token pairs' zero points and scales; then, for each word of a token, its
+                    // eight channels as rows of V^T.
+                    uint32_t z1024[4], z64[4], sv[4];
+                    const uint32_t zw[8] = {z[0].x, z[0].y, z[0].z, z[0].w, z[1].x, z[1].y, z[1].z, z[1].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t zz = __byte_perm(zw[2 * k], zw[2 * k + 1], 0x7632);
+                        z1024[k] = 0x64006400u | zz;
+                        z64[k] = 0xD400D400u | zz << 4;
+                        sv[k] = __byte_perm(zw[2 * k], zw[2 * k + 1], 0x5410);
+                        if ((sv[k] & 0x7C00u) == 0x7C00u) sv[k] &= 0xFFFF0000u;  // NaN: see above
+                        if ((sv[k] & 0x7C000000u) == 0x7C000000u) sv[k] &= 0xFFFFu;
+                    }
+                    const uint32_t vst = v_u32 + st * S::kV;
+#pragma unroll 1
+                    for (int hw = 0; hw < D / 32; ++hw) {  // word, and nibbles 0-3 or 4-7 of it
+                        const bool second = hw >= 2;
+                        const uint32_t pick = (hw & 1) ? 0x7632 : 0x5410;
+                        uint32_t x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if constexpr (D == 128)  // 16 bytes a pair: two words of each token
+                                x[k] = __byte_perm(second ? w[k].y : w[k].x, second ? w[k].w : w[k].z, pick);
+                            else  // 8 bytes a pair
+                                x[k] = __byte_perm((k & 1) ? w[k >> 1].z : w[k >> 1].x, (k & 1) ? w[k >> 1].w : w[k >> 1].y, pick);
+                        }
+                        const int ch = v_r * (D / 8) + hw * 4;
+                        auto store = [&](int row, auto&& value) {
+                            st_shared_16(panel_at(vst, row, v_half), h2_mul(value(0), sv[0]), h2_mul(value(1), sv[1]),
+                                         h2_mul(value(2), sv[2]), h2_mul(value(3), sv[3]));
+                        };
+                        store(ch, [&](int k) { return nib0_f16(x[k], z1024[k]); });
+                        store(ch + 1, [&](int k) { return nib1_f16(x[k], z64[k]); });
+                        store(ch + 2, [&](int k) { return nib0_f16(x[k] >> 8, z1024[k]); });
+                        store(ch + 3, [&](int k) { return nib1_f16(x[k] >> 8, z64[k]); });
+                    }
+                }
+                fence_async_smem();
+                mbar_arrive(&s_full[st]);
+                __syncwarp();
+                if (j + 2 < u.count) fetch(j + 2);
+            }
+        }
+        if (threadIdx.x == kSoftmaxWarps * 32) args.parts[blockIdx.x] = part;
+    } else if (warp < kSoftmaxWarps + kCodesWarps + 2) {
+        // -------------------------------------------------------------- products
+        const int i = warp & 1;
+        if (lane == 0) {
+            const uint32_t idesc_qk = idesc_f16_f32(128, kManyKeys) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+            const uint32_t idesc_pv = idesc_f16_f32(128, D);
+            const uint32_t t_rows = tmem + i * 128, t_o = tmem + 256 + i * D;
+            uint32_t all_units = 0, units = 0;  // units so far, and those with this row tile
+            for (; u.next(args); stage_it += u.count, ++all_units) {
+                wait_phase(&s_q, all_units & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                if (i >= u.row_tiles()) {  // the other tile's alone: only give back what it uses
+                    for (int j = 0; j < u.count; ++j) {
+                        const uint32_t it = stage_it + j;
+                        wait_phase(&s_full[it % S::kStages], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        mbar_arrive(&s_empty[it % S::kStages]);
+                    }
+                    mbar_arrive(&s_q_free);
+                    continue;
+                }
+#pragma unroll 1
+                for (int j = -2; j < u.count; ++j) {
+                    if (j >= 0) {  // O += P V
+                        const uint32_t t = tile_it + j, buf = t & 1, st = (stage_it + j) % S::kStages;
+                        wait_phase(&s_probs[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        if (j == 0 && units > 0)
+                            wait_phase(&s_free[i], (units - 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        tc_fence_after();
+                        const uint32_t vd = desc_low(v_u32 + st * S::kV), pt = t_rows + buf * kManyKeys;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) tc_mma_ts(t_o, pt + k * 8, vd + k * 2, idesc_pv, j + k > 0);
+                        tc_commit(&s_done[i][buf]);
+                        tc_commit(&s_empty[st]);
+                    }
+                    if (j + 2 < u.count) {  // scores two tiles on, once P in their place has been used
+                        const uint32_t it = stage_it + j + 2, t = tile_it + j + 2, buf = t & 1, st = it % S::kStages;
+                        wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        if (t >= 2) wait_phase(&s_done[i][buf], ((t >> 1) - 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        tc_fence_after();
+                        uint32_t qd = desc_low(q_u32 + i * kPanels * S::kPanel), kd = desc_low(k_u32 + st * S::kK);
+#pragma unroll 1
+                        for (int p = 0; p < kPanels; ++p, qd += S::kPanel >> 4, kd += S::kKPanel >> 4)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                tc_mma_ss(t_rows + buf * kManyKeys, qd + k * 2, kd + k * 2, idesc_qk, p + k > 0);
+                        tc_commit(&s_scores[i][buf]);
+                        if (j + 3 == u.count) tc_commit(&s_q_free);
+                    }
+                }
+                tile_it += u.count;
+                ++units;
+            }
+        }
+        __syncwarp();
+    } else {
+        // -------------------------------------------------------------- Q, as it is
+        const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.ldq & 7) == 0;
+        for (uint32_t unit = 0; u.next(args); ++unit) {
+            if (unit > 0) wait_phase(&s_q_free, (unit - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+#pragma unroll 4
+            for (int e = threadIdx.x & (kLoaders - 1); e < u.row_tiles() * 128 * (D / 8); e += kLoaders) {
+                const int row = e / (D / 8), ch = e - row * (D / 8);
                 uint4 w = make_uint4(0, 0, 0, 0);
-                if (row < rows) {
-                    const int tok = (row0 + row) / args.group, gh = row0 + row - tok * args.group;
-                    const uint16_t* src = a.q + (sq.first + tok) * a.ldq + (head * args.group + gh) * D + ch * 8;
+                if (row < u.rows) {
+                    const int tok = (u.row0 + row) / args.group, gh = u.row0 + row - tok * args.group;
+                    const uint16_t* src = a.q + (u.sq.first + tok) * a.ldq + (u.head * args.group + gh) * D + ch * 8;
                     if (vec) {
                         w = *reinterpret_cast<const uint4*>(src);
                     } else {
@@ -976,342 +1410,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 st_shared_16(panel_at(base, row & 127, ch & 7), w.x, w.y, w.z, w.w);
             }
             fence_async_smem();
+            mbar_arrive(&s_q);
         }
-        __syncthreads();
-
-        if (warp < 8) {
-            // ---------------------------------------------------------- softmax
-            const int i = warp >> 2;
-            if (i < row_tiles) {
-                const int r = lane >> 2, c = lane & 3;
-                const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // its 32 TMEM lanes
-                const uint32_t t_s = tmem + i * 128 + lanes, t_o = tmem + 256 + i * D + lanes;
-                float m[4], l[4];
-                int limit[4], limit_min = 0x7FFFFFFF;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = i * 128 + (warp & 3) * 32 + k * 8 + r;
-                    m[k] = -INFINITY;
-                    l[k] = 0.0f;
-                    limit[k] = 0;
-                    if (row < rows) {
-                        limit[k] = a.causal ? sq.kv - sq.n + (row0 + row) / args.group + 1 : sq.kv;
-                        limit_min = min(limit_min, limit[k]);
-                    }
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
-                for (int j = 0; j < count; ++j) {
-                    const uint32_t it = stage_it + j, ti = tile_it[i] + j, st = it & 1;
-                    const uint8_t* cc = cols + st * S::kCols;
-                    const float4* kl = reinterpret_cast<const float4*>(cc) + c;
-                    const float2* rs = reinterpret_cast<const float2*>(cc + 1024) + c;
-                    const int pos0 = (t0 + j) * kManyKeys;
-                    const bool inner = pos0 + kManyKeys <= limit_min;
-                    wait_phase(&s_full[st], (it >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
-                    wait_phase(&s_scores[i], ti & 1, &s_gave_up, v.err_flag, kErrEpiWait);
-                    __syncwarp();
-                    tc_fence_after();
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {  // rows h 16 + r, + 8
-                        uint32_t s[64];
-                        tmem_ld_frag128(t_s + (static_cast<uint32_t>(h) << 20), s);
-                        float big[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float4 w = kl[k * 4];
-#pragma unroll
-                            for (int b = 0; b < 2; ++b) {
-                                float y0 = fmaf(__uint_as_float(s[k * 4 + b * 2]), w.x, w.z);
-                                float y1 = fmaf(__uint_as_float(s[k * 4 + b * 2 + 1]), w.y, w.w);
-                                if (!inner) {
-                                    if (pos0 + k * 8 + c * 2 >= limit[h * 2 + b]) y0 = -INFINITY;
-                                    if (pos0 + k * 8 + c * 2 + 1 >= limit[h * 2 + b]) y1 = -INFINITY;
-                                }
-                                big[b] = fmaxf(big[b], fmaxf(y0, y1));
-                                s[k * 4 + b * 2] = __float_as_uint(y0);
-                                s[k * 4 + b * 2 + 1] = __float_as_uint(y1);
-                            }
-                        }
-                        bool grow = false;
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
-                            big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 2));
-                            grow |= big[b] > m[h * 2 + b] + 8.0f;  // from -inf: any
-                        }
-                        if (__any_sync(0xFFFFFFFFu, grow)) {
-                            float fix[2];
-#pragma unroll
-                            for (int b = 0; b < 2; ++b) {
-                                const float to = fmaxf(m[h * 2 + b], big[b]);
-                                fix[b] = to == -INFINITY ? 1.0f : fast_exp2(m[h * 2 + b] - to);
-                                m[h * 2 + b] = to;
-                                l[h * 2 + b] *= fix[b];
-                            }
-                            if (j > 0) {  // the scores were asked for after the last product into O had ended
-#pragma unroll
-                                for (int ch = 0; ch < D; ch += 64) {
-                                    uint32_t o[32];
-                                    const uint32_t t = t_o + (static_cast<uint32_t>(h) << 20) + ch;
-                                    tmem_ld_frag64(t, o);
-#pragma unroll
-                                    for (int k = 0; k < 32; ++k)
-                                        o[k] = __float_as_uint(__uint_as_float(o[k]) * fix[(k >> 1) & 1]);
-                                    tmem_st_frag64(t, o);
-                                }
-                            }
-                        }
-                        uint32_t p[32];
-                        float base[2];
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) base[b] = m[h * 2 + b] == -INFINITY ? 0.0f : m[h * 2 + b];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float2 w = rs[k * 4];
-#pragma unroll
-                            for (int b = 0; b < 2; ++b) {
-                                const float p0 = fast_exp2(__uint_as_float(s[k * 4 + b * 2]) - base[b]);
-                                const float p1 = fast_exp2(__uint_as_float(s[k * 4 + b * 2 + 1]) - base[b]);
-                                l[h * 2 + b] = fmaf(p0, w.x, fmaf(p1, w.y, l[h * 2 + b]));
-                                const __half2 hp = __floats2half2_rn(p0, p1);
-                                p[k * 2 + b] = *reinterpret_cast<const uint32_t*>(&hp);
-                            }
-                        }
-                        tmem_st_pairs64(t_s + (static_cast<uint32_t>(h) << 20), p);
-                    }
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&s_probs[i]);
-                }
-                // The output, or the unit's part of it.
-                wait_phase(&s_done[i], (tile_it[i] + count - 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
-                __syncwarp();
-                tc_fence_after();
-                const bool whole = t0 == 0 && t1 == tiles;
-                const int64_t slot = blockIdx.x * 2LL + (unit_at > range_begin ? 1 : 0);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    l[k] += __shfl_xor_sync(0xFFFFFFFFu, l[k], 1);
-                    l[k] += __shfl_xor_sync(0xFFFFFFFFu, l[k], 2);
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int ch = 0; ch < D; ch += 64) {
-                        uint32_t o[32];
-                        __syncwarp();
-                        tmem_ld_frag64(t_o + (static_cast<uint32_t>(h) << 20) + ch, o);
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            const int row = i * 128 + (warp & 3) * 32 + h * 16 + b * 8 + r;
-                            if (row >= rows) continue;
-                            const float sum = l[h * 2 + b];
-                            if (whole) {
-                                const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-                                const int tok = (row0 + row) / args.group, gh = row0 + row - tok * args.group;
-                                uint16_t* dst = a.out + (sq.first + tok) * a.ldo + (head * args.group + gh) * D + ch + c * 2;
-                                const bool vec = (reinterpret_cast<uintptr_t>(dst) & 3) == 0;
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    const uint16_t h0 = narrow(__uint_as_float(o[k * 4 + b * 2]) * inv, a.dtype);
-                                    const uint16_t h1 = narrow(__uint_as_float(o[k * 4 + b * 2 + 1]) * inv, a.dtype);
-                                    if (vec) {
-                                        *reinterpret_cast<uint32_t*>(dst + k * 8) = h0 | static_cast<uint32_t>(h1) << 16;
-                                    } else {
-                                        dst[k * 8] = h0;
-                                        dst[k * 8 + 1] = h1;
-                                    }
-                                }
-                            } else {
-                                float* dst = args.part_o + (slot * kManyRows + row) * D + ch + c * 2;
-#pragma unroll
-                                for (int k = 0; k < 8; ++k)
-                                    *reinterpret_cast<float2*>(dst + k * 8) =
-                                        make_float2(__uint_as_float(o[k * 4 + b * 2]), __uint_as_float(o[k * 4 + b * 2 + 1]));
-                                if (ch == 0 && c == 0) args.part_ml[slot * kManyRows + row] = make_float2(m[h * 2 + b], sum);
-                            }
-                        }
-                    }
-                tc_fence_before();
-            }
-        } else if (warp < 12) {
-            // ---------------------------------------------------------- codes to integers
-            const int tid = threadIdx.x - 256;
-            const int32_t* row_table = v.table + static_cast<int64_t>(seq) * v.ld_table;
-            const float fac = a.scale * 1.4426950408889634f;
-            // K: token tid.  V: eight tokens (a half block), a stretch of D / 8 channels:
-            // eight neighbouring lanes write eight different 16-byte columns of a panel.
-            const int v_half = (warp & 1) * 8 + (lane & 7);                        // of 16 half blocks
-            const int v_r = ((warp - 8) >> 1) * 4 + (lane >> 3);                   // channel stretch
-            uint4 kw[D / 32], vw[D / 32], vz[2];
-            uint32_t ks, vs;
-            auto load = [&](int j) {  // tile j's bytes, one tile ahead of their use
-                const int pos0 = (t0 + j) * kManyKeys;
-                const int kpos = pos0 + tid, vpos = pos0 + v_half * 8, token = kpos & (kKvBlock - 1);
-                const uint8_t *kb = nullptr, *vb = nullptr;
-                if (kpos < sq.kv) {
-                    kb = kv_block_at(v, row_table, head, kpos);
-                    if (kb == nullptr) raise_error(v.err_flag, kErrBadPage);
-                }
-                if (vpos < sq.kv) vb = kv_block_at(v, row_table, head, vpos);
-                ks = vs = 0;
-#pragma unroll
-                for (int k = 0; k < D / 32; ++k) kw[k] = vw[k] = make_uint4(0, 0, 0, 0);
-                vz[0] = vz[1] = make_uint4(0, 0, 0, 0);
-                if (kb != nullptr) {
-#pragma unroll
-                    for (int k = 0; k < D / 32; ++k)
-                        kw[k] = *reinterpret_cast<const uint4*>(kb + token * (D / 2) + k * 16);
-                    ks = reinterpret_cast<const uint32_t*>(kb + kv_k_scales(D))[token];
-                    vs = reinterpret_cast<const uint32_t*>(kb + kv_v_scales(D))[token];
-                }
-                if (vb != nullptr) {
-#pragma unroll
-                    for (int k = 0; k < D / 32; ++k)
-                        vw[k] = *reinterpret_cast<const uint4*>(vb + kv_v_codes(D) + (v_half & 1) * 4 * D + v_r * (D / 2) + k * 16);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        vz[k] = *reinterpret_cast<const uint4*>(vb + kv_v_scales(D) + (v_half & 1) * 32 + k * 16);
-                }
-            };
-            load(0);
-            for (int j = 0; j < count; ++j) {
-                const uint32_t it = stage_it + j, st = it & 1;
-                if (it >= 2) wait_phase(&s_empty[st], ((it >> 1) - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
-                // columns' constants
-                {
-                    const float sk = f16_bits_to_f32(static_cast<uint16_t>(ks));
-                    if ((vs & 0xFFFFu) == 0) vs |= 1u;  // never stored, or nobody's: holds zeros whatever its scale
-                    const float sv = f16_bits_to_f32(static_cast<uint16_t>(vs));
-                    uint8_t* cc = cols + st * S::kCols;
-                    float* kl = reinterpret_cast<float*>(cc) + (tid >> 1) * 4 + (tid & 1);
-                    kl[0] = sk * fac;
-                    kl[2] = fast_log2(sv);
-                    // a NaN scale reaches the rows that see it through the exponent, and no other
-                    reinterpret_cast<float*>(cc + 1024)[tid] = sv != sv ? 0.0f : fast_rcp(sv);
-                }
-                const uint32_t kst = k_u32 + st * S::kK, vst = v_u32 + st * S::kV;
-                {
-                    const uint32_t z = ks >> 16, zz = z | z << 16;
-                    const uint32_t z1024 = 0x64006400u | zz, z64 = 0xD400D400u | zz << 4, z128 = 0x43004300u | zz;
-#pragma unroll
-                    for (int k = 0; k < D / 8; ++k) {
-                        const uint4 q4 = kw[k >> 2];
-                        const uint32_t w = (k & 3) == 0 ? q4.x : (k & 3) == 1 ? q4.y : (k & 3) == 2 ? q4.z : q4.w;
-                        uint32_t e0, e1, e2, e3;
-                        if constexpr (BF16) {
-                            e0 = bf2_sub((w & kNib0) | 0x43004300u, z128);
-                            e1 = bf2_sub(((w >> 4) & kNib0) | 0x43004300u, z128);
-                            e2 = bf2_sub(((w >> 8) & kNib0) | 0x43004300u, z128);
-                            e3 = bf2_sub(((w >> 12) & kNib0) | 0x43004300u, z128);
-                        } else {
-                            e0 = nib0_f16(w, z1024);
-                            e1 = nib1_f16(w, z64);
-                            e2 = nib0_f16(w >> 8, z1024);
-                            e3 = nib1_f16(w >> 8, z64);
-                        }
-                        st_shared_16(panel_at(kst + (k >> 3) * S::kPanel, tid, k & 7), e0, e1, e2, e3);
-                    }
-                }
-                {
-                    // Token pairs' zero points; then, for each word of a token, its eight channels as rows of V^T.
-                    uint32_t z1024[4], z64[4];
-                    const uint32_t zw[8] = {vz[0].x, vz[0].y, vz[0].z, vz[0].w, vz[1].x, vz[1].y, vz[1].z, vz[1].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t zz = __byte_perm(zw[2 * k], zw[2 * k + 1], 0x7632);
-                        z1024[k] = 0x64006400u | zz;
-                        z64[k] = 0xD400D400u | zz << 4;
-                    }
-#pragma unroll
-                    for (int w = 0; w < D / 64; ++w) {
-                        uint32_t t[8];  // word w of the eight tokens
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if constexpr (D == 128) {  // 16 bytes a pair: two words of each token
-                                t[2 * k] = w ? vw[k].y : vw[k].x;
-                                t[2 * k + 1] = w ? vw[k].w : vw[k].z;
-                            } else {  // 8 bytes a pair
-                                const uint4 u = vw[k >> 1];
-                                t[2 * k] = (k & 1) ? u.z : u.x;
-                                t[2 * k + 1] = (k & 1) ? u.w : u.y;
-                            }
-                        }
-#pragma unroll
-                        for (int hi = 0; hi < 2; ++hi) {
-                            uint32_t u[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) u[k] = __byte_perm(t[2 * k], t[2 * k + 1], hi ? 0x7632 : 0x5410);
-                            const int ch = v_r * (D / 8) + w * 8 + hi * 4;
-                            const uint32_t panel = vst + (v_half >> 3) * (D * 128);
-                            const int chunk = v_half & 7;
-                            st_shared_16(panel_at(panel, ch, chunk), nib0_f16(u[0], z1024[0]), nib0_f16(u[1], z1024[1]),
-                                         nib0_f16(u[2], z1024[2]), nib0_f16(u[3], z1024[3]));
-                            st_shared_16(panel_at(panel, ch + 1, chunk), nib1_f16(u[0], z64[0]), nib1_f16(u[1], z64[1]),
-                                         nib1_f16(u[2], z64[2]), nib1_f16(u[3], z64[3]));
-                            st_shared_16(panel_at(panel, ch + 2, chunk), nib0_f16(u[0] >> 8, z1024[0]), nib0_f16(u[1] >> 8, z1024[1]),
-                                         nib0_f16(u[2] >> 8, z1024[2]), nib0_f16(u[3] >> 8, z1024[3]));
-                            st_shared_16(panel_at(panel, ch + 3, chunk), nib1_f16(u[0] >> 8, z64[0]), nib1_f16(u[1] >> 8, z64[1]),
-                                         nib1_f16(u[2] >> 8, z64[2]), nib1_f16(u[3] >> 8, z64[3]));
-                        }
-                    }
-                }
-                fence_async_smem();
-                mbar_arrive(&s_full[st]);
-                if (j + 1 < count) load(j + 1);
-            }
-        } else if (lane == 0) {
-            // ---------------------------------------------------------- products
-            auto scores = [&](int i, uint32_t st) {
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t qd = smem_desc_k128(q_u32 + (i * kPanels + (k >> 2)) * S::kPanel + (k & 3) * 32);
-                    const uint64_t kd = smem_desc_k128(k_u32 + st * S::kK + (k >> 2) * S::kPanel + (k & 3) * 32);
-                    tc_mma_f16(tmem + i * 128, qd, kd, idesc_qk, k > 0);
-                }
-                tc_commit(&s_scores[i]);
-            };
-            wait_phase(&s_full[stage_it & 1], (stage_it >> 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-            tc_fence_after();
-            for (int i = 0; i < row_tiles; ++i) scores(i, stage_it & 1);
-            for (int j = 0; j < count; ++j) {
-                const uint32_t st = (stage_it + j) & 1;
-                for (int i = 0; i < row_tiles; ++i) {
-                    wait_phase(&s_probs[i], (tile_it[i] + j) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < kManyKeys / 16; ++k) {
-                        const uint64_t vd = smem_desc_k128(v_u32 + st * S::kV + (k >> 2) * (D * 128) + (k & 3) * 32);
-                        tc_mma_f16_ts(tmem + 256 + i * D, tmem + i * 128 + k * 8, vd, idesc_pv, j > 0 || k > 0);
-                    }
-                    tc_commit(&s_done[i]);
-                    if (i == row_tiles - 1) tc_commit(&s_empty[st]);
-                    if (j + 1 < count) {
-                        const uint32_t it = stage_it + j + 1;
-                        wait_phase(&s_full[it & 1], (it >> 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                        wait_phase(&s_done[i], (tile_it[i] + j) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                        tc_fence_after();
-                        scores(i, it & 1);
-                    }
-                }
-            }
-        }
-        __syncwarp();
-        stage_it += count;
-        tile_it[0] += count;
-        if (row_tiles > 1) tile_it[1] += count;
-        if (t0 == 0 && t1 < tiles) part = ManyPart{seq, head, row0, unit_at > range_begin ? 1 : 0, static_cast<int>((unit_at + tiles - 1) / per)};
-        at += count;
-        __syncthreads();
-        tc_fence_after();
     }
-    if (threadIdx.x == 0) args.parts[blockIdx.x] = part;
-    // Every product has ended: each role waited for the last one of its tile.
+    // Every product has ended: each softmax waited for the last one of its tile.
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == kSoftmaxWarps + kCodesWarps) tmem_dealloc(tmem, 512);
 }
 
 // Adds the parts of a unit that spans CTAs: one CTA per (CTA it begins in,
@@ -1344,11 +1449,11 @@ __global__ void __launch_bounds__(kThreads) attn_q4_many_join_kernel(const ManyA
         for (int j = 0; j < PER; ++j) o[j] = o[j] * f0 + x[j] * f1;
         m = big;
     }
-    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    const float inv = l == 0.0f ? 0.0f : fast_rcp(l);
     const int tok = (part.row0 + row) / args.group, gh = part.row0 + row - tok * args.group;
+    uint16_t* dst = a.out + (first + tok) * a.ldo + (part.head * args.group + gh) * D + lane * PER;
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-        a.out[(first + tok) * a.ldo + (part.head * args.group + gh) * D + lane * PER + j] = narrow(o[j] * inv, a.dtype);
+    for (int j = 0; j < PER; j += 2) store2(dst + j, narrow2(o[j] * inv, o[j + 1] * inv, a.dtype));
 }
 
 }  // namespace
@@ -1361,7 +1466,12 @@ static int check_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int64_t head
     if (rc != MRT_OK) return rc;
     if (heads <= 0 || heads > 65535 || heads % kv->kv_heads != 0)
         return set_error(MRT_ERR_SHAPE, "heads must be a positive multiple of kv_heads");
-    if (batch->seqs * kv->kv_heads > (1LL << 31) - 1) return set_error(MRT_ERR_SHAPE, "too many sequences and heads");
+    // Rows and tiles are numbered in 31 bits.
+    const double group = static_cast<double>(heads / kv->kv_heads), keys = static_cast<double>(batch->max_kv_len) + 128;
+    const double rows = static_cast<double>(batch->tokens) * group;
+    if (rows + 512.0 * batch->seqs > 2147483647.0 || static_cast<double>(batch->seqs) * kv->kv_heads * keys / 32 > 2147483647.0 ||
+        (rows / 256 + batch->seqs) * kv->kv_heads * keys / 128 > 2147483647.0)
+        return set_error(MRT_ERR_SHAPE, "too many rows and keys for one call");
     return MRT_OK;
 }
 

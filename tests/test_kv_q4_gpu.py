@@ -220,8 +220,11 @@ def test_non_finite_rows_read_back_as_nan(cuda_dev):
 def reference(c, q, kx, vx, vs, causal, scale):
     """64-bit attention, and the tolerance of each output.
 
-    Each probability times its value's scale is rounded to FP16 (2^-11, or half
-    the smallest subnormal, 2^-25 of the row's largest, where it is small); a
+    Few rows (32 of a sequence and kv head): each probability times its value's
+    scale is rounded to FP16, 2^-11 of it, or where it is small 2^-25 of the
+    row's largest such product (codes up to 15).  Many rows: each probability
+    is, by 2^-11 or 2^-25 of the row's largest, and each value, by 2^-11 or
+    2^-25.  A
     score is off by FP32 sums of the products' magnitude (2^-23 for each of at
     most 16 chained additions) and its own size, and moves its probability by
     as much; the sums over keys are off by 2^-23 for each of the chained
@@ -232,6 +235,7 @@ def reference(c, q, kx, vx, vs, causal, scale):
     out = torch.zeros(q.shape, dtype=torch.float64)
     tol = torch.zeros(q.shape, dtype=torch.float64)
     row = tok = 0
+    many = max(n for n, _ in c.lens) * H // Hk > 32
     for n, kv in c.lens:
         k, v, sv = kx[tok:tok + kv].cuda(), vx[tok:tok + kv].cuda(), vs[tok:tok + kv].cuda()
         for i in range(n):
@@ -244,10 +248,13 @@ def reference(c, q, kx, vx, vs, causal, scale):
             p = s.softmax(-1)
             o = torch.einsum("hgt,thd->hgd", p, v[:keys])
             off = (16 * 2.0 ** -23 * mag + 2.0 ** -22 * s.abs() + 2.0 ** -21)
-            pv = torch.einsum("hgt,thd->hgd", p * (2.0 ** -11 + 2 * off), v[:keys].abs())
+            pv = torch.einsum("hgt,thd->hgd", p * (2.0 ** (-10 if many else -11) + 2 * off), v[:keys].abs())
             pv += (32 + keys / 16) * 2.0 ** -23 * torch.einsum("hgt,thd->hgd", p, v[:keys].abs() + 30 * sv[:keys])
             mean_off = (p * off).sum(-1, keepdim=True)
-            low = (p * sv[:keys].permute(1, 2, 0)).amax(-1, keepdim=True) * 2.0 ** -25 * 15 * keys
+            if many:
+                low = p.amax(-1, keepdim=True) * 2.0 ** -25 * v[:keys].abs().sum(0)[:, None] + 2.0 ** -25
+            else:
+                low = (p * sv[:keys].permute(1, 2, 0)).amax(-1, keepdim=True) * 2.0 ** -25 * 15 * keys
             out[row + i] = o.reshape(H, D).cpu()
             tol[row + i] = (pv + 2 * mean_off * o.abs() + low + HALF_STEP[q.dtype] * o.abs() + 2.0 ** -25).reshape(H, D).cpu()
         row, tok = row + n, tok + kv
