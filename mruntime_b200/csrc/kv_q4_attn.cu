@@ -723,9 +723,9 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 //                    layout, K as the integers c - z (exact), V as values
 //                    s (c - z) rounded to FP16; four warps the even key tiles,
 //                    four the odd ones
-//   warps 24, 25     the products of tile 0, 1: S_i = Q_i K^T, O_i += P_i V
-//                    (A from TMEM)
-//   warps 26, 27     Q into its panels
+//   warps 24, 25     S_i = Q_i K^T
+//   warps 26, 27     O_i += P_i V (P from TMEM)
+//   warps 28-31      Q into its panels
 //
 // Each role walks the CTA's units by itself and meets the others only at
 // mbarriers, and units follow one another without a stop.  TMEM: two S (P in
@@ -750,9 +750,9 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // Units' key tiles are dealt to the CTAs in equal contiguous stretches, as in
 // the few-rows kernel, parts of units that span CTAs joined from scratch.
 constexpr int kManyRows = 256, kManyKeys = 64;
-constexpr int kSoftmaxWarps = 16, kCodesWarps = 8, kManyWarps = kSoftmaxWarps + kCodesWarps + 4;
+constexpr int kSoftmaxWarps = 16, kCodesWarps = 8, kManyWarps = kSoftmaxWarps + kCodesWarps + 8;
 constexpr int kManyThreads = kManyWarps * 32;
-constexpr int kLoaders = 64;  // threads that bring Q
+constexpr int kLoaders = 128;  // threads that bring Q
 
 struct ManyPart {  // a unit that begins in a CTA's stretch and goes on
     int seq, head, row0;
@@ -782,21 +782,22 @@ struct ManySeq {
     }
 };
 
-// sum_{i < n} floor((a i + b) / m), all >= 0: the lattice points under a line,
-// counted by exchanging the axes until the line is flat.
-__device__ __noinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-    int64_t sum = 0;
+// sum_{i < n} floor((a i + b) / m), the lattice points under a line, counted by
+// exchanging the axes until the line is flat.  a n + b fits in 32 bits (checked
+// on the host); so does the sum, whose parts may wrap.
+__device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+    uint32_t sum = 0;
 #pragma unroll 1
     while (n > 0) {
-        const int64_t qa = a / m, qb = b / m;
-        sum += n * (n - 1) / 2 * qa + n * qb;
+        const uint32_t qa = a / m, qb = b / m;
+        sum += static_cast<uint32_t>(static_cast<uint64_t>(n) * (n - 1) / 2) * qa + n * qb;
         a -= qa * m;
         b -= qb * m;
-        const int64_t top = a * n + b;
+        const uint32_t top = a * n + b;
         if (top < m) break;
         n = top / m;
         b = top - n * m;
-        const int64_t t = m;
+        const uint32_t t = m;
         m = a;
         a = t;
     }
@@ -808,8 +809,7 @@ __device__ __forceinline__ int many_before(const ManySeq& s, int x) {
     if (x == 0) return 0;
     if (!s.causal) return x * s.tiles(0);
     const int y = min(x, s.count - 1);
-    int t = y + static_cast<int>(floor_sum(y, static_cast<int64_t>(kManyKeys) * s.group, kManyRows,
-                                           kManyRows - 1 + static_cast<int64_t>(s.past()) * s.group));
+    int t = y + static_cast<int>(floor_sum(y, kManyKeys * s.group, kManyRows, kManyRows - 1 + s.past() * s.group));
     if (x == s.count) t += s.tiles(s.count - 1);
     return t;
 }
@@ -935,6 +935,21 @@ struct ManyWalk {
     __device__ __forceinline__ int place() const { return unit_at > begin ? 1 : 0; }  // where its part goes
 };
 
+template <int N>
+__device__ __forceinline__ void registers_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int N>
+__device__ __forceinline__ void registers_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Registers a thread: at launch, and as the roles share them out (in groups of
+// four warps: four of softmax, two of codes, products, Q).
+constexpr int kManyRegs = 64, kSoftmaxRegs = 72, kCodesRegs = 72, kOtherRegs = 40;
+static_assert(4 * kSoftmaxRegs + 2 * kCodesRegs + 2 * kOtherRegs == 8 * kManyRegs, "the roles share what the launch has");
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const ManyArgs args) {
     using S = ManyShape<D>;
@@ -945,7 +960,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     // been read.  s_q, s_q_free: Q.
     __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_scores[2][2], s_probs[2][2], s_done[2][2], s_free[2], s_q, s_q_free;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_gave_up, s_seq, s_at, s_sum[kManyWarps];
+    __shared__ int s_gave_up, s_seq, s_at, s_tiles, s_sum[kManyWarps];
     uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     const uint32_t q_u32 = smem_u32(smem), k_u32 = q_u32 + S::kQ, v_u32 = k_u32 + S::kStages * S::kK;
     uint8_t* cols = smem + S::kQ + S::kStages * (S::kK + S::kV);
@@ -983,11 +998,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     griddep_wait();
 
     // This CTA's stretch, and the unit it begins in.
-    int mine = 0;
+    int mine = 0, first_tiles = 0;  // of the thread's sequences, of its first
     for (int b = threadIdx.x; b < v.seqs; b += kManyThreads) {
         ManySeq q;
         if (!many_seq(args, b, &q) && blockIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
-        mine += many_before(q, q.count);
+        const int t = many_before(q, q.count);
+        mine += t;
+        if (b == threadIdx.x) first_tiles = t;
     }
     const int total = block_sum<kManyWarps>(mine, s_sum) * v.kv_heads;
     const int per = (total + args.grid - 1) / args.grid;
@@ -1001,12 +1018,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
 #pragma unroll 1
         for (int b0 = 0; u.seq < 0; b0 += kManyThreads) {  // ends: u.at < total
             const int b = b0 + threadIdx.x;
-            int t = 0;
-            if (b < v.seqs) {
+            int t = first_tiles;
+            if (b0 > 0 && b < v.seqs) {
                 ManySeq q;
                 many_seq(args, b, &q);
-                t = many_before(q, q.count) * v.kv_heads;
+                t = many_before(q, q.count);
             }
+            t = b < v.seqs ? t * v.kv_heads : 0;
             int incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -1026,33 +1044,41 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             if (u.at >= base + incl - t && u.at < base + incl) {
                 s_seq = b;
                 s_at = base + incl - t;
+                s_tiles = t / v.kv_heads;
             }
             __syncthreads();
             u.seq = s_seq;
             u.unit_at = s_at;
         }
         many_seq(args, u.seq, &u.sq);
-        const int a_head = many_before(u.sq, u.sq.count);
+        const int a_head = s_tiles;
         u.head = (u.at - u.unit_at) / a_head;
         u.unit_at += u.head * a_head;
         const int off = u.at - u.unit_at;
         int span = u.sq.count;  // the row tile lies in [x, x + span)
+        int skip = 0;           // key tiles before row tile x
 #pragma unroll 1
         while (span > 1) {
             const int step = (span + kManyThreads - 1) / kManyThreads;
             const int mid = u.x + threadIdx.x * step;
-            const int n = __syncthreads_count(mid < u.x + span && many_before(u.sq, min(mid, u.sq.count)) <= off);
+            const bool in = mid < u.x + span;
+            const int t = in ? many_before(u.sq, mid) : 0;
+            const int n = __syncthreads_count(in && t <= off);
+            if (static_cast<int>(threadIdx.x) == n - 1) s_at = t;
+            __syncthreads();
+            skip = s_at;
             const int next = u.x + (n - 1) * step;
             span = min(step, u.x + span - next);
             u.x = next;
         }
-        u.unit_at += many_before(u.sq, u.x);
+        u.unit_at += skip;
     }
     // Key tiles so far: of the CTA, of the role's row tile.
     uint32_t stage_it = 0, tile_it = 0;
 
     if (warp < kSoftmaxWarps) {
         // -------------------------------------------------------------- softmax
+        registers_up<kSoftmaxRegs>();
         const int i = warp >> 3, r = lane >> 2, c = lane & 3;
         const int row_in = (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + r;  // this lane's rows of the tile: it and + 8
         const uint32_t lanes = static_cast<uint32_t>(row_in - r) << 16;
@@ -1205,6 +1231,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
         }
     } else if (warp < kSoftmaxWarps + kCodesWarps) {
         // -------------------------------------------------------------- codes to operands
+        registers_up<kCodesRegs>();
         // A group's first two warps take K, a token a lane; the others V, a lane eight
         // tokens (a half block) of a stretch of D / 8 channels: eight neighbouring lanes
         // write eight different 16-byte columns of V^T.
@@ -1332,83 +1359,98 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             }
         }
         if (threadIdx.x == kSoftmaxWarps * 32) args.parts[blockIdx.x] = part;
-    } else if (warp < kSoftmaxWarps + kCodesWarps + 2) {
+    } else if (warp < kSoftmaxWarps + kCodesWarps + 4) {
         // -------------------------------------------------------------- products
+        registers_down<kOtherRegs>();
         const int i = warp & 1;
-        if (lane == 0) {
-            const uint32_t idesc_qk = idesc_f16_f32(128, kManyKeys) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
-            const uint32_t idesc_pv = idesc_f16_f32(128, D);
-            const uint32_t t_rows = tmem + i * 128, t_o = tmem + 256 + i * D;
-            uint32_t all_units = 0, units = 0;  // units so far, and those with this row tile
-            for (; u.next(args); stage_it += u.count, ++all_units) {
-                wait_phase(&s_q, all_units & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+        const uint32_t t_rows = tmem + i * 128;
+        if (lane == 0 && (warp & 2) == 0) {  // scores
+            const uint32_t idesc = idesc_f16_f32(128, kManyKeys) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+            uint32_t unit = 0;
+            for (; u.next(args); stage_it += u.count, ++unit) {
+                wait_phase(&s_q, unit & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                if (i >= u.row_tiles()) {
+                    mbar_arrive(&s_q_free);
+                    continue;
+                }
+#pragma unroll 1
+                for (int j = 0; j < u.count; ++j) {
+                    const uint32_t it = stage_it + j, t = tile_it + j, buf = t & 1, st = it % S::kStages;
+                    wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                    // P in their place has been used
+                    if (t >= 2) wait_phase(&s_done[i][buf], ((t >> 1) - 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                    tc_fence_after();
+                    uint32_t qd = desc_low(q_u32 + i * kPanels * S::kPanel), kd = desc_low(k_u32 + st * S::kK);
+#pragma unroll 1
+                    for (int p = 0; p < kPanels; ++p, qd += S::kPanel >> 4, kd += S::kKPanel >> 4)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc_mma_ss(t_rows + buf * kManyKeys, qd + k * 2, kd + k * 2, idesc, p + k > 0);
+                    tc_commit(&s_scores[i][buf]);
+                }
+                tc_commit(&s_q_free);
+                tile_it += u.count;
+            }
+        } else if (lane == 0) {  // output
+            const uint32_t idesc = idesc_f16_f32(128, D), t_o = tmem + 256 + i * D;
+            uint32_t units = 0;  // with this row tile
+            for (; u.next(args); stage_it += u.count) {
                 if (i >= u.row_tiles()) {  // the other tile's alone: only give back what it uses
                     for (int j = 0; j < u.count; ++j) {
                         const uint32_t it = stage_it + j;
                         wait_phase(&s_full[it % S::kStages], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
                         mbar_arrive(&s_empty[it % S::kStages]);
                     }
-                    mbar_arrive(&s_q_free);
                     continue;
                 }
 #pragma unroll 1
-                for (int j = -2; j < u.count; ++j) {
-                    if (j >= 0) {  // O += P V
-                        const uint32_t t = tile_it + j, buf = t & 1, st = (stage_it + j) % S::kStages;
-                        wait_phase(&s_probs[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                        if (j == 0 && units > 0)
-                            wait_phase(&s_free[i], (units - 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                        tc_fence_after();
-                        const uint32_t vd = desc_low(v_u32 + st * S::kV), pt = t_rows + buf * kManyKeys;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) tc_mma_ts(t_o, pt + k * 8, vd + k * 2, idesc_pv, j + k > 0);
-                        tc_commit(&s_done[i][buf]);
-                        tc_commit(&s_empty[st]);
+                for (int j = 0; j < u.count; ++j) {
+                    const uint32_t it = stage_it + j, t = tile_it + j, buf = t & 1, st = it % S::kStages;
+                    if (j == 0) {
+                        if (units > 0) wait_phase(&s_free[i], (units - 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                        ++units;
                     }
-                    if (j + 2 < u.count) {  // scores two tiles on, once P in their place has been used
-                        const uint32_t it = stage_it + j + 2, t = tile_it + j + 2, buf = t & 1, st = it % S::kStages;
-                        wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                        if (t >= 2) wait_phase(&s_done[i][buf], ((t >> 1) - 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                        tc_fence_after();
-                        uint32_t qd = desc_low(q_u32 + i * kPanels * S::kPanel), kd = desc_low(k_u32 + st * S::kK);
-#pragma unroll 1
-                        for (int p = 0; p < kPanels; ++p, qd += S::kPanel >> 4, kd += S::kKPanel >> 4)
+                    wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                    wait_phase(&s_probs[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                    tc_fence_after();
+                    const uint32_t vd = desc_low(v_u32 + st * S::kV), pt = t_rows + buf * kManyKeys;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                tc_mma_ss(t_rows + buf * kManyKeys, qd + k * 2, kd + k * 2, idesc_qk, p + k > 0);
-                        tc_commit(&s_scores[i][buf]);
-                        if (j + 3 == u.count) tc_commit(&s_q_free);
-                    }
+                    for (int k = 0; k < 4; ++k) tc_mma_ts(t_o, pt + k * 8, vd + k * 2, idesc, j + k > 0);
+                    tc_commit(&s_done[i][buf]);
+                    tc_commit(&s_empty[st]);
                 }
                 tile_it += u.count;
-                ++units;
             }
         }
         __syncwarp();
     } else {
         // -------------------------------------------------------------- Q, as it is
+        registers_down<kOtherRegs>();
         const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.ldq & 7) == 0;
+        const int ch = threadIdx.x & (D / 8 - 1);
         for (uint32_t unit = 0; u.next(args); ++unit) {
             if (unit > 0) wait_phase(&s_q_free, (unit - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
-#pragma unroll 4
-            for (int e = threadIdx.x & (kLoaders - 1); e < u.row_tiles() * 128 * (D / 8); e += kLoaders) {
-                const int row = e / (D / 8), ch = e - row * (D / 8);
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (row < u.rows) {
-                    const int tok = (u.row0 + row) / args.group, gh = u.row0 + row - tok * args.group;
-                    const uint16_t* src = a.q + (u.sq.first + tok) * a.ldq + (u.head * args.group + gh) * D + ch * 8;
-                    if (vec) {
-                        w = *reinterpret_cast<const uint4*>(src);
-                    } else {
+#pragma unroll 2
+            for (int row = (threadIdx.x & (kLoaders - 1)) / (D / 8); row < u.row_tiles() * 128; row += kLoaders / (D / 8)) {
+                const uint32_t dst = panel_at(q_u32 + ((row >> 7) * kPanels + (ch >> 3)) * S::kPanel, row & 127, ch & 7);
+                const bool live = row < u.rows;
+                const int tok = live ? (u.row0 + row) / args.group : 0, gh = live ? u.row0 + row - tok * args.group : 0;
+                const uint16_t* src = a.q + (u.sq.first + tok) * a.ldq + (u.head * args.group + gh) * D + ch * 8;
+                if (vec) {
+                    copy_async_16(dst, src, live);
+                } else {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (live) {
                         w.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
                         w.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
                         w.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
                         w.w = src[6] | static_cast<uint32_t>(src[7]) << 16;
                     }
+                    st_shared_16(dst, w.x, w.y, w.z, w.w);
                 }
-                const uint32_t base = q_u32 + ((row >> 7) * kPanels + (ch >> 3)) * S::kPanel;
-                st_shared_16(panel_at(base, row & 127, ch & 7), w.x, w.y, w.z, w.w);
             }
+            copy_async_commit();
+            copy_async_wait<0>();
             fence_async_smem();
             mbar_arrive(&s_q);
         }
@@ -1469,7 +1511,7 @@ static int check_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int64_t head
     // Rows and tiles are numbered in 31 bits.
     const double group = static_cast<double>(heads / kv->kv_heads), keys = static_cast<double>(batch->max_kv_len) + 128;
     const double rows = static_cast<double>(batch->tokens) * group;
-    if (rows + 512.0 * batch->seqs > 2147483647.0 || static_cast<double>(batch->seqs) * kv->kv_heads * keys / 32 > 2147483647.0 ||
+    if (rows + 512.0 * batch->seqs + keys * group > 2147483647.0 || static_cast<double>(batch->seqs) * kv->kv_heads * keys / 32 > 2147483647.0 ||
         (rows / 256 + batch->seqs) * kv->kv_heads * keys / 128 > 2147483647.0)
         return set_error(MRT_ERR_SHAPE, "too many rows and keys for one call");
     return MRT_OK;
