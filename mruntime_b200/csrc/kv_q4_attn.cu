@@ -688,15 +688,30 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
         : "memory");
 }
 
+// mbar_try_wait that may sleep up to 0.1 ms before it answers: a warp that waits
+// leaves its scheduler to the others instead of asking again and again.
+__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+        : "memory");
+    return ok != 0;
+}
+
 // Wait for a phase, bounded: after kWaitLimitNs, or once another thread of the
 // CTA has given up, the wait ends, and the kernel runs on to its end without
 // waiting (every access stays in bounds whatever was computed).  Unlike
 // mbar_wait it does not look at the device's error flag: a bad page of one
 // sequence must not end another's waits.
-__device__ __forceinline__ void wait_phase_slow(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
+__device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
     uint64_t t0 = 0;
-    for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
-        if ((it & 255u) != 0) continue;  // the clock is far away: not read in a wait that ends soon
+#pragma unroll 1
+    for (uint32_t it = 1; !try_wait_long(bar, parity); ++it) {
+        if ((it & 63u) != 0) continue;  // the clock is far away: not read in a wait that ends soon
         if (*gave_up) return;
         if (t0 == 0) t0 = globaltimer_ns();
         if (globaltimer_ns() - t0 > kWaitLimitNs) {
@@ -705,10 +720,6 @@ __device__ __forceinline__ void wait_phase_slow(uint64_t* bar, uint32_t parity, 
             return;
         }
     }
-}
-
-__device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
-    if (!mbar_try_wait(bar, parity)) wait_phase_slow(bar, parity, gave_up, flag, code);
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -725,10 +736,10 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 //                    four the odd ones
 //   warps 24, 25     S_i = Q_i K^T
 //   warps 26, 27     O_i += P_i V (P from TMEM)
-//   warps 28-31      Q into its panels
+//   warps 28-30      Q into its panels
+//   warp 31          the walk over the CTA's units, published a few ahead
 //
-// Each role walks the CTA's units by itself and meets the others only at
-// mbarriers, and units follow one another without a stop.  TMEM: two S (P in
+// Roles meet only at mbarriers, and units follow one another without a stop.  TMEM: two S (P in
 // its first half) for each row tile, O_0, O_1: the scores of the next keys are
 // there while the softmax works on these, so neither waits for the other's
 // whole chain (with 128 keys and one S a tile, softmax 4000 and products 2600
@@ -752,7 +763,7 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 constexpr int kManyRows = 256, kManyKeys = 64;
 constexpr int kSoftmaxWarps = 16, kCodesWarps = 8, kManyWarps = kSoftmaxWarps + kCodesWarps + 8;
 constexpr int kManyThreads = kManyWarps * 32;
-constexpr int kLoaders = 128;  // threads that bring Q
+constexpr int kLoaders = 96;  // threads that bring Q
 
 struct ManyPart {  // a unit that begins in a CTA's stretch and goes on
     int seq, head, row0;
@@ -900,16 +911,25 @@ __device__ __forceinline__ uint32_t nib1_f16(uint32_t w, uint32_t z64) {
     return h2_fma((w & kNib1) | 0x64006400u, kSixteenth, z64);
 }
 
+// A unit as one CTA works on it.
+struct ManyUnit {
+    int seq, head, first, n, kv;  // sequence and kv head, the sequence's first row, new and held tokens
+    int row0, rows;               // of the unit's rows
+    int t0, count;                // its key tiles that are this CTA's; count = 0: no more units
+    int whole, place;             // all of them are; where its part goes else
+    __device__ __forceinline__ int row_tiles() const { return rows > 128 ? 2 : 1; }
+};
+constexpr int kUnits = 4;  // published ahead
+
 // A CTA's stretch of the key tiles, unit by unit.
 struct ManyWalk {
-    int at, end, begin;    // tile numbers: next, end and begin of the stretch
-    int unit_at;           // where the unit begins
+    int at, end, begin;  // tile numbers: next, end and begin of the stretch
+    int unit_at, tiles;  // where the unit begins, its key tiles
     ManySeq sq;
-    int seq, head, x;      // the unit: sequence, kv head, row tile
-    int tiles, t0, count;  // its key tiles; the stretch has [t0, t0 + count) of them
-    int row0, rows;        // its first row, its rows
+    int seq, head, x;    // the unit: sequence, kv head, row tile
 
-    __device__ __forceinline__ bool next(const ManyArgs& g) {
+    __device__ __forceinline__ bool next(const ManyArgs& g, ManyUnit* u) {
+        u->count = 0;
         if (at >= end) return false;
         tiles = sq.tiles(x);
         if (at >= unit_at + tiles) {
@@ -924,15 +944,20 @@ struct ManyWalk {
             }
             tiles = sq.tiles(x);
         }
-        t0 = at - unit_at;
-        count = min(tiles - t0, end - at);
-        row0 = x * kManyRows;
-        rows = min(kManyRows, sq.n * g.group - row0);
-        at += count;
+        u->seq = seq;
+        u->head = head;
+        u->first = sq.first;
+        u->n = sq.n;
+        u->kv = sq.kv;
+        u->row0 = x * kManyRows;
+        u->rows = min(kManyRows, sq.n * g.group - u->row0);
+        u->t0 = at - unit_at;
+        u->count = min(unit_at + tiles, end) - at;
+        u->whole = u->count == tiles;
+        u->place = unit_at > begin ? 1 : 0;
+        at += u->count;
         return true;
     }
-    __device__ __forceinline__ int row_tiles() const { return rows > 128 ? 2 : 1; }
-    __device__ __forceinline__ int place() const { return unit_at > begin ? 1 : 0; }  // where its part goes
 };
 
 template <int N>
@@ -959,6 +984,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     // s_scores: S; s_probs: P; s_done: the product that used it.  s_free: O has
     // been read.  s_q, s_q_free: Q.
     __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_scores[2][2], s_probs[2][2], s_done[2][2], s_free[2], s_q, s_q_free;
+    __shared__ uint64_t s_unit_full[kUnits], s_unit_empty[kUnits];
+    __shared__ ManyUnit s_unit[kUnits];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up, s_seq, s_at, s_tiles, s_sum[kManyWarps];
     uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -980,6 +1007,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 mbar_init(&s_done[i][b], 1);
             }
             mbar_init(&s_free[i], 8);
+        }
+        for (int i = 0; i < kUnits; ++i) {
+            mbar_init(&s_unit_full[i], 1);
+            mbar_init(&s_unit_empty[i], kManyWarps - 1);  // each warp but the walker's
         }
         mbar_init(&s_q, kLoaders);
         mbar_init(&s_q_free, 2);
@@ -1008,15 +1039,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     }
     const int total = block_sum<kManyWarps>(mine, s_sum) * v.kv_heads;
     const int per = (total + args.grid - 1) / args.grid;
-    ManyWalk u;
-    u.at = u.begin = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(blockIdx.x) * per));
-    u.end = u.at + min(total - u.at, per);
-    u.seq = -1;
-    u.head = u.x = u.unit_at = 0;
-    if (u.at < u.end) {
+    ManyWalk walk;
+    walk.at = walk.begin = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(blockIdx.x) * per));
+    walk.end = walk.at + min(total - walk.at, per);
+    walk.seq = -1;
+    walk.head = walk.x = walk.unit_at = 0;
+    if (walk.at < walk.end) {
         int before = 0;
 #pragma unroll 1
-        for (int b0 = 0; u.seq < 0; b0 += kManyThreads) {  // ends: u.at < total
+        for (int b0 = 0; walk.seq < 0; b0 += kManyThreads) {  // ends: walk.at < total
             const int b = b0 + threadIdx.x;
             int t = first_tiles;
             if (b0 > 0 && b < v.seqs) {
@@ -1041,37 +1072,37 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 if (w == warp) base = before;
                 before += s_sum[w];
             }
-            if (u.at >= base + incl - t && u.at < base + incl) {
+            if (walk.at >= base + incl - t && walk.at < base + incl) {
                 s_seq = b;
                 s_at = base + incl - t;
                 s_tiles = t / v.kv_heads;
             }
             __syncthreads();
-            u.seq = s_seq;
-            u.unit_at = s_at;
+            walk.seq = s_seq;
+            walk.unit_at = s_at;
         }
-        many_seq(args, u.seq, &u.sq);
+        many_seq(args, walk.seq, &walk.sq);
         const int a_head = s_tiles;
-        u.head = (u.at - u.unit_at) / a_head;
-        u.unit_at += u.head * a_head;
-        const int off = u.at - u.unit_at;
-        int span = u.sq.count;  // the row tile lies in [x, x + span)
+        walk.head = (walk.at - walk.unit_at) / a_head;
+        walk.unit_at += walk.head * a_head;
+        const int off = walk.at - walk.unit_at;
+        int span = walk.sq.count;  // the row tile lies in [x, x + span)
         int skip = 0;           // key tiles before row tile x
 #pragma unroll 1
         while (span > 1) {
             const int step = (span + kManyThreads - 1) / kManyThreads;
-            const int mid = u.x + threadIdx.x * step;
-            const bool in = mid < u.x + span;
-            const int t = in ? many_before(u.sq, mid) : 0;
+            const int mid = walk.x + threadIdx.x * step;
+            const bool in = mid < walk.x + span;
+            const int t = in ? many_before(walk.sq, mid) : 0;
             const int n = __syncthreads_count(in && t <= off);
             if (static_cast<int>(threadIdx.x) == n - 1) s_at = t;
             __syncthreads();
             skip = s_at;
-            const int next = u.x + (n - 1) * step;
-            span = min(step, u.x + span - next);
-            u.x = next;
+            const int next = walk.x + (n - 1) * step;
+            span = min(step, walk.x + span - next);
+            walk.x = next;
         }
-        u.unit_at += skip;
+        walk.unit_at += skip;
     }
     // Key tiles so far: of the CTA, of the role's row tile.
     uint32_t stage_it = 0, tile_it = 0;
@@ -1083,8 +1114,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
         const int row_in = (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + r;  // this lane's rows of the tile: it and + 8
         const uint32_t lanes = static_cast<uint32_t>(row_in - r) << 16;
         const uint32_t t_rows = tmem + i * 128 + lanes, t_o = tmem + 256 + i * D + lanes;
-        for (; u.next(args); stage_it += u.count) {
-            if (i >= u.row_tiles()) continue;
+        for (uint32_t n = 0;; ++n) {
+            const ManyUnit& u = s_unit[n % kUnits];
+            wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+            const int count = u.count;
+            if (count == 0) break;
+            if (i < u.row_tiles()) {
             float m[2];
             uint64_t l[2];  // sums over even and over odd columns
             int limit[2], limit_min = 0x7FFFFFFF;
@@ -1095,14 +1130,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 l[b] = 0;
                 limit[b] = 0;
                 if (row < u.rows) {
-                    limit[b] = a.causal ? u.sq.kv - u.sq.n + (u.row0 + row) / args.group + 1 : u.sq.kv;
+                    limit[b] = a.causal ? u.kv - u.n + (u.row0 + row) / args.group + 1 : u.kv;
                     limit_min = min(limit_min, limit[b]);
                 }
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
 #pragma unroll 1
-            for (int j = 0; j < u.count; ++j) {
+            for (int j = 0; j < count; ++j) {
                 const uint32_t it = stage_it + j, st = it % S::kStages, t = tile_it + j, buf = t & 1;
                 const uint32_t t_s = t_rows + buf * kManyKeys;
                 const int pos0 = (u.t0 + j) * kManyKeys;
@@ -1184,12 +1219,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 if (lane == 0) mbar_arrive(&s_probs[i][buf]);
             }
             // The output, or the unit's part of it.
-            const uint32_t last = tile_it + u.count - 1;
+            const uint32_t last = tile_it + count - 1;
             wait_phase(&s_done[i][last & 1], (last >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
             __syncwarp();
             tc_fence_after();
-            const bool whole = u.t0 == 0 && u.count == u.tiles;
-            const int64_t slot = blockIdx.x * 2LL + u.place();
+            const bool whole = u.whole;
+            const int64_t slot = blockIdx.x * 2LL + u.place;
             float sums[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -1209,7 +1244,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                     if (whole) {
                         const float inv = sums[b] == 0.0f ? 0.0f : fast_rcp(sums[b]);
                         const int tok = (u.row0 + row) / args.group, gh = u.row0 + row - tok * args.group;
-                        uint16_t* dst = a.out + (u.sq.first + tok) * a.ldo + (u.head * args.group + gh) * D + ch + c * 2;
+                        uint16_t* dst = a.out + (u.first + tok) * a.ldo + (u.head * args.group + gh) * D + ch + c * 2;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             store2(dst + k * 8, narrow2(__uint_as_float(o[k * 4 + b * 2]) * inv,
@@ -1227,7 +1262,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[i]);
-            tile_it += u.count;
+            tile_it += count;
+            }
+            stage_it += count;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_unit_empty[n % kUnits]);
         }
     } else if (warp < kSoftmaxWarps + kCodesWarps) {
         // -------------------------------------------------------------- codes to operands
@@ -1242,16 +1281,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
         const int block_in = is_k ? token >> 4 : v_half >> 1;
         const int offset = is_k ? (token & 15) * (D / 2) : kv_v_codes(D) + (v_half & 1) * 4 * D + v_r * (D / 2);
         const float fac = a.scale * 1.4426950408889634f;
-        ManyPart part{0, 0, 0, 0, -1};
-        for (; u.next(args); stage_it += u.count) {
-            if (u.t0 == 0 && u.count < u.tiles)
-                part = ManyPart{u.seq, u.head, u.row0, u.place(), (u.unit_at + u.tiles - 1) / per};
+        for (uint32_t n = 0;; ++n) {
+            const ManyUnit& u = s_unit[n % kUnits];
+            wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+            const int count = u.count;
+            if (count == 0) break;
             const int32_t* row_table = v.table + static_cast<int64_t>(u.seq) * v.ld_table;
             // Lane l holds the number of block l of eight tiles (-1: none): of those under
             // way and, fetched early, of the next eight.
             auto locate = [&](int j) {
                 const int pos = (u.t0 + j) * kManyKeys + lane * kKvBlock;
-                return j + (lane >> 2) < u.count && pos < u.sq.kv ? kv_block_number(v, row_table, u.head, pos) : -2;
+                return j + (lane >> 2) < count && pos < u.kv ? kv_block_number(v, row_table, u.head, pos) : -2;
             };
             int blocks = locate(0), blocks_next = locate(8);
             uint4 w[D / 32], z[2];  // the codes; K: scales of the token, V: of the eight tokens
@@ -1279,9 +1319,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 }
             };
             const int j0 = (group ^ stage_it) & 1;
-            if (j0 < u.count) fetch(j0);
+            if (j0 < count) fetch(j0);
 #pragma unroll 1
-            for (int j = j0; j < u.count; j += 2) {
+            for (int j = j0; j < count; j += 2) {
                 const uint32_t it = stage_it + j, st = it % S::kStages;
                 if (it >= S::kStages)
                     wait_phase(&s_empty[st], (it / S::kStages - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
@@ -1355,10 +1395,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 fence_async_smem();
                 mbar_arrive(&s_full[st]);
                 __syncwarp();
-                if (j + 2 < u.count) fetch(j + 2);
+                if (j + 2 < count) fetch(j + 2);
             }
+            stage_it += count;
+            if (lane == 0) mbar_arrive(&s_unit_empty[n % kUnits]);
         }
-        if (threadIdx.x == kSoftmaxWarps * 32) args.parts[blockIdx.x] = part;
     } else if (warp < kSoftmaxWarps + kCodesWarps + 4) {
         // -------------------------------------------------------------- products
         registers_down<kOtherRegs>();
@@ -1366,15 +1407,20 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
         const uint32_t t_rows = tmem + i * 128;
         if (lane == 0 && (warp & 2) == 0) {  // scores
             const uint32_t idesc = idesc_f16_f32(128, kManyKeys) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
-            uint32_t unit = 0;
-            for (; u.next(args); stage_it += u.count, ++unit) {
-                wait_phase(&s_q, unit & 1, &s_gave_up, v.err_flag, kErrMmaWait);
-                if (i >= u.row_tiles()) {
+            for (uint32_t n = 0;; ++n) {
+                const ManyUnit& u = s_unit[n % kUnits];
+                wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                const int count = u.count, row_tiles = u.row_tiles();
+                mbar_arrive(&s_unit_empty[n % kUnits]);
+                if (count == 0) break;
+                wait_phase(&s_q, n & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                if (i >= row_tiles) {
                     mbar_arrive(&s_q_free);
+                    stage_it += count;
                     continue;
                 }
 #pragma unroll 1
-                for (int j = 0; j < u.count; ++j) {
+                for (int j = 0; j < count; ++j) {
                     const uint32_t it = stage_it + j, t = tile_it + j, buf = t & 1, st = it % S::kStages;
                     wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
                     // P in their place has been used
@@ -1389,22 +1435,29 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                     tc_commit(&s_scores[i][buf]);
                 }
                 tc_commit(&s_q_free);
-                tile_it += u.count;
+                tile_it += count;
+                stage_it += count;
             }
         } else if (lane == 0) {  // output
             const uint32_t idesc = idesc_f16_f32(128, D), t_o = tmem + 256 + i * D;
             uint32_t units = 0;  // with this row tile
-            for (; u.next(args); stage_it += u.count) {
-                if (i >= u.row_tiles()) {  // the other tile's alone: only give back what it uses
-                    for (int j = 0; j < u.count; ++j) {
+            for (uint32_t n = 0;; ++n) {
+                const ManyUnit& u = s_unit[n % kUnits];
+                wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                const int count = u.count, row_tiles = u.row_tiles();
+                mbar_arrive(&s_unit_empty[n % kUnits]);
+                if (count == 0) break;
+                if (i >= row_tiles) {  // the other tile's alone: only give back what it uses
+                    for (int j = 0; j < count; ++j) {
                         const uint32_t it = stage_it + j;
                         wait_phase(&s_full[it % S::kStages], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
                         mbar_arrive(&s_empty[it % S::kStages]);
                     }
+                    stage_it += count;
                     continue;
                 }
 #pragma unroll 1
-                for (int j = 0; j < u.count; ++j) {
+                for (int j = 0; j < count; ++j) {
                     const uint32_t it = stage_it + j, t = tile_it + j, buf = t & 1, st = it % S::kStages;
                     if (j == 0) {
                         if (units > 0) wait_phase(&s_free[i], (units - 1) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
@@ -1419,23 +1472,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                     tc_commit(&s_done[i][buf]);
                     tc_commit(&s_empty[st]);
                 }
-                tile_it += u.count;
+                tile_it += count;
+                stage_it += count;
             }
         }
         __syncwarp();
-    } else {
+    } else if (warp < kManyWarps - 1) {
         // -------------------------------------------------------------- Q, as it is
         registers_down<kOtherRegs>();
         const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.ldq & 7) == 0;
-        const int ch = threadIdx.x & (D / 8 - 1);
-        for (uint32_t unit = 0; u.next(args); ++unit) {
-            if (unit > 0) wait_phase(&s_q_free, (unit - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+        const int tid = threadIdx.x - (kManyThreads - 128), ch = tid & (D / 8 - 1);
+        for (uint32_t n = 0;; ++n) {
+            const ManyUnit& u = s_unit[n % kUnits];
+            wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+            if (u.count == 0) break;
+            if (n > 0) wait_phase(&s_q_free, (n - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
 #pragma unroll 2
-            for (int row = (threadIdx.x & (kLoaders - 1)) / (D / 8); row < u.row_tiles() * 128; row += kLoaders / (D / 8)) {
+            for (int row = tid / (D / 8); row < u.row_tiles() * 128; row += kLoaders / (D / 8)) {
                 const uint32_t dst = panel_at(q_u32 + ((row >> 7) * kPanels + (ch >> 3)) * S::kPanel, row & 127, ch & 7);
                 const bool live = row < u.rows;
                 const int tok = live ? (u.row0 + row) / args.group : 0, gh = live ? u.row0 + row - tok * args.group : 0;
-                const uint16_t* src = a.q + (u.sq.first + tok) * a.ldq + (u.head * args.group + gh) * D + ch * 8;
+                const uint16_t* src = a.q + (u.first + tok) * a.ldq + (u.head * args.group + gh) * D + ch * 8;
                 if (vec) {
                     copy_async_16(dst, src, live);
                 } else {
@@ -1453,7 +1510,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             copy_async_wait<0>();
             fence_async_smem();
             mbar_arrive(&s_q);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_unit_empty[n % kUnits]);
         }
+    } else {
+        // -------------------------------------------------------------- the walk
+        registers_down<kOtherRegs>();
+        if (lane == 0) {
+            ManyPart part{0, 0, 0, 0, -1};
+            bool more = true;
+            for (uint32_t n = 0; more; ++n) {
+                if (n >= kUnits)
+                    wait_phase(&s_unit_empty[n % kUnits], (n / kUnits - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+                ManyUnit& u = s_unit[n % kUnits];
+                more = walk.next(args, &u);
+                if (more && u.t0 == 0 && !u.whole)
+                    part = ManyPart{u.seq, u.head, u.row0, u.place, (walk.unit_at + walk.tiles - 1) / per};
+                mbar_arrive(&s_unit_full[n % kUnits]);
+            }
+            args.parts[blockIdx.x] = part;
+        }
+        __syncwarp();
     }
     // Every product has ended: each softmax waited for the last one of its tile.
     tc_fence_before();
