@@ -9,14 +9,19 @@
 // so the codes go to the tensor cores as they are and the zero points meet
 // only the group sums of x, once per (row, group).
 //
-// Layout.  Rows in tiles of 16, columns in blocks of 128; a (tile, block) is
-// 1 KB in the order of the MMA's A fragments: [row half][lane][16 bytes], lane
-// (r, c) = (lane / 4, lane % 4) holding for row r (+ 8 in the second half)
-// four words, word i = the codes of columns 32 i + 8 c .. + 7, so that each
-// 32-column stretch of the sum is one word deep in every lane (groups of 32
-// end between words) and a warp's load is 512 contiguous bytes.  Scales:
-// [tile][group][r] pairs (row r, row r + 8); zero points the same, one byte
-// with row r in the low half.  Columns past K have scale 0.
+// Layout.  Rows in tiles of 16, columns in blocks of 128; a (tile, block) is one
+// contiguous piece, brought in by one bulk copy:
+//
+//   codes   1 KB in the order of the MMA's A fragments: [row half][lane][16
+//           bytes], lane (r, c) = (lane / 4, lane % 4) holding for row r (+ 8 in
+//           the second half) four words, word i = the codes of columns 32 i + 8 c
+//           .. + 7, so that each 32-column stretch of the sum is one word deep in
+//           every lane (groups of 32 end between words)
+//   scales  [r][group of the block] FP16 pairs (row r, row r + 8)
+//   zeros   [r][group of the block] bytes, row r in the low half, padded to 16
+//           bytes; absent when every zero point is 8
+//
+// Columns past K have scale 0.
 #include <algorithm>
 #include <string>
 #include <vector>
@@ -32,17 +37,35 @@ struct mrt_weight_q4_s {
     int64_t n = 0, k = 0, group = 0;
     int64_t tiles = 0;   // ceil(n / 16)
     int64_t blocks = 0;  // ceil(k / 128)
-    uint4* codes = nullptr;      // [tiles][blocks][64]
-    uint32_t* scales = nullptr;  // [tiles][blocks * 128 / group][8] FP16 pairs
-    uint8_t* zeros = nullptr;    // [tiles][blocks * 128 / group][8], or null: every zero point is 8
+    bool zeros = false;  // zero points of its own (else all are 8)
+    int piece = 0;       // bytes of a (tile, block)
+    uint8_t* data = nullptr;
     uint16_t* bias = nullptr;    // FP16 [n] or null
 };
 
 namespace mrt {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+// Warps that a multiprocessor's registers have room for, by token tiles.
+__host__ __device__ constexpr int most_warps(int nt) { return nt == 1 ? 24 : 16; }
+
+// Barrier of the CTAs of a cluster (every thread).
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A shared-memory address as CTA `rank` of the cluster has it.
+__device__ __forceinline__ uint32_t cluster_address(uint32_t smem_addr, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
+    return a;
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
 
 __device__ __forceinline__ float ld_any(const void* p, int dt, int64_t i) {
     if (dt == MRT_FP32) return static_cast<const float*>(p)[i];
@@ -53,48 +76,71 @@ __device__ __forceinline__ float ld_any(const void* p, int dt, int64_t i) {
 // ------------------------------------------------------------------ upload
 
 struct Q4Store {
-    uint4* codes;
-    uint32_t* scales;
-    uint8_t* zeros;
+    uint8_t* data;
+    int piece, zeros;
     int64_t n, k, group, blocks;
+    __device__ __forceinline__ uint8_t* at(int64_t tile, int64_t block) const { return data + (tile * blocks + block) * piece; }
 };
 
-__device__ __forceinline__ void store_code(const Q4Store& w, int64_t n, int64_t k, uint32_t code) {
-    const int64_t tile = n >> 4, block = k >> 7;
+constexpr int kCodeBytes = 1024;
+__host__ __device__ __forceinline__ int zeros_at(int per) { return kCodeBytes + per * 32; }
+__host__ __device__ __forceinline__ int piece_bytes(int per, bool zeros) {
+    return zeros_at(per) + (zeros ? (per * 8 + 15) / 16 * 16 : 0);
+}
+
+// The word of columns k .. k + 7 (k a multiple of 8) of row n.
+__device__ __forceinline__ uint32_t* word_of(const Q4Store& w, int64_t n, int64_t k) {
     const int row = static_cast<int>(n & 15), kk = static_cast<int>(k & 127);
-    const int lane = (row & 7) * 4 + ((kk >> 3) & 3);
-    uint32_t* word = reinterpret_cast<uint32_t*>(w.codes + (tile * w.blocks + block) * 64 + (row >> 3) * 32 + lane) +
-                     (kk >> 5);
-    atomicOr(word, code << (4 * pair_nibble(kk & 7)));
+    return reinterpret_cast<uint32_t*>(w.at(n >> 4, k >> 7)) + ((row >> 3) * 32 + (row & 7) * 4 + ((kk >> 3) & 3)) * 4 + (kk >> 5);
 }
 
-__device__ __forceinline__ void store_scale(const Q4Store& w, int64_t n, int64_t g, uint16_t scale, uint32_t zero) {
-    const int64_t i = ((n >> 4) * (w.blocks * 128 / w.group) + g) * 8 + (n & 7);
-    reinterpret_cast<uint16_t*>(w.scales + i)[(n >> 3) & 1] = scale;
-    if (w.zeros != nullptr)
-        atomicOr(reinterpret_cast<uint32_t*>(w.zeros) + (i >> 2), zero << (8 * (i & 3) + 4 * ((n >> 3) & 1)));
+// Scale and zero point of group g of row n.
+__device__ __forceinline__ uint16_t* scale_of(const Q4Store& w, int64_t n, int64_t g) {
+    const int per = static_cast<int>(128 / w.group);
+    const int i = static_cast<int>(n & 7) * per + static_cast<int>(g % per);
+    return reinterpret_cast<uint16_t*>(w.at(n >> 4, g / per) + kCodeBytes) + i * 2 + ((n >> 3) & 1);
 }
 
-// One warp per (row, group).  Codes given ([n][k / 2] bytes, the even column
-// in the low half): laid out as they are.
+__device__ __forceinline__ uint8_t* zero_of(const Q4Store& w, int64_t n, int64_t g) {
+    const int per = static_cast<int>(128 / w.group);
+    return w.at(n >> 4, g / per) + zeros_at(per) + static_cast<int>(n & 7) * per + static_cast<int>(g % per);
+}
+
+// Codes given: [n][k / 2] bytes, the even column in the low half.
 __global__ void q4_import_kernel(const uint8_t* codes, const void* scales, int sdt, const uint8_t* zeros, Q4Store w) {
+    const int64_t tile = blockIdx.x / w.blocks, block = blockIdx.x - tile * w.blocks;
+    const int per = static_cast<int>(128 / w.group);
     const int64_t groups = w.k / w.group;
-    const int64_t id = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (id >= w.n * groups) return;
-    const int64_t n = id / groups, g = id - n * groups;
-    for (int j = lane; j < w.group; j += 32) {
-        const int64_t k = g * w.group + j;
-        const uint8_t b = codes[n * (w.k / 2) + (k >> 1)];
-        store_code(w, n, k, (k & 1) ? b >> 4 : b & 15u);
+    uint8_t* piece = w.at(tile, block);
+    const int t = threadIdx.x;  // one thread a word
+    const int64_t n = tile * 16 + (t >> 7) * 8 + ((t >> 4) & 7), k = block * 128 + (t & 3) * 32 + ((t >> 2) & 3) * 8;
+    uint32_t word = 0;
+    if (n < w.n && k < w.k) {
+        const uint8_t* src = codes + n * (w.k / 2) + k / 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t b = src[j];
+            word |= (b & 15u) << (4 * pair_nibble(2 * j)) | (b >> 4) << (4 * pair_nibble(2 * j + 1));
+        }
     }
-    if (lane == 0)
-        store_scale(w, n, g, f32_to_f16_bits(ld_any(scales, sdt, n * groups + g)),
-                    zeros != nullptr ? zeros[n * groups + g] & 15u : 8u);
+    reinterpret_cast<uint32_t*>(piece)[t] = word;
+    if (t < 8 * per) {  // one thread a pair of rows of a group
+        const int64_t g = block * per + t % per;
+        uint32_t pair = 0, zero = 0;
+        for (int h = 0; h < 2; ++h) {
+            const int64_t row = tile * 16 + t / per + h * 8;
+            if (row >= w.n || g >= groups) continue;
+            pair |= static_cast<uint32_t>(f32_to_f16_bits(ld_any(scales, sdt, row * groups + g))) << (16 * h);
+            if (zeros != nullptr) zero |= (zeros[row * groups + g] & 15u) << (4 * h);
+        }
+        reinterpret_cast<uint32_t*>(piece + kCodeBytes)[t] = pair;
+        if (w.zeros) piece[zeros_at(per) + t] = static_cast<uint8_t>(zero);
+    }
 }
 
 // Codes from a full-precision weight: round to nearest on the group's range,
-// widened to hold zero (asymmetric) or centred on code 8 (symmetric).
+// widened to hold zero (asymmetric) or centred on code 8 (symmetric).  One warp
+// per (row, group); storage is zeroed before.
 __global__ void q4_quantise_kernel(const void* src, int dt, Q4Store w) {
     const int64_t groups = w.k / w.group;
     const int64_t id = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
@@ -112,16 +158,25 @@ __global__ void q4_quantise_kernel(const void* src, int dt, Q4Store w) {
         lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
     }
-    const float step = w.zeros != nullptr ? __fmul_rn(hi - lo, 1.0f / 15.0f) : __fmul_rn(fmaxf(-lo, hi), 1.0f / 7.0f);
+    const float step = w.zeros ? __fmul_rn(hi - lo, 1.0f / 15.0f) : __fmul_rn(fmaxf(-lo, hi), 1.0f / 7.0f);
     const uint16_t sb = f32_to_f16_bits(fminf(fmaxf(step, 5.9604644775390625e-8f), 65504.0f));
     const float inv = __fdiv_rn(1.0f, f16_bits_to_f32(sb));
-    const float z = w.zeros != nullptr ? fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f) : 8.0f;
+    const float z = w.zeros ? fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f) : 8.0f;
     for (int j = lane; j < w.group; j += 32) {
         const int64_t k = g * w.group + j;
         const float c = rintf(__fmul_rn(ld_any(src, dt, n * w.k + k), inv)) + z;
-        store_code(w, n, k, static_cast<uint32_t>(fminf(fmaxf(c, 0.0f), 15.0f)));  // NaN becomes code 0
+        const uint32_t code = static_cast<uint32_t>(fminf(fmaxf(c, 0.0f), 15.0f));  // NaN becomes code 0
+        atomicOr(word_of(w, n, k), code << (4 * pair_nibble(static_cast<int>(k & 7))));
     }
-    if (lane == 0) store_scale(w, n, g, sb, static_cast<uint32_t>(z));
+    if (lane == 0) {
+        *scale_of(w, n, g) = sb;
+        if (w.zeros) {
+            uint8_t* p = zero_of(w, n, g);
+            const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+            atomicOr(reinterpret_cast<uint32_t*>(a & ~uintptr_t(3)),
+                     static_cast<uint32_t>(z) << (8 * (a & 3) + 4 * ((n >> 3) & 1)));
+        }
+    }
 }
 
 __global__ void q4_read_kernel(Q4Store w, uint16_t* dst, int64_t ld) {
@@ -129,25 +184,18 @@ __global__ void q4_read_kernel(Q4Store w, uint16_t* dst, int64_t ld) {
     for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < total;
          e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t n = e / w.k, k = e - n * w.k;
-        const int row = static_cast<int>(n & 15), kk = static_cast<int>(k & 127);
-        const int lane = (row & 7) * 4 + ((kk >> 3) & 3);
-        const uint32_t word = reinterpret_cast<const uint32_t*>(w.codes + ((n >> 4) * w.blocks + (k >> 7)) * 64 +
-                                                                (row >> 3) * 32 + lane)[kk >> 5];
-        const int c = (word >> (4 * pair_nibble(kk & 7))) & 15;
-        const int64_t i = ((n >> 4) * (w.blocks * 128 / w.group) + k / w.group) * 8 + (n & 7);
-        const float s = f16_bits_to_f32(reinterpret_cast<const uint16_t*>(w.scales + i)[(n >> 3) & 1]);
-        const int z = w.zeros != nullptr ? (w.zeros[i] >> (4 * ((n >> 3) & 1))) & 15 : 8;
-        dst[n * ld + k] = f32_to_f16_bits(__fmul_rn(s, static_cast<float>(c - z)));
+        const int c = (*word_of(w, n, k) >> (4 * pair_nibble(static_cast<int>(k & 7)))) & 15;
+        const int z = w.zeros ? (*zero_of(w, n, k / w.group) >> (4 * ((n >> 3) & 1))) & 15 : 8;
+        dst[n * ld + k] = f32_to_f16_bits(__fmul_rn(f16_bits_to_f32(*scale_of(w, n, k / w.group)), static_cast<float>(c - z)));
     }
 }
 
 // ------------------------------------------------------------------ product
 
 struct GemvQ4Args {
-    const uint4* codes;
-    const uint32_t* scales;
-    const uint8_t* zeros;  // or null: 8
-    int n, k, blocks, group;
+    const uint8_t* data;
+    int piece, zeros;
+    int n, k, blocks, tiles;
     const uint16_t* x;
     int64_t ldx;
     int x_vec;  // x rows can be read 16 bytes at a time
@@ -158,173 +206,379 @@ struct GemvQ4Args {
     const uint16_t* res;
     int64_t ldr;
     int M;
-    int chunk;  // column blocks of x in shared memory at a time
+    int wk;         // warps of a tile (they take its column blocks in turn)
+    int slice;      // column blocks of a CTA
+    int stages;     // pieces that a warp has under way
+    int* err_flag;
 };
 
 // Two token tiles of eight at most in one launch.
 constexpr int kMaxTokens = 16;
+constexpr int kMaxStages = 4, kMinStages = 2;
+constexpr int kPair = 2;  // neighbouring pieces that a stage holds
+constexpr int kSmemMost = 218 * 1024;  // of a multiprocessor's CTAs together
 
-// Bytes of dynamic shared memory: x rows (padded so that eight rows land in
-// different banks) and their group sums.
-__host__ __device__ __forceinline__ int x_stride(int chunk) { return chunk * 256 + 64; }
+// Shared memory: the warps' rings; x rows of the CTA's columns, 64 bytes apart
+// from a multiple of 128 so that eight rows' reads fall into different banks;
+// their group sums; sums of the warps of a tile.
+__host__ __device__ __forceinline__ int x_stride(int slice) { return slice * 256 + 64; }
+__host__ __device__ __forceinline__ int gemv_smem(int M, int slice, int per, int nt, int warps, bool sums, int stages, int piece) {
+    return warps * stages * kPair * piece + M * x_stride(slice) + slice * per * nt * 32 + (sums ? 2 * warps * 16 * nt * 32 : 0);
+}
 
-// One CTA per 16 rows, its eight warps taking the column blocks in turn.  x is
-// staged in shared memory chunk by chunk together with its group sums.
-template <int NT>
-__global__ void __launch_bounds__(kThreads) gemv_q4_kernel(const GemvQ4Args a) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float red[kWarps][16][NT * 8];
+// Wait for a bulk copy, bounded like every wait of the library; once one has
+// given up (`late`) the warp's others hardly wait.
+__device__ __forceinline__ void wait_piece(uint64_t* bar, uint32_t parity, int* flag, bool& late) {
+    uint64_t t0 = 0;
+#pragma unroll 1
+    for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
+        if ((it & 255u) != 0) continue;
+        if (t0 == 0) t0 = globaltimer_ns();
+        if (globaltimer_ns() - t0 > (late ? kWaitLimitNs >> 10 : kWaitLimitNs)) {
+            late = true;
+            raise_error(flag, kErrTmaWait);
+            return;
+        }
+    }
+}
+
+__device__ __forceinline__ void store_y(const GemvQ4Args& a, int64_t n, int m, float sum) {
+    const float v = sum * 16777216.0f;
+    if (a.out_f32) {
+        static_cast<float*>(a.y)[m * a.ldy + n] = v;
+    } else {
+        const uint16_t h = round_out(v, a.bias, n);
+        static_cast<uint16_t*>(a.y)[m * a.ldy + n] = add_residual(h, a.res, m * a.ldr + n);
+    }
+}
+
+// What bounds it: for few tokens the weights' bytes, so every warp keeps up to
+// eight pieces of them under way (two a copy), the first before it waits for the kernel that
+// makes x (with loads into registers, four deep, a warp waited for more than it
+// asked for: 21.5 us for 37888 x 3584 at one token); for 16 tokens, beside them, x
+// from shared memory (eight KB a KB of codes, in FP16).  x is brought in once a
+// CTA, with its group sums, and CTAs stay for all the row tiles they take.
+//
+// Split.  A multiprocessor holds one CTA of 24 or 16 warps (one or two token
+// tiles), or two or three smaller ones; wk of a CTA's warps share a tile.  Grid x takes the tiles in turn; grid y cuts the columns into
+// slices, one a CTA, whose sums the CTAs of a cluster (1, KS) add through each
+// other's shared memory in slice order, each a part of the rows.  wk and KS by
+// plan_gemv().
+template <int PER, int NT, bool ZEROS>
+__global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const GemvQ4Args a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t s_full[most_warps(NT)][kMaxStages];
+    const int warps = blockDim.x >> 5, threads = blockDim.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const int tile = blockIdx.x;
-    const int per_block = 128 / a.group;  // groups in a column block
-    const int stride = x_stride(a.chunk);
-    float* xs = reinterpret_cast<float*>(smem + a.M * stride);  // [group of the chunk][NT * 8]
+    const int stage_bytes = kPair * a.piece;
+    uint8_t* ring = smem + warp * a.stages * stage_bytes;
+    uint8_t* xb = smem + warps * a.stages * stage_bytes;
+    const int stride = x_stride(a.slice);
+    float* xs = reinterpret_cast<float*>(xb + a.M * stride);  // [group of the slice][NT * 8]
+    float* red = xs + a.slice * PER * NT * 8;                 // [2][warp][16][NT * 8]
+    const int b0 = blockIdx.y * a.slice, nb = min(a.slice, a.blocks - b0);
+    const int wt = warp / a.wk, wi = warp - wt * a.wk, per_cta = warps / a.wk;
+
+    // The warp's pieces, in order: of its tiles the block pairs wi, wi + wk, ..
+    const int pairs = (nb + kPair - 1) / kPair, mine = pairs > wi ? (pairs - wi + a.wk - 1) / a.wk : 0;
+    const int step = gridDim.x * per_cta;
+    // The next pair to fetch (lane 0's).
+    int f_tile = mine > 0 ? blockIdx.x * per_cta + wt : a.tiles, f_block = wi * kPair;
+    const uint8_t* f_src = a.data + (static_cast<int64_t>(f_tile) * a.blocks + b0) * a.piece;
+    auto fetch = [&](int stage) {
+        if (lane != 0 || f_tile >= a.tiles) return;
+        const uint32_t bytes = nb - f_block >= kPair ? stage_bytes : a.piece;
+        mbar_arrive_expect_tx(&s_full[warp][stage], bytes);
+        bulk_load(ring + stage * stage_bytes, f_src + f_block * a.piece, bytes, &s_full[warp][stage]);
+        f_block += a.wk * kPair;
+        if (f_block >= nb) {
+            f_block = wi * kPair;
+            f_tile += step;
+            f_src += static_cast<int64_t>(step) * a.blocks * a.piece;
+        }
+    };
+    if (lane == 0) {
+        for (int i = 0; i < a.stages; ++i) mbar_init(&s_full[warp][i], 1);
+        fence_barrier_init();
+    }
+    __syncwarp();
+    for (int i = 0; i < a.stages; ++i) fetch(i);
 
     griddep_wait();
     griddep_launch_dependents();
-    float tot[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) tot[t][j] = 0.0f;
-
-    for (int b0 = 0; b0 < a.blocks; b0 += a.chunk) {
-        const int nb = min(a.chunk, a.blocks - b0);
-        __syncthreads();
-        // Stage x: 8 columns per thread and step, their sum to the group's.
-        for (int i = threadIdx.x; i < (a.M * nb * 16 + 31) / 32 * 32; i += kThreads) {
-            const int m = i / (nb * 16), p = i - m * nb * 16;
-            const int k = b0 * 128 + p * 8;
+    // x, 8 columns a thread and step; then the groups' sums.
+    const int row_chunks = nb * 16, chunks = a.M * row_chunks;
+    for (int i = threadIdx.x; i < chunks; i += threads) {
+        const int m = i / row_chunks, p = i - m * row_chunks;
+        const int k = b0 * 128 + p * 8;
+        const bool in = k < a.k;  // K is a multiple of 32
+        const uint16_t* src = in ? a.x + m * a.ldx + k : a.x;
+        uint8_t* dst = xb + m * stride + p * 16;
+        if (a.x_vec) {
+            copy_async_16(smem_u32(dst), src, in);
+        } else {
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (m < a.M && k < a.k) {  // K is a multiple of 32
-                const uint16_t* src = a.x + m * a.ldx + k;
-                if (a.x_vec) {
-                    v = *reinterpret_cast<const uint4*>(src);
-                } else {
-                    v.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
-                    v.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
-                    v.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
-                    v.w = src[6] | static_cast<uint32_t>(src[7]) << 16;
-                }
+            if (in) {
+                v.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
+                v.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
+                v.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
+                v.w = src[6] | static_cast<uint32_t>(src[7]) << 16;
             }
+            *reinterpret_cast<uint4*>(dst) = v;
+        }
+    }
+    copy_async_commit();
+    copy_async_wait<0>();
+    __syncthreads();
+    for (int i = threadIdx.x; i < (chunks + 31) / 32 * 32; i += threads) {
+        const int m = i / row_chunks, p = i - m * row_chunks;
+        float s = 0.0f;
+        if (m < a.M) {
+            const uint4 v = *reinterpret_cast<const uint4*>(xb + m * stride + p * 16);
             const uint32_t h[4] = {v.x, v.y, v.z, v.w};
-            float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
                 s += f.x + f.y;
             }
-            for (int o = 1; o < a.group / 8; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-            if (m < a.M) {
-                *reinterpret_cast<uint4*>(smem + m * stride + p * 16) = v;
-                if ((p & (a.group / 8 - 1)) == 0) xs[(p / (a.group / 8)) * NT * 8 + m] = s * 5.9604644775390625e-8f;
-            }
         }
-        __syncthreads();
-        for (int b = warp; b < nb; b += kWarps) {
-            const uint4* src = a.codes + (static_cast<int64_t>(tile) * a.blocks + b0 + b) * 64 + lane;
-            const uint4 lo = ld_stream_16B(src), hi = ld_stream_16B(src + 32);
-            const uint32_t w0[4] = {lo.x, lo.y, lo.z, lo.w}, w1[4] = {hi.x, hi.y, hi.z, hi.w};
-            float ev[NT][4], od[NT][4];
+        constexpr int kLanes = 16 / PER;  // lanes of a group
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (i % (a.group / 32) == 0) {
+        for (int o = 1; o < kLanes; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        if (m < a.M && (p & (kLanes - 1)) == 0) xs[(p / kLanes) * NT * 8 + m] = s * 5.9604644775390625e-8f;
+    }
+    __syncthreads();
+
+    int turn = 0, stage = 0;
+    uint32_t phase = 0;
+    bool late = false;
+    // Columns past M of a token tile repeat its last token: never stored.
+    const uint8_t* x_row[NT];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) x_row[t] = xb + min(t * 8 + r, a.M - 1) * stride + c * 16;
+    for (int tile0 = blockIdx.x * per_cta; tile0 < a.tiles; tile0 += step, turn ^= 1) {
+        float tot[NT][4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) ev[t][j] = od[t][j] = 0.0f;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tot[t][j] = 0.0f;
+        const int tile = tile0 + wt;
+#pragma unroll 1
+        for (int b = tile < a.tiles ? wi * kPair : nb; b < nb; b += a.wk * kPair) {
+            wait_piece(&s_full[warp][stage], phase, a.err_flag, late);
+            const uint8_t* piece = ring + stage * stage_bytes;
+            uint4 lo[kPair], hi[kPair];
+            uint32_t sp[kPair][PER], zp[kPair];
+#pragma unroll
+            for (int u = 0; u < kPair; ++u, piece += a.piece) {  // (of a lone block the second is an old one: not used)
+                lo[u] = *reinterpret_cast<const uint4*>(piece + lane * 16);
+                hi[u] = *reinterpret_cast<const uint4*>(piece + 512 + lane * 16);
+                if constexpr (PER == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(piece + kCodeBytes + r * 16);
+                    sp[u][0] = v.x; sp[u][1] = v.y; sp[u][2] = v.z; sp[u][3] = v.w;
+                    zp[u] = ZEROS ? *reinterpret_cast<const uint32_t*>(piece + zeros_at(PER) + r * 4) : 0u;
+                } else if constexpr (PER == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(piece + kCodeBytes + r * 8);
+                    sp[u][0] = v.x; sp[u][1] = v.y;
+                    zp[u] = ZEROS ? *reinterpret_cast<const uint16_t*>(piece + zeros_at(PER) + r * 2) : 0u;
+                } else {
+                    sp[u][0] = *reinterpret_cast<const uint32_t*>(piece + kCodeBytes + r * 4);
+                    zp[u] = ZEROS ? piece[zeros_at(PER) + r] : 0u;
                 }
-                const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
+            }
+            __syncwarp();
+            fetch(stage);
+            if (++stage == a.stages) {
+                stage = 0;
+                phase ^= 1;
+            }
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (t * 8 + r < a.M)
-                        x = *reinterpret_cast<const uint4*>(smem + (t * 8 + r) * stride + b * 256 + i * 64 + c * 16);
-                    mma_f16(ev[t], w0[i] & kNib0, w1[i] & kNib0, u0 & kNib0, u1 & kNib0, x.x, x.z);
-                    mma_f16(od[t], w0[i] & kNib1, w1[i] & kNib1, u0 & kNib1, u1 & kNib1, x.y, x.w);
-                }
-                if ((i + 1) % (a.group / 32) == 0) {  // the group ends here
-                    const int g = b * per_block + i / (a.group / 32);
-                    const int64_t gi = (static_cast<int64_t>(tile) * a.blocks * per_block + b0 * per_block + g) * 8 + r;
-                    const uint32_t sp = __ldg(a.scales + gi);
-                    const uint32_t zp = a.zeros != nullptr ? __ldg(a.zeros + gi) : 0x88u;
-                    const float s0 = f16_bits_to_f32(static_cast<uint16_t>(sp)), s1 = f16_bits_to_f32(static_cast<uint16_t>(sp >> 16));
-                    const float z0 = static_cast<float>(zp & 15u), z1 = static_cast<float>(zp >> 4);
+            for (int u = 0; u < kPair; ++u) {
+                if (b + u >= nb) break;
+                const uint32_t w0[4] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w}, w1[4] = {hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+                float ev[NT][4], od[NT][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    constexpr int kWords = 4 / PER;  // of a group
+                    const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        const float2 sx = *reinterpret_cast<const float2*>(xs + g * NT * 8 + t * 8 + c * 2);
-                        const float x0 = t * 8 + c * 2 < a.M ? sx.x : 0.0f, x1 = t * 8 + c * 2 + 1 < a.M ? sx.y : 0.0f;
-                        tot[t][0] = fmaf(s0, fmaf(-z0, x0, fmaf(od[t][0], 0.0625f, ev[t][0])), tot[t][0]);
-                        tot[t][1] = fmaf(s0, fmaf(-z0, x1, fmaf(od[t][1], 0.0625f, ev[t][1])), tot[t][1]);
-                        tot[t][2] = fmaf(s1, fmaf(-z1, x0, fmaf(od[t][2], 0.0625f, ev[t][2])), tot[t][2]);
-                        tot[t][3] = fmaf(s1, fmaf(-z1, x1, fmaf(od[t][3], 0.0625f, ev[t][3])), tot[t][3]);
+                        const uint4 x = *reinterpret_cast<const uint4*>(x_row[t] + (b + u) * 256 + i * 64);
+                        if (i % kWords == 0) {
+                            mma_f16_first(ev[t], w0[i] & kNib0, w1[i] & kNib0, u0 & kNib0, u1 & kNib0, x.x, x.y);
+                            mma_f16_first(od[t], w0[i] & kNib1, w1[i] & kNib1, u0 & kNib1, u1 & kNib1, x.z, x.w);
+                        } else {
+                            mma_f16(ev[t], w0[i] & kNib0, w1[i] & kNib0, u0 & kNib0, u1 & kNib0, x.x, x.y);
+                            mma_f16(od[t], w0[i] & kNib1, w1[i] & kNib1, u0 & kNib1, u1 & kNib1, x.z, x.w);
+                        }
+                    }
+                    if ((i + 1) % kWords == 0) {  // the group ends here
+                        const int g = i / kWords;
+                        const float s0 = f16_bits_to_f32(static_cast<uint16_t>(sp[u][g])), s1 = f16_bits_to_f32(static_cast<uint16_t>(sp[u][g] >> 16));
+                        const float z0 = ZEROS ? static_cast<float>((zp[u] >> (8 * g)) & 15u) : 8.0f;
+                        const float z1 = ZEROS ? static_cast<float>((zp[u] >> (8 * g + 4)) & 15u) : 8.0f;
+                        const float* xg = xs + ((b + u) * PER + g) * NT * 8 + c * 2;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            const float2 sx = *reinterpret_cast<const float2*>(xg + t * 8);
+                            tot[t][0] = fmaf(s0, fmaf(-z0, sx.x, fmaf(od[t][0], 0.0625f, ev[t][0])), tot[t][0]);
+                            tot[t][1] = fmaf(s0, fmaf(-z0, sx.y, fmaf(od[t][1], 0.0625f, ev[t][1])), tot[t][1]);
+                            tot[t][2] = fmaf(s1, fmaf(-z1, sx.x, fmaf(od[t][2], 0.0625f, ev[t][2])), tot[t][2]);
+                            tot[t][3] = fmaf(s1, fmaf(-z1, sx.y, fmaf(od[t][3], 0.0625f, ev[t][3])), tot[t][3]);
+                        }
                     }
                 }
             }
         }
-    }
+        if (a.wk == 1 && gridDim.y == 1) {  // the warp has whole sums
+            const int64_t n = tile * 16LL + r;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        red[warp][r][t * 8 + c * 2] = tot[t][0];
-        red[warp][r][t * 8 + c * 2 + 1] = tot[t][1];
-        red[warp][r + 8][t * 8 + c * 2] = tot[t][2];
-        red[warp][r + 8][t * 8 + c * 2 + 1] = tot[t][3];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * NT * 8; i += kThreads) {
-        const int row = i & 15, m = i >> 4;
-        const int64_t n = tile * 16LL + row;
-        if (m >= a.M || n >= a.n) continue;
-        float s = 0.0f;
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += red[w][row][m];
-        s *= 16777216.0f;
-        if (a.out_f32) {
-            static_cast<float*>(a.y)[m * a.ldy + n] = s;
+                for (int j = 0; j < 4; ++j) {
+                    const int m = t * 8 + c * 2 + (j & 1);
+                    const int64_t row = n + (j >> 1) * 8;
+                    if (tile < a.tiles && m < a.M && row < a.n) store_y(a, row, m, tot[t][j]);
+                }
+            continue;
+        }
+        float* part = red + turn * warps * 16 * NT * 8;  // the other turn's may still be read
+        float* p = part + warp * 16 * NT * 8;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            *reinterpret_cast<float2*>(p + r * NT * 8 + t * 8 + c * 2) = make_float2(tot[t][0], tot[t][1]);
+            *reinterpret_cast<float2*>(p + (r + 8) * NT * 8 + t * 8 + c * 2) = make_float2(tot[t][2], tot[t][3]);
+        }
+        const int rows = per_cta * 16;
+        if (gridDim.y == 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < rows * NT * 8; i += threads) {
+                const int m = i / rows, row = i - m * rows;  // neighbouring threads, neighbouring rows
+                const int64_t n = tile0 * 16LL + row;
+                if (m >= a.M || n >= a.n) continue;
+                const float* q = part + ((row >> 4) * a.wk * 16 + (row & 15)) * NT * 8 + m;
+                float s = 0.0f;
+                for (int w = 0; w < a.wk; ++w) s += q[w * 16 * NT * 8];
+                store_y(a, n, m, s);
+            }
         } else {
-            const uint16_t h = round_out(s, a.bias, n);
-            static_cast<uint16_t*>(a.y)[m * a.ldy + n] = add_residual(h, a.res, m * a.ldr + n);
+            // Slices of a cluster: this launch has one turn, so nothing is written again.
+            cluster_barrier();
+            const int rank = blockIdx.y, ranks = gridDim.y;
+            for (int i = threadIdx.x + rank * threads; i < rows * NT * 8; i += threads * ranks) {
+                const int m = i / rows, row = i - m * rows;
+                const int64_t n = tile0 * 16LL + row;
+                if (m >= a.M || n >= a.n) continue;
+                const uint32_t at = smem_u32(part + ((row >> 4) * a.wk * 16 + (row & 15)) * NT * 8 + m);
+                float s = 0.0f;
+                for (int k = 0; k < ranks; ++k)
+                    for (int w = 0; w < a.wk; ++w) s += ld_cluster_f32(cluster_address(at, k) + w * 16 * NT * 8 * 4);
+                store_y(a, n, m, s);
+            }
+            cluster_barrier();  // the others have read this CTA's sums
         }
     }
 }
 
-template <int NT>
-cudaError_t launch(const GemvQ4Args& a, cudaStream_t s) {
-    const int smem = a.M * x_stride(a.chunk) + a.chunk * (128 / a.group) * NT * 8 * 4;
+struct GemvPlan {
+    int warps, wk, ks;
+    int per_sm;  // CTAs a multiprocessor
+};
+
+// Candidates by time, in microseconds.  A multiprocessor works off a piece in
+// 0.036 us when its warps are many, a warp alone in 0.35 us; x comes into every
+// CTA from L2; larger CTAs start later, and joining sums costs.
+GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
+    GemvPlan best{0, 0, 0, 0};
+    double best_us = 0.0;
+    const int nt = M <= 8 ? 1 : 2;
+    for (int per_sm = nt == 1 ? 3 : 2; per_sm > 0; --per_sm)
+        for (int ks = 1; ks <= 8; ks *= 2)
+            for (int wk : {1, 2, 4, 8, 12, 16, 24}) {
+                const int warps = most_warps(nt) / per_sm, slice = (blocks + ks - 1) / ks;
+                if (warps % wk != 0 || (ks > 1 && (ks - 1) * slice >= blocks) || (wk > 1 && (wk - 1) * kPair >= slice)) continue;
+                if (gemv_smem(M, slice, per, nt, warps, wk * ks > 1, kMinStages, piece) > kSmemMost / per_sm) continue;
+                const int per_cta = warps / wk;
+                const int64_t ctas = static_cast<int64_t>((tiles + per_cta - 1) / per_cta) * ks, room = static_cast<int64_t>(sms) * per_sm;
+                if (ks > 1 && ctas > room) continue;  // slices' CTAs take one turn
+                const int64_t turns = (ctas + room - 1) / room, live = std::min(ctas, room);
+                const int warp_pieces = (slice + wk * kPair - 1) / (wk * kPair) * kPair;
+                const double sm_pieces = static_cast<double>((live + sms - 1) / sms) * turns * per_cta * slice;
+                const double work = std::max(sm_pieces * (nt == 1 ? 0.036 : 0.046), turns * warp_pieces * 0.35);
+                const double x = (live * 256.0 / 8.0e6 + 0.0025 * per_sm) * M * slice / (per_sm == 1 ? 1.0 : 1.0);
+                const double us = work + x + 0.05 * warps + (wk > 1 ? 0.3 * turns : 0.0) + (ks > 1 ? 1.5 : 0.0);
+                if (best.wk == 0 || us < best_us) {
+                    best = GemvPlan{warps, wk, ks, per_sm};
+                    best_us = us;
+                }
+            }
+    return best;
+}
+
+template <int PER, int NT, bool ZEROS>
+cudaError_t launch(GemvQ4Args a, const GemvPlan& p, int sms, cudaStream_t s) {
+    a.stages = kMaxStages;
+    auto bytes = [&] { return gemv_smem(a.M, a.slice, PER, NT, p.warps, p.wk * p.ks > 1, a.stages, a.piece); };
+    while (bytes() > kSmemMost / p.per_sm) --a.stages;
+    if (a.stages < kMinStages) return cudaErrorInvalidValue;  // (the plan says that they fit)
+    cudaError_t e = cudaFuncSetAttribute(gemv_q4_kernel<PER, NT, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (e != cudaSuccess) return e;
+    const int per_cta = p.warps / p.wk, ctas = (a.tiles + per_cta - 1) / per_cta;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.n + 15) / 16));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(static_cast<unsigned>(p.ks > 1 ? ctas : std::min(ctas, sms * p.per_sm)), static_cast<unsigned>(p.ks));
+    cfg.blockDim = dim3(static_cast<unsigned>(p.warps) * 32);
+    cfg.dynamicSmemBytes = static_cast<size_t>(bytes());
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = static_cast<unsigned>(p.ks);
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemv_q4_kernel<NT>, a);
+    cfg.numAttrs = p.ks > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, gemv_q4_kernel<PER, NT, ZEROS>, a);
     if (e == cudaSuccess) note_launches(1);
     return e;
 }
 
-cudaError_t launch_gemv_q4(GemvQ4Args a, cudaStream_t s) {
-    // The chunk of x that fits 32 KB (48 KB is what a launch has without asking).
-    a.chunk = std::max(1, std::min(a.blocks, 32768 / (a.M * 256 + (128 / a.group) * 64)));
-    return a.M <= 8 ? launch<1>(a, s) : launch<2>(a, s);
+// Tokens of one launch: sixteen, or as many as leave x room in shared memory
+// (0: not even one does).
+int tokens_at_once(int64_t M, int tiles, int blocks, int per, int piece, int sms, GemvPlan* plan) {
+    for (int m = static_cast<int>(std::min<int64_t>(M, kMaxTokens)); m > 0; m = m > 8 ? 8 : m / 2) {
+        *plan = plan_gemv(m, tiles, blocks, per, piece, sms);
+        if (plan->wk > 0) return m;
+    }
+    return 0;
 }
+
+cudaError_t launch_gemv_q4(GemvQ4Args a, const GemvPlan& p, int per, int sms, cudaStream_t s) {
+    a.wk = p.wk;
+    a.slice = (a.blocks + p.ks - 1) / p.ks;
+    const bool z = a.zeros != 0;
+    switch (per * 2 + (a.M > 8)) {
+        case 2: return z ? launch<1, 1, true>(a, p, sms, s) : launch<1, 1, false>(a, p, sms, s);
+        case 3: return z ? launch<1, 2, true>(a, p, sms, s) : launch<1, 2, false>(a, p, sms, s);
+        case 4: return z ? launch<2, 1, true>(a, p, sms, s) : launch<2, 1, false>(a, p, sms, s);
+        case 5: return z ? launch<2, 2, true>(a, p, sms, s) : launch<2, 2, false>(a, p, sms, s);
+        case 8: return z ? launch<4, 1, true>(a, p, sms, s) : launch<4, 1, false>(a, p, sms, s);
+        default: return z ? launch<4, 2, true>(a, p, sms, s) : launch<4, 2, false>(a, p, sms, s);
+    }
+}
+
 
 // ------------------------------------------------------------------ handles
 
 void free_handle(mrt_weight_q4_s* w) {
     if (w == nullptr) return;
-    if (w->codes) cudaFree(w->codes);
-    if (w->scales) cudaFree(w->scales);
-    if (w->zeros) cudaFree(w->zeros);
+    if (w->data) cudaFree(w->data);
     if (w->bias) cudaFree(w->bias);
     delete w;
 }
 
 Q4Store store_of(const mrt_weight_q4_s* w) {
-    return Q4Store{w->codes, w->scales, w->zeros, w->n, w->k, w->group, w->blocks};
+    return Q4Store{w->data, w->piece, w->zeros ? 1 : 0, w->n, w->k, w->group, w->blocks};
 }
 
 int check_shape(int64_t N, int64_t K, int64_t group) {
@@ -332,13 +586,14 @@ int check_shape(int64_t N, int64_t K, int64_t group) {
     if (N <= 0 || K <= 0 || N > (1LL << 31) - 16 || K > (1LL << 31) - 128)
         return set_error(MRT_ERR_SHAPE, "N and K must be positive and fit in 31 bits");
     if (K % group != 0) return set_error(MRT_ERR_SHAPE, "K must be a multiple of the group");
+    if ((N + 15) / 16 * ((K + 127) / 128) > (1LL << 31) - 1) return set_error(MRT_ERR_SHAPE, "the weight is too large");
     return MRT_OK;
 }
 
 bool any_dtype(int dt) { return dt == MRT_FP16 || dt == MRT_BF16 || dt == MRT_FP32; }
 size_t dtype_size(int dt) { return dt == MRT_FP32 ? 4 : 2; }
 
-// Handle with zeroed storage (codes and zero points are OR-ed in).
+// Handle with its storage, zeroed.
 int new_handle(int64_t N, int64_t K, int64_t group, bool zeros, cudaStream_t s, mrt_weight_q4_s** out) {
     DevCtx* c = current_ctx();
     if (!c) return MRT_ERR_CUDA;
@@ -349,14 +604,11 @@ int new_handle(int64_t N, int64_t K, int64_t group, bool zeros, cudaStream_t s, 
     w->group = group;
     w->tiles = (N + 15) / 16;
     w->blocks = (K + 127) / 128;
-    const size_t cb = static_cast<size_t>(w->tiles) * w->blocks * 1024;
-    const size_t gs = static_cast<size_t>(w->tiles) * (w->blocks * 128 / group) * 8;
-    cudaError_t e = cudaMalloc(&w->codes, cb);
-    if (e == cudaSuccess) e = cudaMalloc(&w->scales, gs * 4);
-    if (e == cudaSuccess && zeros) e = cudaMalloc(&w->zeros, gs);
-    if (e == cudaSuccess) e = cudaMemsetAsync(w->codes, 0, cb, s);
-    if (e == cudaSuccess) e = cudaMemsetAsync(w->scales, 0, gs * 4, s);
-    if (e == cudaSuccess && zeros) e = cudaMemsetAsync(w->zeros, 0, gs, s);
+    w->zeros = zeros;
+    w->piece = piece_bytes(static_cast<int>(128 / group), zeros);
+    const size_t bytes = static_cast<size_t>(w->tiles) * w->blocks * w->piece;
+    cudaError_t e = cudaMalloc(&w->data, bytes);
+    if (e == cudaSuccess) e = cudaMemsetAsync(w->data, 0, bytes, s);
     if (e != cudaSuccess) {
         free_handle(w);
         return cuda_error(e, "allocating 4-bit weight storage");
@@ -376,6 +628,7 @@ cudaError_t on_device(const void* src, size_t bytes, int src_on_device, cudaStre
     return e;
 }
 
+constexpr int kThreads = 256;  // of the upload kernels
 unsigned warp_blocks(int64_t warps) { return static_cast<unsigned>((warps * 32 + kThreads - 1) / kThreads); }
 
 int finish(mrt_weight_q4_s* w, cudaError_t e, cudaStream_t s, mrt_weight_q4* out) {
@@ -439,7 +692,7 @@ extern "C" int mrt_weight_q4_import(const void* codes, const void* scales, int s
     if (e == cudaSuccess) e = on_device(scales, ng * dtype_size(scale_dtype), src_on_device, s, &ds, &ss);
     if (e == cudaSuccess) e = on_device(zeros, ng, src_on_device, s, &dz, &sz);
     if (e == cudaSuccess) {
-        q4_import_kernel<<<warp_blocks(static_cast<int64_t>(ng)), kThreads, 0, s>>>(
+        q4_import_kernel<<<static_cast<unsigned>(w->tiles * w->blocks), 256, 0, s>>>(
             static_cast<const uint8_t*>(dc), ds, scale_dtype, static_cast<const uint8_t*>(dz), store_of(w));
         note_launches(1);
         e = cudaGetLastError();
@@ -523,25 +776,29 @@ extern "C" int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, cons
     if (!c) return MRT_ERR_CUDA;
     if (c->device != w->device) return set_error(MRT_ERR_INVALID_ARG, "weight lives on another device");
     GemvQ4Args a{};
-    a.codes = w->codes;
-    a.scales = w->scales;
-    a.zeros = w->zeros;
+    a.data = w->data;
+    a.piece = w->piece;
+    a.zeros = w->zeros ? 1 : 0;
+    a.err_flag = c->d_err;
     a.n = static_cast<int>(w->n);
     a.k = static_cast<int>(w->k);
     a.blocks = static_cast<int>(w->blocks);
-    a.group = static_cast<int>(w->group);
+    a.tiles = static_cast<int>(w->tiles);
     a.ldx = ldx;
     a.x_vec = (reinterpret_cast<uintptr_t>(x_dev) & 15) == 0 && (ldx & 7) == 0;
     a.ldy = ldy;
     a.out_f32 = y_dtype == MRT_FP32;
     a.bias = use_bias ? w->bias : nullptr;
     a.ldr = ldr;
-    for (int64_t m = 0; m < M; m += kMaxTokens) {
-        a.M = static_cast<int>(std::min<int64_t>(kMaxTokens, M - m));
+    const int per = static_cast<int>(128 / w->group);
+    GemvPlan plan;
+    for (int64_t m = 0; m < M; m += a.M) {
+        a.M = tokens_at_once(M - m, a.tiles, a.blocks, per, a.piece, c->sms, &plan);
+        if (a.M == 0) return set_error(MRT_ERR_SHAPE, "K is too large for a token in shared memory");
         a.x = static_cast<const uint16_t*>(x_dev) + m * ldx;
         a.y = static_cast<uint8_t*>(y_dev) + m * ldy * (a.out_f32 ? 4 : 2);
         a.res = res_dev != nullptr ? static_cast<const uint16_t*>(res_dev) + m * ldr : nullptr;
-        const cudaError_t e = launch_gemv_q4(a, static_cast<cudaStream_t>(stream));
+        const cudaError_t e = launch_gemv_q4(a, plan, per, c->sms, static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) return cuda_error(e, "4-bit gemv launch");
     }
     return MRT_OK;

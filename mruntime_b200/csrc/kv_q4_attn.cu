@@ -238,11 +238,10 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
             for (int j = 0; j < PER; ++j) {
                 const int ch = lane * PER + j, word = (ch % (D / 4)) >> 3, jj = ch & 7;
                 const float y = x[j] * down;
-                const __half h = __float2half_rn((jj & 2) ? y * 0.0625f : y);
-                sum += __half2float(h) * ((jj & 2) ? 16.0f : 1.0f);
+                const __half h = __float2half_rn((jj & 4) ? y * 0.0625f : y);
+                sum += __half2float(h) * ((jj & 4) ? 16.0f : 1.0f);
                 const int slot = ((row >> 3) * kWords + word) * 32 + (row & 7) * 4 + ch / (D / 4);
-                // registers x, y: columns (0,1), (4,5); z, w: (2,3), (6,7)
-                reinterpret_cast<__half*>(qf + slot)[((jj & 2) ? 4 : 0) + ((jj & 4) ? 2 : 0) + (jj & 1)] = h;
+                reinterpret_cast<__half*>(qf + slot)[jj] = h;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -1343,13 +1342,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                         uint32_t e0, e1, e2, e3;
                         if constexpr (BF16) {
                             e0 = bf2_sub((x & kNib0) | 0x43004300u, z128);
-                            e1 = bf2_sub(((x >> 4) & kNib0) | 0x43004300u, z128);
-                            e2 = bf2_sub(((x >> 8) & kNib0) | 0x43004300u, z128);
+                            e1 = bf2_sub(((x >> 8) & kNib0) | 0x43004300u, z128);
+                            e2 = bf2_sub(((x >> 4) & kNib0) | 0x43004300u, z128);
                             e3 = bf2_sub(((x >> 12) & kNib0) | 0x43004300u, z128);
                         } else {
                             e0 = nib0_f16(x, z1024);
-                            e1 = nib1_f16(x, z64);
-                            e2 = nib0_f16(x >> 8, z1024);
+                            e1 = nib0_f16(x >> 8, z1024);
+                            e2 = nib1_f16(x, z64);
                             e3 = nib1_f16(x >> 8, z64);
                         }
                         st_shared_16(panel_at(kst + (k >> 3) * S::kKPanel, token, k & 7), e0, e1, e2, e3);

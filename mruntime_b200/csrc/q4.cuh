@@ -19,19 +19,31 @@ constexpr uint32_t kNib0 = 0x000F000Fu;  // codes at bits 0-3 of each half: valu
 constexpr uint32_t kNib1 = 0x00F000F0u;  // codes at bits 4-7 of each half: value c * 2^-20
 
 // Nibble position, within the 32-bit word of eight consecutive columns, of
-// column j: (0,1) -> nibbles 0 and 4, (2,3) -> 1 and 5, (4,5) -> 2 and 6,
-// (6,7) -> 3 and 7, so that one mask yields two neighbouring columns as the
-// halves of one operand register.
-__host__ __device__ __forceinline__ int pair_nibble(int j) { return (j >> 1) + ((j & 1) << 2); }
+// column j: (0,1) -> nibbles 0 and 4, (2,3) -> 2 and 6, (4,5) -> 1 and 5,
+// (6,7) -> 3 and 7.  One mask yields two neighbouring columns as the halves of
+// an operand register, the word and the word shifted by eight with the first
+// mask columns 0-3, with the second 4-7: the other operand's registers are
+// neighbours of one 16-byte load.
+__host__ __device__ __forceinline__ int pair_nibble(int j) {
+    return ((j & 1) << 2) | (j & 2) | (j >> 2);
+}
 
 // D += A(16 x 16, row) * B(16 x 8, col), FP16 operands, FP32 sums.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// D = A * B.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // The 8 x 8 matrix of 16-bit values that a warp holds one row pair a lane, transposed.

@@ -3,8 +3,10 @@
 Tolerance of an output: half a step of its type (2^-11 relative for FP16, and
 2^-25 absolute below the normals), plus the FP32 sums: with A = sum_k s (c + z)
 |x| the magnitude that passes through them, each of the chained additions
-(at most 20 within a group and at the end, and one for every column block) off
-by at most 2^-23 of it.  Bias and residual add a rounding each.
+off by at most 2^-23 of it: at most 20 at the end of a group and of the sum, one
+for every column block, and 4 matrix instructions of a group, each of which
+aligns 16 products and its sum so far to the largest and cuts them off there, 17
+times 2^-23.  Bias and residual add a rounding each.
 """
 import numpy as np
 import pytest
@@ -32,7 +34,7 @@ def make(N, K, group, zeros, seed):
 
 def bound(x, w, mag, out_eps, K):
     y = x.double() @ w.t()
-    fp32 = (20 + K // 128 + 1) * 2.0 ** -23 * (x.double().abs() @ mag.t())
+    fp32 = (20 + 4 * 17 + K // 128 + 1) * 2.0 ** -23 * (x.double().abs() @ mag.t())
     return y, fp32 + out_eps * (y.abs() + fp32) + 2.0 ** -25
 
 

@@ -225,10 +225,12 @@ def reference(c, q, kx, vx, vs, causal, scale):
     row's largest such product (codes up to 15).  Many rows: each probability
     is, by 2^-11 or 2^-25 of the row's largest, and each value, by 2^-11 or
     2^-25.  A
-    score is off by FP32 sums of the products' magnitude (2^-23 for each of at
-    most 16 chained additions) and its own size, and moves its probability by
-    as much; the sums over keys are off by 2^-23 for each of the chained
-    additions (a rounding per 16 keys, and the joins); the output by half a step.
+    score is off by FP32 sums of the products' magnitude (2^-23 for each of the
+    chained additions: 17 in a matrix instruction, which aligns 16 products and
+    its sum so far to the largest and cuts them off there, D / 16 of them) and its
+    own size, and moves its probability by as much; the sums over keys are off by
+    2^-23 for each of theirs (17 per 16 keys, and the joins); the output by half a
+    step.
     Codes and zero points may be summed apart: s (c + z) <= |value| + 30 s, and a
     key's 30 s is at most 4 times its largest channel."""
     H, Hk, D = c.H, c.Hk, c.D
@@ -247,9 +249,9 @@ def reference(c, q, kx, vx, vs, causal, scale):
             mag = torch.einsum("hgd,thd->hgt", qd.abs(), k[:keys].abs() + 4 * k[:keys].abs().amax(-1, keepdim=True)) * abs(scale)
             p = s.softmax(-1)
             o = torch.einsum("hgt,thd->hgd", p, v[:keys])
-            off = (16 * 2.0 ** -23 * mag + 2.0 ** -22 * s.abs() + 2.0 ** -21)
+            off = (17 * D / 16 * 2.0 ** -23 * mag + 2.0 ** -22 * s.abs() + 2.0 ** -21)
             pv = torch.einsum("hgt,thd->hgd", p * (2.0 ** (-10 if many else -11) + 2 * off), v[:keys].abs())
-            pv += (32 + keys / 16) * 2.0 ** -23 * torch.einsum("hgt,thd->hgd", p, v[:keys].abs() + 30 * sv[:keys])
+            pv += (32 + 17 * keys / 16) * 2.0 ** -23 * torch.einsum("hgt,thd->hgd", p, v[:keys].abs() + 30 * sv[:keys])
             mean_off = (p * off).sum(-1, keepdim=True)
             if many:
                 low = p.amax(-1, keepdim=True) * 2.0 ** -25 * v[:keys].abs().sum(0)[:, None] + 2.0 ** -25
