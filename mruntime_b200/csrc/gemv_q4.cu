@@ -306,46 +306,47 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
 
     griddep_wait();
     griddep_launch_dependents();
-    // x, 8 columns a thread and step; then the groups' sums.
+    // x, 8 columns a thread and step, and the groups' sums: four loads under way a
+    // thread, whole warps, so that a group's lanes are there for its sum.
     const int row_chunks = nb * 16, chunks = a.M * row_chunks;
-    for (int i = threadIdx.x; i < chunks; i += threads) {
-        const int m = i / row_chunks, p = i - m * row_chunks;
-        const int k = b0 * 128 + p * 8;
-        const bool in = k < a.k;  // K is a multiple of 32
-        const uint16_t* src = in ? a.x + m * a.ldx + k : a.x;
-        uint8_t* dst = xb + m * stride + p * 16;
-        if (a.x_vec) {
-            copy_async_16(smem_u32(dst), src, in);
-        } else {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (in) {
-                v.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
-                v.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
-                v.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
-                v.w = src[6] | static_cast<uint32_t>(src[7]) << 16;
+    for (int i0 = threadIdx.x; i0 < (chunks + 31) / 32 * 32; i0 += threads * 4) {
+        uint4 v[4];
+        int at[4];  // token and chunk of its row
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = i0 + q * threads, m = i / row_chunks, p = i - m * row_chunks, k = b0 * 128 + p * 8;
+            at[q] = m << 16 | p;
+            v[q] = make_uint4(0, 0, 0, 0);
+            if (m < a.M && k < a.k) {  // K is a multiple of 32
+                const uint16_t* src = a.x + m * a.ldx + k;
+                if (a.x_vec) {
+                    v[q] = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    v[q].x = src[0] | static_cast<uint32_t>(src[1]) << 16;
+                    v[q].y = src[2] | static_cast<uint32_t>(src[3]) << 16;
+                    v[q].z = src[4] | static_cast<uint32_t>(src[5]) << 16;
+                    v[q].w = src[6] | static_cast<uint32_t>(src[7]) << 16;
+                }
             }
-            *reinterpret_cast<uint4*>(dst) = v;
         }
-    }
-    copy_async_commit();
-    copy_async_wait<0>();
-    __syncthreads();
-    for (int i = threadIdx.x; i < (chunks + 31) / 32 * 32; i += threads) {
-        const int m = i / row_chunks, p = i - m * row_chunks;
-        float s = 0.0f;
-        if (m < a.M) {
-            const uint4 v = *reinterpret_cast<const uint4*>(xb + m * stride + p * 16);
-            const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int m = at[q] >> 16, p = at[q] & 0xFFFF;
+            const uint32_t h[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+            float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
                 s += f.x + f.y;
             }
-        }
-        constexpr int kLanes = 16 / PER;  // lanes of a group
+            constexpr int kLanes = 16 / PER;  // lanes of a group
 #pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        if (m < a.M && (p & (kLanes - 1)) == 0) xs[(p / kLanes) * NT * 8 + m] = s * 5.9604644775390625e-8f;
+            for (int o = 1; o < kLanes; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            if (m < a.M) {
+                *reinterpret_cast<uint4*>(xb + m * stride + p * 16) = v[q];
+                if ((p & (kLanes - 1)) == 0) xs[(p / kLanes) * NT * 8 + m] = s * 5.9604644775390625e-8f;
+            }
+        }
     }
     __syncthreads();
 
@@ -357,11 +358,9 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
 #pragma unroll
     for (int t = 0; t < NT; ++t) x_row[t] = xb + min(t * 8 + r, a.M - 1) * stride + c * 16;
     for (int tile0 = blockIdx.x * per_cta; tile0 < a.tiles; tile0 += step, turn ^= 1) {
-        float tot[NT][4];
+        uint64_t tot[NT][2];  // rows r and r + 8: tokens 2c, 2c + 1 of a token tile
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tot[t][j] = 0.0f;
+        for (int t = 0; t < NT; ++t) tot[t][0] = tot[t][1] = 0;
         const int tile = tile0 + wt;
 #pragma unroll 1
         for (int b = tile < a.tiles ? wi * kPair : nb; b < nb; b += a.wk * kPair) {
@@ -415,16 +414,18 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
                     if ((i + 1) % kWords == 0) {  // the group ends here
                         const int g = i / kWords;
                         const float s0 = f16_bits_to_f32(static_cast<uint16_t>(sp[u][g])), s1 = f16_bits_to_f32(static_cast<uint16_t>(sp[u][g] >> 16));
-                        const float z0 = ZEROS ? static_cast<float>((zp[u] >> (8 * g)) & 15u) : 8.0f;
-                        const float z1 = ZEROS ? static_cast<float>((zp[u] >> (8 * g + 4)) & 15u) : 8.0f;
+                        // (2^23 + z in FP32 is 0x4B000000 | z)
+                        const float z0 = ZEROS ? __uint_as_float(0x4B000000u | ((zp[u] >> (8 * g)) & 15u)) - 8388608.0f : 8.0f;
+                        const float z1 = ZEROS ? __uint_as_float(0x4B000000u | ((zp[u] >> (8 * g + 4)) & 15u)) - 8388608.0f : 8.0f;
                         const float* xg = xs + ((b + u) * PER + g) * NT * 8 + c * 2;
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            const float2 sx = *reinterpret_cast<const float2*>(xg + t * 8);
-                            tot[t][0] = fmaf(s0, fmaf(-z0, sx.x, fmaf(od[t][0], 0.0625f, ev[t][0])), tot[t][0]);
-                            tot[t][1] = fmaf(s0, fmaf(-z0, sx.y, fmaf(od[t][1], 0.0625f, ev[t][1])), tot[t][1]);
-                            tot[t][2] = fmaf(s1, fmaf(-z1, sx.x, fmaf(od[t][2], 0.0625f, ev[t][2])), tot[t][2]);
-                            tot[t][3] = fmaf(s1, fmaf(-z1, sx.y, fmaf(od[t][3], 0.0625f, ev[t][3])), tot[t][3]);
+                            const uint64_t sx = *reinterpret_cast<const uint64_t*>(xg + t * 8);
+                            const uint64_t sixteenth = pair2(0.0625f, 0.0625f);
+                            const uint64_t e0 = fma2(pair2(od[t][0], od[t][1]), sixteenth, pair2(ev[t][0], ev[t][1]));
+                            const uint64_t e1 = fma2(pair2(od[t][2], od[t][3]), sixteenth, pair2(ev[t][2], ev[t][3]));
+                            tot[t][0] = fma2(pair2(s0, s0), fma2(pair2(-z0, -z0), sx, e0), tot[t][0]);
+                            tot[t][1] = fma2(pair2(s1, s1), fma2(pair2(-z1, -z1), sx, e1), tot[t][1]);
                         }
                     }
                 }
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
                 for (int j = 0; j < 4; ++j) {
                     const int m = t * 8 + c * 2 + (j & 1);
                     const int64_t row = n + (j >> 1) * 8;
-                    if (tile < a.tiles && m < a.M && row < a.n) store_y(a, row, m, tot[t][j]);
+                    if (tile < a.tiles && m < a.M && row < a.n) store_y(a, row, m, (j & 1) ? high2(tot[t][j >> 1]) : low2(tot[t][j >> 1]));
                 }
             continue;
         }
@@ -446,8 +447,8 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
         float* p = part + warp * 16 * NT * 8;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            *reinterpret_cast<float2*>(p + r * NT * 8 + t * 8 + c * 2) = make_float2(tot[t][0], tot[t][1]);
-            *reinterpret_cast<float2*>(p + (r + 8) * NT * 8 + t * 8 + c * 2) = make_float2(tot[t][2], tot[t][3]);
+            *reinterpret_cast<uint64_t*>(p + r * NT * 8 + t * 8 + c * 2) = tot[t][0];
+            *reinterpret_cast<uint64_t*>(p + (r + 8) * NT * 8 + t * 8 + c * 2) = tot[t][1];
         }
         const int rows = per_cta * 16;
         if (gridDim.y == 1) {
@@ -471,8 +472,14 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
                 if (m >= a.M || n >= a.n) continue;
                 const uint32_t at = smem_u32(part + ((row >> 4) * a.wk * 16 + (row & 15)) * NT * 8 + m);
                 float s = 0.0f;
-                for (int k = 0; k < ranks; ++k)
-                    for (int w = 0; w < a.wk; ++w) s += ld_cluster_f32(cluster_address(at, k) + w * 16 * NT * 8 * 4);
+                for (int w = 0; w < a.wk; ++w) {
+                    float v[8];  // all asked for, then added
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        v[k] = k < ranks ? ld_cluster_f32(cluster_address(at, k) + w * 16 * NT * 8 * 4) : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) s += v[k];
+                }
                 store_y(a, n, m, s);
             }
             cluster_barrier();  // the others have read this CTA's sums
@@ -486,7 +493,7 @@ struct GemvPlan {
 };
 
 // Candidates by time, in microseconds.  A multiprocessor works off a piece in
-// 0.036 us when its warps are many, a warp alone in 0.35 us; x comes into every
+// 0.025 us when its warps are many, a warp alone in 0.3 us; x comes into every
 // CTA from L2; larger CTAs start later, and joining sums costs.
 GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
     GemvPlan best{0, 0, 0, 0};
@@ -503,10 +510,13 @@ GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
                 if (ks > 1 && ctas > room) continue;  // slices' CTAs take one turn
                 const int64_t turns = (ctas + room - 1) / room, live = std::min(ctas, room);
                 const int warp_pieces = (slice + wk * kPair - 1) / (wk * kPair) * kPair;
-                const double sm_pieces = static_cast<double>((live + sms - 1) / sms) * turns * per_cta * slice;
-                const double work = std::max(sm_pieces * (nt == 1 ? 0.036 : 0.046), turns * warp_pieces * 0.35);
-                const double x = (live * 256.0 / 8.0e6 + 0.0025 * per_sm) * M * slice / (per_sm == 1 ? 1.0 : 1.0);
-                const double us = work + x + 0.05 * warps + (wk > 1 ? 0.3 * turns : 0.0) + (ks > 1 ? 1.5 : 0.0);
+                // of the busiest multiprocessor, of all of them
+                const double most = static_cast<double>((live + sms - 1) / sms) * turns * per_cta * slice;
+                const double mean = static_cast<double>(tiles) * blocks / sms;
+                const double a_piece = (per == 4 ? 0.030 : 0.025) * (nt == 1 ? 1.0 : 1.3);
+                const double work = std::max((0.3 * most + 0.7 * mean) * a_piece, std::max(1.0, mean / (per_sm * per_cta * slice)) * warp_pieces * 0.3);
+                const double x = live * 256.0 / 8.0e6 * M * slice + M * slice * 16.0 / (warps * 32) * 0.1;
+                const double us = work + x + 0.04 * warps + (wk > 1 ? 0.3 * turns : 0.0) + (ks > 1 ? 1.5 : 0.0);
                 if (best.wk == 0 || us < best_us) {
                     best = GemvPlan{warps, wk, ks, per_sm};
                     best_us = us;
