@@ -14,6 +14,9 @@
 // per position are held as a fraction of 2^64, so p times it, wrapping, is the
 // phase, and only the remainder goes through sincospi (in 64 bits; a token's
 // pairs are shared by all its heads).
+#include <cuda_bf16.h>
+
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -70,7 +73,6 @@ int kv_bind(mrt_kv_q4 kv, KvView* v, int* sms) {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 
 struct Freqs {
     uint64_t turn[64];
@@ -78,7 +80,9 @@ struct Freqs {
 
 struct AppendArgs {
     KvView v;
-    int dtype, heads, rotate, per_cta;
+    int dtype, heads, rotate;
+    int tokens;  // of a CTA
+    int rows;    // of a token that a CTA takes (grid y covers the others)
     const uint16_t* q;
     int64_t ldq;
     uint16_t* q_out;
@@ -87,189 +91,230 @@ struct AppendArgs {
     int64_t ldk;
     const uint16_t* val;
     int64_t ldv;
+    int vec;  // rows can be read and written 16 bytes at a time
 };
 
-__device__ __forceinline__ float widen(uint16_t h, int dtype) {
-    return dtype == MRT_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+constexpr int kMaxTokens = 8;  // of a CTA
+
+__device__ __forceinline__ float widen(uint32_t h, int dtype) {
+    return dtype == MRT_BF16 ? bf16_bits_to_f32(static_cast<uint16_t>(h)) : __half2float(__ushort_as_half(static_cast<uint16_t>(h)));
 }
 
-__device__ __forceinline__ uint16_t narrow(float f, int dtype) {
-    if (dtype == MRT_FP16) return f32_to_f16_bits(f);
-    return f != f ? static_cast<uint16_t>(0x7FC0) : f32_to_bf16_bits(f);
+// Two neighbouring values, rounded to nearest.
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, int dtype) {
+    if (dtype == MRT_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The sequence of row t (block-wide; -1: none, or a sequence outside its bounds).
-__device__ __forceinline__ int find_seq(const KvView& v, int t, int* s_seq) {
-    if (threadIdx.x == 0) *s_seq = -1;
+// Eight neighbouring 16-bit values at any alignment of two bytes.
+__device__ __forceinline__ uint4 load8(const uint16_t* p, bool vec) {
+    if (vec) return *reinterpret_cast<const uint4*>(p);
+    uint4 v;
+    v.x = p[0] | static_cast<uint32_t>(p[1]) << 16;
+    v.y = p[2] | static_cast<uint32_t>(p[3]) << 16;
+    v.z = p[4] | static_cast<uint32_t>(p[5]) << 16;
+    v.w = p[6] | static_cast<uint32_t>(p[7]) << 16;
+    return v;
+}
+
+__device__ __forceinline__ void store8(uint16_t* p, uint4 v, bool vec) {
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) = v;
+        return;
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        p[2 * j] = static_cast<uint16_t>(w[j]);
+        p[2 * j + 1] = static_cast<uint16_t>(w[j] >> 16);
+    }
+}
+
+// Sequence and position of `count` rows from t0 on (block-wide): seq[i] < 0 for
+// a row that is nobody's or breaks the call's bounds (which is reported).
+__device__ __forceinline__ void find_rows(const KvView& v, int t0, int count, int* seq, int* pos) {
+    if (threadIdx.x < count) seq[threadIdx.x] = -1;
     __syncthreads();
-    for (int b = threadIdx.x; b < v.seqs; b += blockDim.x)
-        if (v.q_start[b] <= t && t < v.q_start[b + 1]) *s_seq = b;
+    for (int b = threadIdx.x; b < v.seqs; b += blockDim.x) {
+        const int f = v.q_start[b], e = v.q_start[b + 1];
+        if (e <= t0 || f >= t0 + count || e <= f) continue;
+        int first, n, kv;
+        if (!kv_seq(v, b, &first, &n, &kv)) {
+            raise_error(v.err_flag, kErrBadPage);
+            continue;
+        }
+        for (int i = max(f - t0, 0); i < min(e - t0, count); ++i) {
+            const int p = kv - n + (t0 + i - f);
+            if (p < 0) continue;
+            seq[i] = b;
+            pos[i] = p;
+        }
+    }
     __syncthreads();
-    return *s_seq;
 }
 
-// Lane l's D / 32 neighbouring channels of a row.
-template <int PER>
-__device__ __forceinline__ void load_row(const uint16_t* p, int lane, int dtype, float (&x)[PER]) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = widen(p[lane * PER + j], dtype);
-}
-
-// Row quantised into its block's words and scale.
-template <int PER>
-__device__ __forceinline__ void store_row(uint8_t* block, int token, int lane, bool value, const float (&x)[PER]) {
-    constexpr int D = PER * 32;
-    float lo = 0.0f, hi = 0.0f;
-    bool odd = false;  // NaN, infinity, or beyond FP16
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        lo = fminf(lo, x[j]);
-        hi = fmaxf(hi, x[j]);
-        odd |= !(fabsf(x[j]) <= 65504.0f);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
-    }
-    odd = __any_sync(0xFFFFFFFFu, odd);
-    uint16_t sb = f32_to_f16_bits(fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 5.9604644775390625e-8f));
-    const float inv = __fdiv_rn(1.0f, f16_bits_to_f32(sb));
-    const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
-    uint32_t zero = static_cast<uint32_t>(z);
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint32_t c = static_cast<uint32_t>(fminf(fmaxf(__fadd_rn(rintf(__fmul_rn(x[j], inv)), z), 0.0f), 15.0f));
-        const int in_word = (lane * PER + j) & 7;
-        word |= c << (4 * (value ? in_word : pair_nibble(in_word)));
-    }
-#pragma unroll
-    for (int o = 1; o < 8 / PER; o <<= 1) word |= __shfl_xor_sync(0xFFFFFFFFu, word, o);
-    if (odd) {  // no scale says what the row holds: it reads back as NaN
-        word = 0;
-        sb = 0x7FFFu;
-        zero = 0;
-    }
-    const int w = lane * PER / 8;
-    if (lane % (8 / PER) == 0)
-        *reinterpret_cast<uint32_t*>(block + (value ? kv_v_word(D, token, w) : kv_k_word(D, token, w))) = word;
-    if (lane == 0)
-        reinterpret_cast<uint32_t*>(block + (value ? kv_v_scales(D) : kv_k_scales(D)))[token] = sb | zero << 16;
-}
-
-// One CTA per token (and stretch of heads), one warp per head at a time.
-template <int PER>
+// A row of D channels is D / 8 lanes with eight each, so a warp has two or four
+// rows; every lane packs whole words.  CTAs take tokens (prompts: eight, so that
+// the angles' sines, in 64 bits, and the search for the sequence are shared by
+// many rows) and all their rows, or, when tokens are few, a stretch of them.
+template <int D>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a, const Freqs f) {
-    constexpr int D = PER * 32, HALF = D / 2;
-    __shared__ float cs[HALF], sn[HALF];
-    __shared__ int s_seq;
+    constexpr int LANES = D / 8, HALF = D / 2;
+    __shared__ float cs[kMaxTokens * HALF], sn[kMaxTokens * HALF];
+    __shared__ int s_seq[kMaxTokens], s_pos[kMaxTokens];
     griddep_wait();
     griddep_launch_dependents();
     const KvView& v = a.v;
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = find_seq(v, t, &s_seq);
-    if (b < 0) return;
-    int first, n, kv;
-    if (!kv_seq(v, b, &first, &n, &kv)) {
-        if (threadIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
-        return;
+    const int t0 = blockIdx.x * a.tokens, count = min(a.tokens, v.tokens - t0);
+    find_rows(v, t0, count, s_seq, s_pos);
+    if (a.rotate) {
+        for (int i = threadIdx.x; i < count * HALF; i += kThreads) {
+            const int t = i / HALF, j = i - t * HALF;
+            if (s_seq[t] < 0) continue;
+            const double half_turns = static_cast<double>(static_cast<int64_t>(static_cast<uint64_t>(s_pos[t]) * f.turn[j])) * 0x1p-63;
+            double sv, cv;
+            sincospi(half_turns, &sv, &cv);
+            cs[i] = static_cast<float>(cv);
+            sn[i] = static_cast<float>(sv);
+        }
+        __syncthreads();
     }
-    const int pos = kv - n + (t - first);
-    if (pos < 0) return;
-    if (a.rotate && threadIdx.x < HALF) {
-        const double half_turns =
-            static_cast<double>(static_cast<int64_t>(static_cast<uint64_t>(pos) * f.turn[threadIdx.x])) * 0x1p-63;
-        double sv, cv;
-        sincospi(half_turns, &sv, &cv);
-        cs[threadIdx.x] = static_cast<float>(cv);
-        sn[threadIdx.x] = static_cast<float>(sv);
-    }
-    __syncthreads();
-    const int tasks = a.heads + 2 * v.kv_heads;
-    const int last = min(tasks, static_cast<int>(blockIdx.y + 1) * a.per_cta);
-    for (int task = blockIdx.y * a.per_cta + warp; task < last; task += kWarps) {
-        const bool is_q = task < a.heads, is_v = task >= a.heads + v.kv_heads;
-        const int h = is_q ? task : (is_v ? task - a.heads - v.kv_heads : task - a.heads);
-        const uint16_t* src = is_q ? a.q + t * a.ldq : (is_v ? a.val + t * a.ldv : a.k + t * a.ldk);
-        float x[PER];
-        load_row<PER>(src + h * D, lane, a.dtype, x);
-        if (!is_v && a.rotate) {
+    const int lane = threadIdx.x & (LANES - 1);
+    const int rows = a.heads + 2 * v.kv_heads, row0 = blockIdx.y * a.rows, here = min(a.rows, rows - row0);
+    const int items = count * here, per_pass = kThreads / LANES;
+    // Whole warps go round, so that a row's lanes are there for its shuffles.
+    for (int i0 = 0; i0 < items; i0 += per_pass) {
+        const int i = i0 + threadIdx.x / LANES, t = i / here, row = row0 + i - t * here;
+        const bool live = i < items && s_seq[t] >= 0;
+        const bool is_q = row < a.heads, is_v = row >= a.heads + v.kv_heads;
+        const int h = is_q ? row : (is_v ? row - a.heads - v.kv_heads : row - a.heads);
+        const int64_t tok = t0 + t;
+        float x[8];
+        if (live) {
+            const uint16_t* src = is_q ? a.q + tok * a.ldq : (is_v ? a.val + tok * a.ldv : a.k + tok * a.ldk);
+            const uint4 w = load8(src + h * D + lane * 8, a.vec);
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], 16);
-                const int i = (lane & 15) * PER + j;
-                const float c = cs[i], s = sn[i];
-                x[j] = lane < 16 ? __fsub_rn(__fmul_rn(x[j], c), __fmul_rn(other, s))
-                                 : __fadd_rn(__fmul_rn(other, s), __fmul_rn(x[j], c));
+            for (int j = 0; j < 8; ++j) x[j] = widen(ww[j >> 1] >> (16 * (j & 1)), a.dtype);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+        }
+        if (a.rotate) {
+            const bool turn = live && !is_v, second = lane >= LANES / 2;
+            const int at = t * HALF + (lane & (LANES / 2 - 1)) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], LANES / 2);
+                if (turn) {
+                    const float c = cs[at + j], s = sn[at + j];
+                    x[j] = second ? __fadd_rn(__fmul_rn(other, s), __fmul_rn(x[j], c))
+                                  : __fsub_rn(__fmul_rn(x[j], c), __fmul_rn(other, s));
+                }
             }
         }
-        if (is_q) {
+        float lo = 0.0f, hi = 0.0f;
+        bool odd = false;  // NaN, infinity, or beyond FP16
 #pragma unroll
-            for (int j = 0; j < PER; ++j) a.q_out[t * a.ldqo + h * D + lane * PER + j] = narrow(x[j], a.dtype);
+        for (int j = 0; j < 8; ++j) {
+            lo = fminf(lo, x[j]);
+            hi = fmaxf(hi, x[j]);
+            odd |= !(fabsf(x[j]) <= 65504.0f);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+        }
+        const uint32_t group = __ballot_sync(0xFFFFFFFFu, odd) >> (threadIdx.x & 31 & ~(LANES - 1));
+        odd = (group & ((1u << LANES) - 1)) != 0;
+        if (!live) continue;
+        if (is_q) {
+            store8(a.q_out + tok * a.ldqo + h * D + lane * 8,
+                   make_uint4(narrow2(x[0], x[1], a.dtype), narrow2(x[2], x[3], a.dtype), narrow2(x[4], x[5], a.dtype),
+                              narrow2(x[6], x[7], a.dtype)), a.vec);
             continue;
         }
-        uint8_t* block = kv_block_at(v, v.table + static_cast<int64_t>(b) * v.ld_table, h, pos);
+        const int pos = s_pos[t], token = pos & (kKvBlock - 1);
+        uint8_t* block = kv_block_at(v, v.table + static_cast<int64_t>(s_seq[t]) * v.ld_table, h, pos);
         if (block == nullptr) {
             if (lane == 0) raise_error(v.err_flag, kErrBadPage);
             continue;
         }
-        store_row<PER>(block, pos & (kKvBlock - 1), lane, is_v, x);
+        uint16_t sb = __half_as_ushort(__float2half_rn(fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 5.9604644775390625e-8f)));
+        const float inv = __fdiv_rn(1.0f, __half2float(__ushort_as_half(sb)));
+        const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
+        uint32_t zero = static_cast<uint32_t>(z), word = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t c = static_cast<uint32_t>(fminf(fmaxf(__fadd_rn(rintf(__fmul_rn(x[j], inv)), z), 0.0f), 15.0f));
+            word |= c << (4 * (is_v ? j : pair_nibble(j)));
+        }
+        if (odd) {  // no scale says what the row holds: it reads back as NaN
+            word = 0;
+            sb = 0x7FFFu;
+            zero = 0;
+        }
+        *reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_word(D, token, lane) : kv_k_word(D, token, lane))) = word;
+        if (lane == 0)
+            reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_scales(D) : kv_k_scales(D)))[token] = sb | zero << 16;
     }
 }
 
 struct ReadArgs {
     KvView v;
-    int dtype;
+    int dtype, tokens;
     uint16_t* k;
     int64_t ldk;
     uint16_t* val;
     int64_t ldv;
+    int vec;
 };
 
-template <int PER>
+template <int D>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
-    constexpr int D = PER * 32;
-    __shared__ int s_seq;
+    constexpr int LANES = D / 8;
+    __shared__ int s_seq[kMaxTokens], s_pos[kMaxTokens];
     griddep_wait();
     griddep_launch_dependents();
     const KvView& v = a.v;
-    const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = find_seq(v, t, &s_seq);
-    if (b < 0) return;
-    int first, n, kv;
-    if (!kv_seq(v, b, &first, &n, &kv)) {
-        if (threadIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
-        return;
-    }
-    const int pos = kv - n + (t - first);
-    if (pos < 0) return;
-    for (int task = warp; task < 2 * v.kv_heads; task += kWarps) {
-        const bool value = task >= v.kv_heads;
-        const int h = value ? task - v.kv_heads : task;
+    const int t0 = blockIdx.x * a.tokens, count = min(a.tokens, v.tokens - t0);
+    find_rows(v, t0, count, s_seq, s_pos);
+    const int lane = threadIdx.x & (LANES - 1), rows = 2 * v.kv_heads;
+    for (int i = threadIdx.x / LANES; i < count * rows; i += kThreads / LANES) {
+        const int t = i / rows, row = i - t * rows;
+        const bool value = row >= v.kv_heads;
+        const int h = value ? row - v.kv_heads : row;
         uint16_t* dst = value ? a.val : a.k;
-        if (dst == nullptr) continue;
-        dst += t * (value ? a.ldv : a.ldk) + h * D;
-        const uint8_t* block = kv_block_at(v, v.table + static_cast<int64_t>(b) * v.ld_table, h, pos);
+        if (dst == nullptr || s_seq[t] < 0) continue;
+        const int pos = s_pos[t], token = pos & (kKvBlock - 1);
+        const uint8_t* block = kv_block_at(v, v.table + static_cast<int64_t>(s_seq[t]) * v.ld_table, h, pos);
         if (block == nullptr) {
             if (lane == 0) raise_error(v.err_flag, kErrBadPage);
             continue;
         }
-        const int token = pos & (kKvBlock - 1);
         const uint32_t sz = reinterpret_cast<const uint32_t*>(block + (value ? kv_v_scales(D) : kv_k_scales(D)))[token];
-        const float s = f16_bits_to_f32(static_cast<uint16_t>(sz));
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(block + (value ? kv_v_word(D, token, lane) : kv_k_word(D, token, lane)));
+        const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(sz)));
         const int z = static_cast<int>(sz >> 16);
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int ch = lane * PER + j;
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(
-                block + (value ? kv_v_word(D, token, ch >> 3) : kv_k_word(D, token, ch >> 3)));
-            const int nib = value ? ch & 7 : pair_nibble(ch & 7);
-            const int c = (w >> (4 * nib)) & 15;
-            dst[ch] = narrow(__fmul_rn(s, static_cast<float>(c - z)), a.dtype);
-        }
+        for (int j = 0; j < 8; ++j)
+            x[j] = __fmul_rn(s, static_cast<float>(static_cast<int>((w >> (4 * (value ? j : pair_nibble(j)))) & 15u) - z));
+        store8(dst + (t0 + t) * (value ? a.ldv : a.ldk) + h * D + lane * 8,
+               make_uint4(narrow2(x[0], x[1], a.dtype), narrow2(x[2], x[3], a.dtype), narrow2(x[4], x[5], a.dtype),
+                          narrow2(x[6], x[7], a.dtype)), a.vec);
     }
 }
+
+// Tokens of a CTA: as many as leave every multiprocessor two CTAs.
+int tokens_of(int tokens, int sms) { return std::max(1, std::min(kMaxTokens, tokens / (2 * sms))); }
+
+bool aligned16(const void* p, int64_t ld) { return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0); }
 
 template <typename... P, typename... A>
 cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
@@ -375,14 +420,16 @@ extern "C" int mrt_kv_q4_append(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dty
     a.ldk = ldk;
     a.val = static_cast<const uint16_t*>(v_dev);
     a.ldv = ldv;
-    const int tasks = a.heads + 2 * a.v.kv_heads;
-    a.per_cta = tasks;
+    a.vec = aligned16(a.q, ldq) && aligned16(a.q_out, ldqo) && aligned16(a.k, ldk) && aligned16(a.val, ldv);
+    a.tokens = tokens_of(a.v.tokens, sms);
+    const int rows = a.heads + 2 * a.v.kv_heads, pass = kThreads / static_cast<int>(D / 8);
+    a.rows = a.tokens > 1 ? rows : pass;  // few tokens: one pass a CTA
     Freqs f;
     for (int i = 0; i < 64; ++i) f.turn[i] = kv->freq[i];
-    const dim3 grid(static_cast<unsigned>(a.v.tokens), static_cast<unsigned>((tasks + a.per_cta - 1) / a.per_cta));
+    const dim3 grid(static_cast<unsigned>((a.v.tokens + a.tokens - 1) / a.tokens), static_cast<unsigned>((rows + a.rows - 1) / a.rows));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = D == 128 ? launch_pdl(kv_append_kernel<4>, grid, kThreads, s, a, f)
-                                   : launch_pdl(kv_append_kernel<2>, grid, kThreads, s, a, f);
+    const cudaError_t e = D == 128 ? launch_pdl(kv_append_kernel<128>, grid, kThreads, s, a, f)
+                                   : launch_pdl(kv_append_kernel<64>, grid, kThreads, s, a, f);
     return e == cudaSuccess ? MRT_OK : cuda_error(e, "4-bit cache append launch");
 }
 
@@ -396,15 +443,18 @@ extern "C" int mrt_kv_q4_read(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype
     const int64_t D = kv->head_dim;
     if ((k_dev != nullptr && ldk < kv->kv_heads * D) || (v_dev != nullptr && ldv < kv->kv_heads * D))
         return set_error(MRT_ERR_SHAPE, "a token's stride must cover its heads");
-    if ((rc = kv_bind(kv, &a.v, nullptr)) != MRT_OK) return rc;
+    int sms = 0;
+    if ((rc = kv_bind(kv, &a.v, &sms)) != MRT_OK) return rc;
     a.dtype = dtype;
     a.k = static_cast<uint16_t*>(k_dev);
     a.ldk = ldk;
     a.val = static_cast<uint16_t*>(v_dev);
     a.ldv = ldv;
-    const dim3 grid(static_cast<unsigned>(a.v.tokens));
+    a.vec = aligned16(k_dev, ldk) && aligned16(v_dev, ldv);
+    a.tokens = tokens_of(a.v.tokens, sms);
+    const dim3 grid(static_cast<unsigned>((a.v.tokens + a.tokens - 1) / a.tokens));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = D == 128 ? launch_pdl(kv_read_kernel<4>, grid, kThreads, s, a)
-                                   : launch_pdl(kv_read_kernel<2>, grid, kThreads, s, a);
+    const cudaError_t e = D == 128 ? launch_pdl(kv_read_kernel<128>, grid, kThreads, s, a)
+                                   : launch_pdl(kv_read_kernel<64>, grid, kThreads, s, a);
     return e == cudaSuccess ? MRT_OK : cuda_error(e, "4-bit cache read launch");
 }
