@@ -92,6 +92,7 @@ struct AppendArgs {
     const uint16_t* val;
     int64_t ldv;
     int vec;  // rows can be read and written 16 bytes at a time
+    uint64_t row_magic;  // 2^40 / rows, rounded up: i * it >> 40 = i / rows for i rows < 2^40
 };
 
 constexpr int kMaxTokens = 8;  // of a CTA
@@ -157,14 +158,42 @@ __device__ __forceinline__ void find_rows(const KvView& v, int t0, int count, in
     __syncthreads();
 }
 
-// A row of D channels is D / 8 lanes with eight each, so a warp has two or four
-// rows; every lane packs whole words.  CTAs take tokens (prompts: eight, so that
-// the angles' sines, in 64 bits, and the search for the sequence are shared by
-// many rows) and all their rows, or, when tokens are few, a stretch of them.
+__device__ __forceinline__ void widen8(uint4 w, int dtype, float (&x)[8]) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = widen(v[j >> 1] >> (16 * (j & 1)) & 0xFFFFu, dtype);
+}
+
+__device__ __forceinline__ uint4 narrow8(const float (&x)[8], int dtype) {
+    return make_uint4(narrow2(x[0], x[1], dtype), narrow2(x[2], x[3], dtype), narrow2(x[4], x[5], dtype),
+                      narrow2(x[6], x[7], dtype));
+}
+
+// The codes of eight values: rint(x inv) + z, kept in 0..15 (adding 1.5 * 2^23
+// rounds to the nearest whole number, ties to even, and leaves it in the low
+// bits).  The product has its own rounding: scalar operations, because a product
+// and a sum of register pairs become one fused operation.
+__device__ __forceinline__ uint32_t codes8(const float (&x)[8], float inv, int z, bool value) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int c = __float_as_int(__fadd_rn(__fmul_rn(x[j], inv), 12582912.0f)) - 0x4B400000 + z;
+        word |= static_cast<uint32_t>(min(max(c, 0), 15)) << (4 * (value ? j : pair_nibble(j)));
+    }
+    return word;
+}
+
+// A row of D channels is D / 16 lanes, each with eight channels and the eight
+// that the rotation pairs them with, so a warp has four or eight rows, no value
+// changes lanes and every lane packs whole words.  CTAs take tokens (prompts:
+// eight, so that the angles' sines, in 64 bits, and the search for the sequence
+// are shared by many rows) and all their rows, or, when tokens are few, a stretch
+// of them.  Bound by instructions (a prompt's bytes would take a third of its
+// time).
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a, const Freqs f) {
-    constexpr int LANES = D / 8, HALF = D / 2;
-    __shared__ float cs[kMaxTokens * HALF], sn[kMaxTokens * HALF];
+    constexpr int LANES = D / 16, HALF = D / 2;
+    __shared__ __align__(16) float cs[kMaxTokens * HALF], sn[kMaxTokens * HALF];
     __shared__ int s_seq[kMaxTokens], s_pos[kMaxTokens];
     griddep_wait();
     griddep_launch_dependents();
@@ -185,46 +214,57 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a,
     }
     const int lane = threadIdx.x & (LANES - 1);
     const int rows = a.heads + 2 * v.kv_heads, row0 = blockIdx.y * a.rows, here = min(a.rows, rows - row0);
-    const int items = count * here, per_pass = kThreads / LANES;
+    const int items = count * here;
     // Whole warps go round, so that a row's lanes are there for its shuffles.
-    for (int i0 = 0; i0 < items; i0 += per_pass) {
-        const int i = i0 + threadIdx.x / LANES, t = i / here, row = row0 + i - t * here;
-        const bool live = i < items && s_seq[t] >= 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < items; i0 += kThreads / LANES) {
+        const int i = i0 + threadIdx.x / LANES;
+        const int t = static_cast<int>(static_cast<uint64_t>(i) * a.row_magic >> 40);  // i / here for a whole token's rows
+        const int ti = a.tokens > 1 ? t : 0, row = row0 + i - ti * here;
+        const bool live = i < items && s_seq[ti] >= 0;
         const bool is_q = row < a.heads, is_v = row >= a.heads + v.kv_heads;
         const int h = is_q ? row : (is_v ? row - a.heads - v.kv_heads : row - a.heads);
-        const int64_t tok = t0 + t;
-        float x[8];
+        const int64_t tok = t0 + ti;
+        const int ch = h * D + lane * 8;
+        float x0[8] = {}, x1[8] = {};
         if (live) {
-            const uint16_t* src = is_q ? a.q + tok * a.ldq : (is_v ? a.val + tok * a.ldv : a.k + tok * a.ldk);
-            const uint4 w = load8(src + h * D + lane * 8, a.vec);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            const uint16_t* src = (is_q ? a.q + tok * a.ldq : (is_v ? a.val + tok * a.ldv : a.k + tok * a.ldk)) + ch;
+            const uint4 w0 = load8(src, a.vec), w1 = load8(src + HALF, a.vec);
+            widen8(w0, a.dtype, x0);
+            widen8(w1, a.dtype, x1);
+            if (a.rotate && !is_v) {
+                const float4* c4 = reinterpret_cast<const float4*>(cs + ti * HALF + lane * 8);
+                const float4* s4 = reinterpret_cast<const float4*>(sn + ti * HALF + lane * 8);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = widen(ww[j >> 1] >> (16 * (j & 1)), a.dtype);
-        } else {
+                for (int j = 0; j < 2; ++j) {
+                    const float c[4] = {c4[j].x, c4[j].y, c4[j].z, c4[j].w}, s[4] = {s4[j].x, s4[j].y, s4[j].z, s4[j].w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = 0.0f;
-        }
-        if (a.rotate) {
-            const bool turn = live && !is_v, second = lane >= LANES / 2;
-            const int at = t * HALF + (lane & (LANES / 2 - 1)) * 8;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], LANES / 2);
-                if (turn) {
-                    const float c = cs[at + j], s = sn[at + j];
-                    x[j] = second ? __fadd_rn(__fmul_rn(other, s), __fmul_rn(x[j], c))
-                                  : __fsub_rn(__fmul_rn(x[j], c), __fmul_rn(other, s));
+                    for (int k = 0; k < 4; ++k) {  // products and sums each rounded
+                        float &p = x0[j * 4 + k], &q = x1[j * 4 + k];
+                        const float y = __fsub_rn(__fmul_rn(p, c[k]), __fmul_rn(q, s[k]));
+                        q = __fadd_rn(__fmul_rn(p, s[k]), __fmul_rn(q, c[k]));
+                        p = y;
+                    }
                 }
             }
+            if (is_q) {
+                uint16_t* dst = a.q_out + tok * a.ldqo + ch;
+                store8(dst, narrow8(x0, a.dtype), a.vec);
+                store8(dst + HALF, narrow8(x1, a.dtype), a.vec);
+            }
         }
+        const bool held = live && !is_q;
+        if (!__any_sync(0xFFFFFFFFu, held)) continue;
         float lo = 0.0f, hi = 0.0f;
         bool odd = false;  // NaN, infinity, or beyond FP16
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            lo = fminf(lo, x[j]);
-            hi = fmaxf(hi, x[j]);
-            odd |= !(fabsf(x[j]) <= 65504.0f);
+            lo = fminf(lo, fminf(x0[j], x1[j]));
+            hi = fmaxf(hi, fmaxf(x0[j], x1[j]));
+            const float sum = fabsf(x0[j]) + fabsf(x1[j]);
+            odd |= sum != sum;  // a NaN (a sum of magnitudes is none else)
         }
+        odd |= !(fmaxf(-lo, hi) <= 65504.0f);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
@@ -232,34 +272,24 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a,
         }
         const uint32_t group = __ballot_sync(0xFFFFFFFFu, odd) >> (threadIdx.x & 31 & ~(LANES - 1));
         odd = (group & ((1u << LANES) - 1)) != 0;
-        if (!live) continue;
-        if (is_q) {
-            store8(a.q_out + tok * a.ldqo + h * D + lane * 8,
-                   make_uint4(narrow2(x[0], x[1], a.dtype), narrow2(x[2], x[3], a.dtype), narrow2(x[4], x[5], a.dtype),
-                              narrow2(x[6], x[7], a.dtype)), a.vec);
-            continue;
-        }
-        const int pos = s_pos[t], token = pos & (kKvBlock - 1);
-        uint8_t* block = kv_block_at(v, v.table + static_cast<int64_t>(s_seq[t]) * v.ld_table, h, pos);
+        if (!held) continue;
+        const int pos = s_pos[ti], token = pos & (kKvBlock - 1);
+        uint8_t* block = kv_block_at(v, v.table + static_cast<int64_t>(s_seq[ti]) * v.ld_table, h, pos);
         if (block == nullptr) {
             if (lane == 0) raise_error(v.err_flag, kErrBadPage);
             continue;
         }
         uint16_t sb = __half_as_ushort(__float2half_rn(fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 5.9604644775390625e-8f)));
-        const float inv = __fdiv_rn(1.0f, __half2float(__ushort_as_half(sb)));
-        const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
-        uint32_t zero = static_cast<uint32_t>(z), word = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t c = static_cast<uint32_t>(fminf(fmaxf(__fadd_rn(rintf(__fmul_rn(x[j], inv)), z), 0.0f), 15.0f));
-            word |= c << (4 * (is_v ? j : pair_nibble(j)));
-        }
+        const float inv = __frcp_rn(__half2float(__ushort_as_half(sb)));
+        uint32_t zero = static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f));
+        uint32_t w0 = codes8(x0, inv, static_cast<int>(zero), is_v), w1 = codes8(x1, inv, static_cast<int>(zero), is_v);
         if (odd) {  // no scale says what the row holds: it reads back as NaN
-            word = 0;
+            w0 = w1 = 0;
             sb = 0x7FFFu;
             zero = 0;
         }
-        *reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_word(D, token, lane) : kv_k_word(D, token, lane))) = word;
+        *reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_word(D, token, lane) : kv_k_word(D, token, lane))) = w0;
+        *reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_word(D, token, lane + LANES) : kv_k_word(D, token, lane + LANES))) = w1;
         if (lane == 0)
             reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_scales(D) : kv_k_scales(D)))[token] = sb | zero << 16;
     }
@@ -273,11 +303,12 @@ struct ReadArgs {
     uint16_t* val;
     int64_t ldv;
     int vec;
+    uint64_t row_magic;
 };
 
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
-    constexpr int LANES = D / 8;
+    constexpr int LANES = D / 16, HALF = D / 2;
     __shared__ int s_seq[kMaxTokens], s_pos[kMaxTokens];
     griddep_wait();
     griddep_launch_dependents();
@@ -285,8 +316,9 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
     const int t0 = blockIdx.x * a.tokens, count = min(a.tokens, v.tokens - t0);
     find_rows(v, t0, count, s_seq, s_pos);
     const int lane = threadIdx.x & (LANES - 1), rows = 2 * v.kv_heads;
+#pragma unroll 1
     for (int i = threadIdx.x / LANES; i < count * rows; i += kThreads / LANES) {
-        const int t = i / rows, row = i - t * rows;
+        const int t = static_cast<int>(static_cast<uint64_t>(i) * a.row_magic >> 40), row = i - t * rows;
         const bool value = row >= v.kv_heads;
         const int h = value ? row - v.kv_heads : row;
         uint16_t* dst = value ? a.val : a.k;
@@ -298,18 +330,31 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
             continue;
         }
         const uint32_t sz = reinterpret_cast<const uint32_t*>(block + (value ? kv_v_scales(D) : kv_k_scales(D)))[token];
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(block + (value ? kv_v_word(D, token, lane) : kv_k_word(D, token, lane)));
         const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(sz)));
-        const int z = static_cast<int>(sz >> 16);
-        float x[8];
+        const uint64_t s2 = pair2(s, s);
+        const float less = -8388608.0f - static_cast<float>(sz >> 16);  // -(2^23 + z): exact
+        const uint64_t less2 = pair2(less, less);
+        dst += (t0 + t) * (value ? a.ldv : a.ldk) + h * D + lane * 8;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            x[j] = __fmul_rn(s, static_cast<float>(static_cast<int>((w >> (4 * (value ? j : pair_nibble(j)))) & 15u) - z));
-        store8(dst + (t0 + t) * (value ? a.ldv : a.ldk) + h * D + lane * 8,
-               make_uint4(narrow2(x[0], x[1], a.dtype), narrow2(x[2], x[3], a.dtype), narrow2(x[4], x[5], a.dtype),
-                          narrow2(x[6], x[7], a.dtype)), a.vec);
+        for (int part = 0; part < 2; ++part) {
+            const int wi = lane + part * LANES;
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(block + (value ? kv_v_word(D, token, wi) : kv_k_word(D, token, wi)));
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // 2^23 + c in FP32 is 0x4B000000 | c
+                const uint32_t c0 = (w >> (4 * (value ? 2 * j : pair_nibble(2 * j)))) & 15u;
+                const uint32_t c1 = (w >> (4 * (value ? 2 * j + 1 : pair_nibble(2 * j + 1)))) & 15u;
+                const uint64_t v = mul2(s2, add2(pair2(0x4B000000u | c0, 0x4B000000u | c1), less2));
+                x[2 * j] = low2(v);
+                x[2 * j + 1] = high2(v);
+            }
+            store8(dst + part * HALF, narrow8(x, a.dtype), a.vec);
+        }
     }
 }
+
+uint64_t magic_of(int rows) { return ((1ull << 40) + rows - 1) / rows; }
 
 // Tokens of a CTA: as many as leave every multiprocessor two CTAs.
 int tokens_of(int tokens, int sms) { return std::max(1, std::min(kMaxTokens, tokens / (2 * sms))); }
@@ -422,8 +467,9 @@ extern "C" int mrt_kv_q4_append(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dty
     a.ldv = ldv;
     a.vec = aligned16(a.q, ldq) && aligned16(a.q_out, ldqo) && aligned16(a.k, ldk) && aligned16(a.val, ldv);
     a.tokens = tokens_of(a.v.tokens, sms);
-    const int rows = a.heads + 2 * a.v.kv_heads, pass = kThreads / static_cast<int>(D / 8);
-    a.rows = a.tokens > 1 ? rows : pass;  // few tokens: one pass a CTA
+    const int rows = a.heads + 2 * a.v.kv_heads, pass = kThreads / static_cast<int>(D / 16);
+    a.rows = a.tokens > 1 ? rows : std::min(pass, 16);  // few tokens: less than a pass a CTA
+    a.row_magic = magic_of(rows);
     Freqs f;
     for (int i = 0; i < 64; ++i) f.turn[i] = kv->freq[i];
     const dim3 grid(static_cast<unsigned>((a.v.tokens + a.tokens - 1) / a.tokens), static_cast<unsigned>((rows + a.rows - 1) / a.rows));
@@ -451,6 +497,7 @@ extern "C" int mrt_kv_q4_read(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype
     a.val = static_cast<uint16_t*>(v_dev);
     a.ldv = ldv;
     a.vec = aligned16(k_dev, ldk) && aligned16(v_dev, ldv);
+    a.row_magic = magic_of(2 * a.v.kv_heads);
     a.tokens = tokens_of(a.v.tokens, sms);
     const dim3 grid(static_cast<unsigned>((a.v.tokens + a.tokens - 1) / a.tokens));
     cudaStream_t s = static_cast<cudaStream_t>(stream);

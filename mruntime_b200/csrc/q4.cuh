@@ -84,7 +84,8 @@ __device__ __forceinline__ void copy_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Two FP32 values in one 64-bit register pair.
+// Two FP32 values in one 64-bit register pair.  (A product of pairs that only a
+// sum uses is fused with it: use them where one rounding is as good as two.)
 __device__ __forceinline__ uint64_t pair2(uint32_t lo, uint32_t hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
