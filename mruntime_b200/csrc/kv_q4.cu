@@ -281,17 +281,27 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a,
         }
         uint16_t sb = __half_as_ushort(__float2half_rn(fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 5.9604644775390625e-8f)));
         const float inv = __frcp_rn(__half2float(__ushort_as_half(sb)));
-        uint32_t zero = static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f));
+        float zero = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
         uint32_t w0 = codes8(x0, inv, static_cast<int>(zero), is_v), w1 = codes8(x1, inv, static_cast<int>(zero), is_v);
         if (odd) {  // no scale says what the row holds: it reads back as NaN
             w0 = w1 = 0;
             sb = 0x7FFFu;
-            zero = 0;
+            zero = 0.0f;
         }
-        *reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_word(D, token, lane) : kv_k_word(D, token, lane))) = w0;
-        *reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_word(D, token, lane + LANES) : kv_k_word(D, token, lane + LANES))) = w1;
+        if (is_v) {
+            uint16_t* d0 = reinterpret_cast<uint16_t*>(block + kv_v_half(D, token, lane));
+            uint16_t* d1 = reinterpret_cast<uint16_t*>(block + kv_v_half(D, token, lane + LANES));
+            d0[0] = static_cast<uint16_t>(w0);
+            d0[2] = static_cast<uint16_t>(w0 >> 16);
+            d1[0] = static_cast<uint16_t>(w1);
+            d1[2] = static_cast<uint16_t>(w1 >> 16);
+        } else {
+            *reinterpret_cast<uint32_t*>(block + kv_k_word(D, token, lane)) = w0;
+            *reinterpret_cast<uint32_t*>(block + kv_k_word(D, token, lane + LANES)) = w1;
+        }
         if (lane == 0)
-            reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_scales(D) : kv_k_scales(D)))[token] = sb | zero << 16;
+            reinterpret_cast<uint32_t*>(block + (is_v ? kv_v_scales(D) : kv_k_scales(D)))[token] =
+                sb | static_cast<uint32_t>(__half_as_ushort(__float2half_rn(zero))) << 16;
     }
 }
 
@@ -332,13 +342,19 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
         const uint32_t sz = reinterpret_cast<const uint32_t*>(block + (value ? kv_v_scales(D) : kv_k_scales(D)))[token];
         const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(sz)));
         const uint64_t s2 = pair2(s, s);
-        const float less = -8388608.0f - static_cast<float>(sz >> 16);  // -(2^23 + z): exact
+        const float less = -8388608.0f - __half2float(__ushort_as_half(static_cast<uint16_t>(sz >> 16)));  // -(2^23 + z): exact
         const uint64_t less2 = pair2(less, less);
         dst += (t0 + t) * (value ? a.ldv : a.ldk) + h * D + lane * 8;
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
             const int wi = lane + part * LANES;
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(block + (value ? kv_v_word(D, token, wi) : kv_k_word(D, token, wi)));
+            uint32_t w;
+            if (value) {
+                const uint16_t* p = reinterpret_cast<const uint16_t*>(block + kv_v_half(D, token, wi));
+                w = p[0] | static_cast<uint32_t>(p[2]) << 16;
+            } else {
+                w = *reinterpret_cast<const uint32_t*>(block + kv_k_word(D, token, wi));
+            }
             float x[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {

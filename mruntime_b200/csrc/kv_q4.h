@@ -24,10 +24,9 @@ namespace mrt {
 //   K codes   16 rows of D / 2 bytes, a token each: eight channels a word, in
 //             the nibble order of pair_nibble().
 //   V codes   2 halves (tokens 0-7, 8-15) of 32 lanes (r, c) = (channel
-//             stretch, token pair): tokens 2c and 2c + 1, channels
-//             [r D/8, (r + 1) D/8), D / 16 bytes each; eight channels a word,
-//             in natural nibble order.
-//   K scales  16 words: FP16 scale | zero point << 16.
+//             stretch, token pair): channels [r D/8, (r + 1) D/8) of tokens
+//             2c and 2c + 1, four channels a word, token 2c's in the low half.
+//   K scales  16 words: FP16 scale | FP16 zero point << 16.
 //   V scales  16 words.
 //
 // Both orders are those in which the attention kernel's lanes read their MMA
@@ -42,11 +41,11 @@ __host__ __device__ __forceinline__ int kv_v_scales(int D) { return kKvBlock * D
 
 // Byte offset in a block of the K word `w` (channels 8w..8w+7) of token t.
 __host__ __device__ __forceinline__ int kv_k_word(int D, int t, int w) { return t * (D / 2) + w * 4; }
-// The same for V.
-__host__ __device__ __forceinline__ int kv_v_word(int D, int t, int w) {
-    const int per = D / 64;  // words of a lane's stretch
+// The same for V channels 8w..8w+3; those of the next four channels lie four bytes on.
+__host__ __device__ __forceinline__ int kv_v_half(int D, int t, int w) {
+    const int per = D / 64;  // eights of a stretch
     const int r = w / per, j = w - r * per;
-    return kv_v_codes(D) + (t >> 3) * 4 * D + (r * 4 + ((t & 7) >> 1)) * (D / 8) + (t & 1) * (D / 16) + j * 4;
+    return kv_v_codes(D) + (t >> 3) * 4 * D + (r * 4 + ((t & 7) >> 1)) * (D / 8) + j * 8 + (t & 1) * 2;
 }
 
 // A cache and the sequences of one call, as kernels see them.
@@ -61,13 +60,23 @@ struct KvView {
     int* err_flag;
 };
 
-// Number in the pool of the block that holds position `pos` of a sequence whose
-// table row is given, or -1 when the row names no page of the cache there.
+// Place, in a sequence's table row, of the page that holds position `pos`.
+__device__ __forceinline__ int kv_slot(const KvView& v, int pos) {
+    const int block = pos / kKvBlock;
+    return v.page_shift >= 0 ? block >> v.page_shift : block / (v.page_tokens / kKvBlock);
+}
+
+// Number in the pool of the block of that page that holds it, or -1 when it is
+// no page of the cache.
+__device__ __forceinline__ int kv_block_in(const KvView& v, int page, int slot, int head, int pos) {
+    const int blocks = v.page_tokens / kKvBlock;
+    return page < 0 || page >= v.pages ? -1 : (page * v.kv_heads + head) * blocks + (pos / kKvBlock - slot * blocks);
+}
+
+// Both for a sequence whose table row is given.
 __device__ __forceinline__ int kv_block_number(const KvView& v, const int32_t* row, int head, int pos) {
-    const int blocks = v.page_tokens / kKvBlock, block = pos / kKvBlock;
-    const int slot = v.page_shift >= 0 ? block >> v.page_shift : block / blocks;
-    const int page = slot < v.ld_table ? row[slot] : -1;
-    return page < 0 || page >= v.pages ? -1 : (page * v.kv_heads + head) * blocks + (block - slot * blocks);
+    const int slot = kv_slot(v, pos);
+    return kv_block_in(v, slot < v.ld_table ? row[slot] : -1, slot, head, pos);
 }
 
 // The block itself, or null.

@@ -51,6 +51,9 @@ __device__ __forceinline__ void store2(uint16_t* dst, uint32_t v) {
     }
 }
 
+// Own writes to shared memory come before later asynchronous ones.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // ------------------------------------------------------------------ few rows
 
 // Rows of one (sequence, kv head) are its new tokens times the query heads that
@@ -60,22 +63,24 @@ __device__ __forceinline__ void store2(uint16_t* dst, uint32_t v) {
 // the M operands straight from their bytes (q4.cuh).
 //
 // Softmax.  In powers of two, with a value's scale taken into the exponent:
-// y = scale log2(e) q.k + log2 s_v, p' = 2^(y - m), m the running maximum of y.
-// So p' is the probability times its value's scale, relative to the largest
-// such product: FP16 operands keep eleven bits of whatever matters, however
-// unlike the scales are.  The sum is of p' / s_v, and the zero points' part of
-// the output, sum p' z (of the same rounded p'), is one number a row.
+// y = scale log2(e) q.k + log2 s_v, p' = 2^(y - m), m at most eight below the
+// running maximum of y (so it seldom has to be moved).  So p' is the probability
+// times its value's scale, relative to the largest such product within 2^8: FP16
+// operands keep eleven bits of whatever matters, however unlike the scales are.
+// The sum is of p' / s_v, and the zero points' part of the output, sum p' z (of
+// the same rounded p'), is one more row of the second product.
 //
 // Split.  The 32-token tiles of all (sequence, kv head) units, in order, are
 // dealt to the CTAs in equal contiguous stretches, whatever the lengths: no
 // CTA waits for a long sequence, and no plan from the host is needed (lengths
 // are read here).  A CTA's warps take a stretch's tiles in turn, each with its
-// own ring of asynchronous copies, and join at the end of the unit.  A unit
-// that spans CTAs leaves its parts in scratch (two places a CTA: a unit that
-// began earlier, and one that goes on) and attn_q4_join_kernel adds them in
-// order.
+// own ring of bulk copies, and join at the end of the unit, the next unit's
+// first tiles already under way.  A unit that spans CTAs leaves its parts in
+// scratch (two places a CTA: a unit that began earlier, and one that goes on)
+// and attn_q4_join_kernel adds them in order.
 constexpr int kTile = 32;
 constexpr int kTileBlocks = kTile / kKvBlock;
+constexpr float kLowest = -3.402823466e38f;  // m before any key: 2^(m - anything seen) is 0
 
 struct RowsArgs {
     AttnQ4Args a;
@@ -84,6 +89,7 @@ struct RowsArgs {
     float* part_o;      // [2 * grid][8 NT][D]
     float2* part_ml;    // [2 * grid][8 NT]
     int grid;
+    int warps;          // of a CTA
 };
 
 // Tiles of sequence b (0: none of its rows is computed).
@@ -93,20 +99,6 @@ __device__ __forceinline__ int seq_tiles(const KvView& v, int b) {
     return max(1, (kv + kTile - 1) / kTile);
 }
 
-// Sum over the block of one number a thread (every thread gets it).
-template <int W>
-__device__ __forceinline__ int block_sum(int x, int* s) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
-    __syncthreads();
-    int t = 0;
-#pragma unroll 1
-    for (int w = 0; w < W; ++w) t += s[w];
-    return t;
-}
-
 __device__ __forceinline__ int tiles_a_cta(int total, int grid, int warps) {
     const int per = (total + grid - 1) / grid;
     return per < warps ? warps : per;
@@ -114,125 +106,244 @@ __device__ __forceinline__ int tiles_a_cta(int total, int grid, int warps) {
 
 template <int D, int NT, int W>
 struct RowsShape {
+    static constexpr bool kWhole = W > 8;  // a CTA has one unit, all of it
     static constexpr int kRows = NT * 8;
     static constexpr int kBlock = kKvBlock * (D + 8);
     static constexpr int kStage = kTileBlocks * kBlock;
-    static constexpr int kStages = W > 8 ? 2 : 4;
+    static constexpr int kStages = kWhole ? 2 : 3;
     static constexpr int kRing = W * kStages * kStage;
-    static constexpr int kMerge = W * kRows * D * 4;
+    // A warp's part of a unit: eight rows in the last slot of its ring, the others
+    // behind the rings; of a lone unit, all in its ring.
+    static constexpr int kOthers = kWhole ? 0 : W * (kRows - 8) * D * 4;
     static constexpr int kQ = NT * (D / 32) * 32 * 16;
-    static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kQ;
+    static constexpr int kBytes = kRing + kOthers + kQ;
+    static_assert((kWhole ? kRows : 8) * D * 4 <= (kWhole ? kStages : 1) * kStage, "parts fit");
+    static __device__ __forceinline__ float* part(uint8_t* smem, int w, int row) {
+        if (kWhole) return reinterpret_cast<float*>(smem + w * kStages * kStage) + row * D;
+        if (row < 8) return reinterpret_cast<float*>(smem + (w * kStages + kStages - 1) * kStage) + row * D;
+        return reinterpret_cast<float*>(smem + kRing) + (w * (kRows - 8) + row - 8) * D;
+    }
 };
 
-// The codes of one word as the halves of two operand registers each.
+// A part of a (sequence, kv head) as a CTA works on it.
+struct RowsUnit {
+    int seq, head, tiles, at;  // `at`: number of its first tile among all tiles
+    int t0, t1;                // tiles of this CTA
+    int first, n, kv;
+};
+
+// Wait for a warp's bulk copies, bounded; once one wait has given up (`late`)
+// the warp's others hardly wait.
+__device__ __forceinline__ void wait_tile(uint64_t* bar, uint32_t parity, int* flag, bool& late) {
+    uint64_t t0 = 0;
+#pragma unroll 1
+    for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
+        if ((it & 255u) != 0) continue;
+        if (t0 == 0) t0 = globaltimer_ns();
+        if (globaltimer_ns() - t0 > (late ? kWaitLimitNs >> 10 : kWaitLimitNs)) {
+            late = true;
+            raise_error(flag, kErrTmaWait);
+            return;
+        }
+    }
+}
+
+// max that keeps a NaN.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
 template <int D, int NT, int W>
-__global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args) {
+__global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 3 : 2))) attn_q4_few_kernel(const RowsArgs args) {
     using S = RowsShape<D, NT, W>;
-    constexpr int kWords = D / 32;  // words of a lane: K row part, and V channel stretch of two tokens
+    constexpr int kWords = D / 32;               // words of a lane: K row part, and V channel stretch of two tokens
+    constexpr int kMine = (S::kRows + W - 1) / W;  // rows whose q a warp lays out
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t s_full[W][S::kStages];
     __shared__ int s_sum[W];
     __shared__ int s_seq, s_at;
     __shared__ float s_fac[S::kRows], s_sumq[S::kRows];
     __shared__ int s_limit[S::kRows];
     __shared__ float s_m[W][S::kRows], s_l[W][S::kRows];
-    uint8_t* ring = smem;
-    float* merge = reinterpret_cast<float*>(smem);  // once the ring has run dry
     uint4* qf = reinterpret_cast<uint4*>(smem + S::kBytes - S::kQ);
     const AttnQ4Args& a = args.a;
     const KvView& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    uint8_t* ring = smem + warp * S::kStages * S::kStage;
 
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < S::kStages; ++i) mbar_init(&s_full[warp][i], kTileBlocks);
+        fence_barrier_init();
+    }
+    __syncwarp();
     griddep_wait();
     griddep_launch_dependents();
 
-    // This CTA's stretch of the tiles, and the sequence it begins in.
-    int mine = 0;
-    for (int b = threadIdx.x; b < v.seqs; b += W * 32) {
-        mine += seq_tiles(v, b);
-        int f, n, kv;
-        if (!kv_seq(v, b, &f, &n, &kv) && blockIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
-    }
-    const int total = block_sum<W>(mine, s_sum) * v.kv_heads;
-    int at, end, seq;
-    int seq_at;  // tile number at which the sequence begins
-    if (args.split) {
+    // This CTA's stretch of the tiles, and the unit it begins in.
+    RowsUnit u;
+    int at, end, seq_at;  // seq_at: tile number at which the unit's sequence begins
+    if constexpr (!S::kWhole) {
+        int incl, t, base, chunk;
+        auto scan = [&](int b0) {  // tiles of W * 32 sequences from b0 on
+            const int b = b0 + threadIdx.x;
+            t = b < v.seqs ? seq_tiles(v, b) * v.kv_heads : 0;
+            incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            if (lane == 31) s_sum[warp] = incl;
+            __syncthreads();
+            base = chunk = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (w < warp) base += s_sum[w];
+                chunk += s_sum[w];
+            }
+            __syncthreads();
+        };
+        int total = 0;
+        for (int b0 = (v.seqs - 1) / (W * 32) * (W * 32); b0 >= 0; b0 -= W * 32) {  // the first ones last
+            scan(b0);
+            total += chunk;
+        }
+        if (blockIdx.x == 0)
+            for (int b = threadIdx.x; b < v.seqs; b += W * 32) {
+                int f, n, kv;
+                if (!kv_seq(v, b, &f, &n, &kv)) raise_error(v.err_flag, kErrBadPage);
+            }
         const int per = tiles_a_cta(total, args.grid, W);
         at = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(blockIdx.x) * per));
         end = min(total - at, per) + at;
         if (at >= end) return;
-        int before = 0;
-        seq = -1;
-        seq_at = 0;
-        for (int b0 = 0; seq < 0; b0 += W * 32) {  // ends: at < total
-            const int b = b0 + threadIdx.x;
-            const int t = b < v.seqs ? seq_tiles(v, b) * v.kv_heads : 0;
-            int incl = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                if (lane >= o) incl += u;
+        for (int b0 = 0, before = 0;;) {  // ends: at < total
+            const int lo = before + base + incl - t;
+            if (at >= lo && at < lo + t) {
+                s_seq = b0 + threadIdx.x;
+                s_at = lo;
             }
-            __syncthreads();
-            if (threadIdx.x == 0) s_seq = -1;
-            if (lane == 31) s_sum[warp] = incl;
-            __syncthreads();
-            int base = before;
-#pragma unroll 1
-            for (int w = 0; w < warp; ++w) base += s_sum[w];
-            if (at >= base + incl - t && at < base + incl) {
-                s_seq = b;
-                s_at = base + incl - t;
-            }
-#pragma unroll 1
-            for (int w = 0; w < W; ++w) before += s_sum[w];
-            __syncthreads();
-            seq = s_seq;
-            seq_at = s_at;
+            before += chunk;
+            if (at < before) break;
+            b0 += W * 32;
+            scan(b0);
         }
+        __syncthreads();
+        u.seq = s_seq;
+        seq_at = s_at;
+        u.tiles = seq_tiles(v, u.seq);
     } else {
-        seq = blockIdx.x / v.kv_heads;
-        const int t = seq_tiles(v, seq);
-        if (t == 0) return;
+        u.seq = blockIdx.x / v.kv_heads;
+        u.tiles = seq_tiles(v, u.seq);
+        int f, n, kv;
+        if (!kv_seq(v, u.seq, &f, &n, &kv) && threadIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
+        if (u.tiles == 0) return;
         seq_at = 0;
-        at = static_cast<int>(blockIdx.x % v.kv_heads) * t;
-        end = at + t;
+        at = static_cast<int>(blockIdx.x % v.kv_heads) * u.tiles;
+        end = at + u.tiles;
     }
     const int range_begin = at;
 
-    while (at < end) {
-        // The next unit of the stretch: tiles [t0, t1) of (seq, head).
-        int tiles = seq_tiles(v, seq);
-        while (at >= seq_at + tiles * v.kv_heads) {
-            seq_at += tiles * v.kv_heads;
-            ++seq;
-            tiles = seq_tiles(v, seq);
+    // The unit that `at` lies in.
+    auto find = [&]() {
+        while (at >= seq_at + u.tiles * v.kv_heads) {
+            seq_at += u.tiles * v.kv_heads;
+            ++u.seq;
+            u.tiles = seq_tiles(v, u.seq);
         }
-        const int head = (at - seq_at) / tiles;
-        const int unit_at = seq_at + head * tiles;
-        const int t0 = at - unit_at;
-        const int t1 = min(tiles, t0 + (end - at));
-        int first, n, kv;
-        kv_seq(v, seq, &first, &n, &kv);
-        const int rows = n * args.group;  // <= 8 NT
+        u.head = (at - seq_at) / u.tiles;
+        u.at = seq_at + u.head * u.tiles;
+        u.t0 = at - u.at;
+        u.t1 = min(u.tiles, u.t0 + (end - at));
+        kv_seq(v, u.seq, &u.first, &u.n, &u.kv);
+    };
 
+    // This warp's tiles of the unit: t0 + warp, + W, ....  Lane l sees to block l of
+    // sixteen of them: its page's number (asked for sixteen tiles early) and address.
+    int count, page_next;
+    const uint8_t* blk = nullptr;
+    const int32_t* row_table;
+    auto block_pos = [&](int i) { return (u.t0 + warp + (i + (lane >> 1)) * W) * kTile + (lane & 1) * kKvBlock; };
+    auto ask = [&](int i) {  // -2: no such block
+        const int pos = block_pos(i);
+        page_next = -2;
+        if (i + (lane >> 1) < count && pos < u.kv) {
+            const int slot = kv_slot(v, pos);
+            page_next = slot < v.ld_table ? row_table[slot] : -1;
+        }
+    };
+    auto issue = [&](int i) {
+        if (i >= count) return;
+        if ((i & 15) == 0) {
+            const int pos = block_pos(i);
+            blk = nullptr;
+            if (page_next != -2) {
+                const int n = kv_block_in(v, page_next, kv_slot(v, pos), u.head, pos);
+                if (n < 0) raise_error(v.err_flag, kErrBadPage);
+                else blk = v.data + static_cast<int64_t>(n) * S::kBlock;
+            }
+            ask(i + 16);
+        }
+        if ((lane >> 1) == (i & 15)) {
+            uint64_t* bar = &s_full[warp][i % S::kStages];
+            if (blk != nullptr) {
+                mbar_arrive_expect_tx(bar, S::kBlock);
+                bulk_load(ring + (i % S::kStages) * S::kStage + (lane & 1) * S::kBlock, blk, S::kBlock, bar);
+            } else {
+                mbar_arrive(bar);
+            }
+        }
+    };
+    // q of this warp's rows of the unit, D / 32 neighbouring channels a lane.
+    uint32_t qw[kMine][D / 64];
+    auto start = [&]() {
+        row_table = v.table + static_cast<int64_t>(u.seq) * v.ld_table;
+        count = u.t1 - u.t0 > warp ? (u.t1 - u.t0 - warp + W - 1) / W : 0;
+        ask(0);
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int row = warp + k * W, i = row / args.group, g = row - i * args.group;
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) qw[k][j] = 0;
+            if (row < u.n * args.group) {
+                const uint16_t* src = a.q + (u.first + i) * a.ldq + (u.head * args.group + g) * D + lane * (D / 32);
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) qw[k][j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < (S::kWhole ? S::kStages : S::kStages - 1); ++i) issue(i);
+    };
+    find();
+    start();
+    uint32_t phases = 0;  // of the ring's slots
+    bool late = false;
+
+    for (;;) {
         // q: each row to FP16 by a power of two (its largest channel to
         // 2^13..2^14: FP16 and BF16 rows keep all their bits down to 2^-23 of
         // it), in the order of the MMA's B fragments.
-        for (int row = warp; row < S::kRows; row += W) {
+        const int rows = u.n * args.group;  // <= 8 NT
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {
+            const int row = warp + k * W;
+            if (S::kRows % W != 0 && row >= S::kRows) break;
             constexpr int PER = D / 32;
             float x[PER], big = 0.0f;
-            const int i = row / args.group, g = row - i * args.group;
-            const bool live = row < rows;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                x[j] = live ? widen(a.q[(first + i) * a.ldq + (head * args.group + g) * D + lane * PER + j], a.dtype) : 0.0f;
+                x[j] = widen(static_cast<uint16_t>(qw[k][j >> 1] >> (16 * (j & 1))), a.dtype);
                 big = fmaxf(big, fabsf(x[j]));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-            int e = big > 0.0f && big <= 3.402823466e38f ? ilogbf(big) - 13 : 0;
-            e = max(e, -100);
-            const float down = scalbnf(1.0f, -e);
+            const int e = big < INFINITY ? max((__float_as_int(big) >> 23) - 140, -100) : 0;
+            const float down = pow2(-e);
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
@@ -246,14 +357,15 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
             if (lane == 0) {
-                s_fac[row] = scalbnf(a.scale * 1.4426950408889634f, 24 + e);
+                s_fac[row] = a.scale * (1.4426950408889634f * 4096.0f) * pow2(12 + e);
                 s_sumq[row] = sum * 5.9604644775390625e-8f;
-                s_limit[row] = !live ? 0 : (a.causal ? kv - n + i + 1 : kv);
+                s_limit[row] = row >= rows ? 0 : (a.causal ? u.kv - u.n + row / args.group + 1 : u.kv);
             }
         }
         __syncthreads();
+        if constexpr (!S::kWhole) issue(S::kStages - 1);  // its slot held the last unit's part
         float fac[NT][2], sq[NT][2];
-        int limit[NT][2], limit_min = 0x7FFFFFFF;
+        int limit_min = 0x7FFFFFFF;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -261,79 +373,43 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
                 const int row = t * 8 + c * 2 + j;
                 fac[t][j] = s_fac[row];
                 sq[t][j] = s_sumq[row];
-                limit[t][j] = s_limit[row];
-                if (row < rows) limit_min = min(limit_min, limit[t][j]);
+                if (row < rows) limit_min = min(limit_min, s_limit[row]);
             }
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
-        uint4 qr[NT <= 2 ? NT : 1][kWords];
-        if constexpr (NT <= 2) {
+        uint4 qr[NT == 1 ? NT : 1][kWords];
+        if constexpr (NT == 1) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) qr[t][i] = qf[(t * kWords + i) * 32 + lane];
+            for (int i = 0; i < kWords; ++i) qr[0][i] = qf[i * 32 + lane];
         }
 
-        float m[NT][2], l[NT][2], zs[NT][2], o[D / 16][NT][4];
+        float m[NT][2], l[NT][2], zs[NT][4], o[D / 16][NT][4];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                m[t][j] = -INFINITY;
-                l[t][j] = zs[t][j] = 0.0f;
+                m[t][j] = kLowest;
+                l[t][j] = 0.0f;
             }
 #pragma unroll
-            for (int ct = 0; ct < D / 16; ++ct)
+            for (int j = 0; j < 4; ++j) {
+                zs[t][j] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[ct][t][j] = 0.0f;
+                for (int ct = 0; ct < D / 16; ++ct) o[ct][t][j] = 0.0f;
+            }
         }
 
-        // This warp's tiles: t0 + warp, + W, ...; lane l holds the page of the
-        // l-th of the next 32 blocks.
-        const int32_t* row_table = v.table + static_cast<int64_t>(seq) * v.ld_table;
-        uint8_t* my_ring = ring + warp * S::kStages * S::kStage;
-        const uint32_t my_ring_u32 = smem_u32(my_ring);
-        const int count = t1 - t0 > warp ? (t1 - t0 - warp + W - 1) / W : 0;
-        const uint8_t* blk = nullptr;  // lane's block address, or null
-        auto fill = [&](int i) {       // addresses of blocks of tiles i .. i + 15
-            const int tile = t0 + warp + (i + (lane >> 1)) * W;
-            const int pos = tile * kTile + (lane & 1) * kKvBlock;
-            blk = nullptr;
-            if (i + (lane >> 1) < count && pos < kv) {
-                blk = kv_block_at(v, row_table, head, pos);
-                if (blk == nullptr) raise_error(v.err_flag, kErrBadPage);
-            }
-        };
-        auto issue = [&](int i) {
-            if (i < count) {
-                if ((i & 15) == 0) fill(i);
-                const uint32_t dst = my_ring_u32 + (i % S::kStages) * S::kStage;
-#pragma unroll
-                for (int h = 0; h < kTileBlocks; ++h) {
-                    const uint64_t src = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(blk), (i & 15) * 2 + h);
-                    const uint8_t* p = src != 0 ? reinterpret_cast<const uint8_t*>(src) : v.data;
-#pragma unroll
-                    for (int x = 0; x < (S::kBlock + 511) / 512; ++x) {
-                        const int off = x * 512 + lane * 16;
-                        if (off < S::kBlock) copy_async_16(dst + h * S::kBlock + off, p + off, src != 0);
-                    }
-                }
-            }
-            copy_async_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) issue(i);
-
+#pragma unroll 1
         for (int i = 0; i < count; ++i) {
-            copy_async_wait<S::kStages - 2>();
-            __syncwarp();
-            issue(i + S::kStages - 1);
-            const uint8_t* stage = my_ring + (i % S::kStages) * S::kStage;
-            const int pos0 = (t0 + warp + i * W) * kTile;
-            const bool inner = pos0 + kTile <= limit_min;  // every row sees every token
+            const int slot = i % S::kStages;
+            wait_tile(&s_full[warp][slot], (phases >> slot) & 1, v.err_flag, late);
+            phases ^= 1u << slot;
+            const uint8_t* stage = ring + slot * S::kStage;
+            const int pos0 = (u.t0 + warp + i * W) * kTile;
 
             float y[kTileBlocks][NT][4];
-            float rs[kTileBlocks][2], zv[kTileBlocks][2];
+            float rs[kTileBlocks][2];
+            uint32_t z[kTileBlocks][2];  // zero points of V: tokens 2c, 2c + 1 and 2c + 8, 2c + 9
 #pragma unroll
             for (int h = 0; h < kTileBlocks; ++h) {
                 const uint8_t* b = stage + h * S::kBlock;
@@ -349,166 +425,167 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
                     k1[0] = u1.x; k1[1] = u1.y;
                 }
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y[h][t][j] = 0.0f;
-#pragma unroll
                 for (int w = 0; w < kWords; ++w) {
                     const uint32_t s0 = k0[w] >> 8, s1 = k1[w] >> 8;
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
                         uint4 q;
-                        if constexpr (NT <= 2) q = qr[t][w];
+                        if constexpr (NT == 1) q = qr[t][w];
                         else q = qf[(t * kWords + w) * 32 + lane];
-                        mma_f16(y[h][t], k0[w] & kNib0, k1[w] & kNib0, s0 & kNib0, s1 & kNib0, q.x, q.y);
+                        if (w == 0) mma_f16_first(y[h][t], k0[w] & kNib0, k1[w] & kNib0, s0 & kNib0, s1 & kNib0, q.x, q.y);
+                        else mma_f16(y[h][t], k0[w] & kNib0, k1[w] & kNib0, s0 & kNib0, s1 & kNib0, q.x, q.y);
                         mma_f16(y[h][t], k0[w] & kNib1, k1[w] & kNib1, s0 & kNib1, s1 & kNib1, q.z, q.w);
                     }
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int token = half * 8 + r;
-                    uint32_t ks = reinterpret_cast<const uint32_t*>(b + kv_k_scales(D))[token];
-                    uint32_t vs = reinterpret_cast<const uint32_t*>(b + kv_v_scales(D))[token];
-                    if (pos0 + h * kKvBlock + token >= kv) ks = vs = 0x3C00u;  // nobody's: scale 1, zero point 0
-                    if ((vs & 0xFFFFu) == 0) vs |= 1u;  // never stored: holds zeros whatever its scale
-                    const float sk = f16_bits_to_f32(static_cast<uint16_t>(ks)), sv = f16_bits_to_f32(static_cast<uint16_t>(vs));
-                    const float zk = static_cast<float>(ks >> 16), lv = fast_log2(sv);
-                    rs[h][half] = fast_rcp(sv);
-                    zv[h][half] = static_cast<float>(vs >> 16);
+                    const uint32_t ks = reinterpret_cast<const uint32_t*>(b + kv_k_scales(D))[token];
+                    const uint16_t vs = *reinterpret_cast<const uint16_t*>(b + kv_v_scales(D) + token * 4);
+                    const float sk = f16_bits_to_f32(static_cast<uint16_t>(ks)), zk = f16_bits_to_f32(static_cast<uint16_t>(ks >> 16));
+                    // (never stored: scale 0; it holds zeros whatever its scale)
+                    const float sv = max_nan(f16_bits_to_f32(vs), 5.9604644775390625e-8f), lv = fast_log2(sv);
+                    // A row that sees a NaN scale has a NaN p; the others' sums must not.
+                    rs[h][half] = fminf(fast_rcp(sv), 16777216.0f);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             float& e = y[h][t][half * 2 + j];
                             e = fmaf(fmaf(-zk, sq[t][j], e) * sk, fac[t][j], lv);
-                            if (!inner && pos0 + h * kKvBlock + token >= limit[t][j]) e = -INFINITY;
                         }
+                    const uint2 zw = *reinterpret_cast<const uint2*>(b + kv_v_scales(D) + half * 32 + c * 8);
+                    z[h][half] = __byte_perm(zw.x, zw.y, 0x7632);
                 }
             }
-            uint32_t pb[kTileBlocks][NT][2];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float base[2], fix[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float big = fmaxf(fmaxf(y[0][t][j], y[0][t][2 + j]), fmaxf(y[1][t][j], y[1][t][2 + j]));
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, off));
-                    big = fmaxf(big, m[t][j]);
-                    base[j] = big == -INFINITY ? 0.0f : big;  // no key seen yet
-                    fix[j] = fast_exp2(m[t][j] - base[j]);
-                    m[t][j] = big;
-                }
-                if (__any_sync(0xFFFFFFFFu, fix[0] != 1.0f || fix[1] != 1.0f)) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        l[t][j] *= fix[j];
-                        zs[t][j] *= fix[j];
-#pragma unroll
-                        for (int ct = 0; ct < D / 16; ++ct) {
-                            o[ct][t][j] *= fix[j];
-                            o[ct][t][2 + j] *= fix[j];
-                        }
-                    }
-                }
+            if (pos0 + kTile > limit_min) {  // some row does not see every token
 #pragma unroll
                 for (int h = 0; h < kTileBlocks; ++h)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int pos = pos0 + h * kKvBlock + half * 8;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                if (pos + r >= s_limit[t * 8 + c * 2 + j]) y[h][t][half * 2 + j] = -INFINITY;
+                        // nobody's: bytes of any kind
+                        if (pos + 2 * c >= u.kv) z[h][half] &= 0xFFFF0000u;
+                        if (pos + 2 * c + 1 >= u.kv) z[h][half] &= 0x0000FFFFu;
+                    }
+            }
+            bool far = false;
+            float big[NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    big[t][j] = fmaxf(fmaxf(y[0][t][j], y[0][t][2 + j]), fmaxf(y[1][t][j], y[1][t][2 + j]));
+                    far |= big[t][j] > m[t][j] + 8.0f;
+                }
+            if (__any_sync(0xFFFFFFFFu, far)) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float x = fmaxf(big[t][j], m[t][j]);
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, off));
+                        const float fix = fast_exp2(m[t][j] - x);
+                        m[t][j] = x;
+                        l[t][j] *= fix;
+                        zs[t][j] *= fix;
+#pragma unroll
+                        for (int ct = 0; ct < D / 16; ++ct) {
+                            o[ct][t][j] *= fix;
+                            o[ct][t][2 + j] *= fix;
+                        }
+                    }
+            }
+#pragma unroll
+            for (int h = 0; h < kTileBlocks; ++h) {
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float p[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float e = y[h][t][half * 2 + j];
-                            p[j] = fast_exp2(e - base[j]);
-                            // a masked token's scale may be NaN: it must not enter the sum
-                            const float add = p[j] * rs[h][half];
-                            l[t][j] += !inner && e == -INFINITY ? 0.0f : add;
+                            p[j] = fast_exp2(y[h][t][half * 2 + j] - m[t][j]);
+                            l[t][j] = fmaf(p[j], rs[h][half], l[t][j]);
                         }
                         const __half2 hp = __floats2half2_rn(p[0], p[1]);
-                        const float2 back = __half22float2(hp);
-                        zs[t][0] = fmaf(back.x, zv[h][half], zs[t][0]);
-                        zs[t][1] = fmaf(back.y, zv[h][half], zs[t][1]);
-                        pb[h][t][half] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hp));
+                        pb[t][half] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&hp));
                     }
-            }
-#pragma unroll
-            for (int h = 0; h < kTileBlocks; ++h) {
+                    mma_f16(zs[t], z[h][0], 0u, z[h][1], 0u, pb[t][0], pb[t][1]);
+                }
                 const uint8_t* vp = stage + h * S::kBlock + kv_v_codes(D) + lane * (D / 8);
-                // [token half][token of the pair][word]
-                uint32_t vw[2][2][D / 64];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if constexpr (D == 128) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(vp + half * 4 * D);
-                        vw[half][0][0] = u.x; vw[half][0][1] = u.y;
-                        vw[half][1][0] = u.z; vw[half][1][1] = u.w;
-                    } else {
-                        const uint2 u = *reinterpret_cast<const uint2*>(vp + half * 4 * D);
-                        vw[half][0][0] = u.x;
-                        vw[half][1][0] = u.y;
-                    }
+                uint32_t v0[kWords], v1[kWords];  // tokens 0-7, 8-15
+                if constexpr (D == 128) {
+                    const uint4 u0 = *reinterpret_cast<const uint4*>(vp), u1 = *reinterpret_cast<const uint4*>(vp + 4 * D);
+                    v0[0] = u0.x; v0[1] = u0.y; v0[2] = u0.z; v0[3] = u0.w;
+                    v1[0] = u1.x; v1[1] = u1.y; v1[2] = u1.z; v1[3] = u1.w;
+                } else {
+                    const uint2 u0 = *reinterpret_cast<const uint2*>(vp), u1 = *reinterpret_cast<const uint2*>(vp + 4 * D);
+                    v0[0] = u0.x; v0[1] = u0.y;
+                    v1[0] = u1.x; v1[1] = u1.y;
                 }
 #pragma unroll
-                for (int w = 0; w < D / 64; ++w)
+                for (int w = 0; w < kWords; ++w) {
+                    const uint32_t s0 = v0[w] >> 8, s1 = v1[w] >> 8;
 #pragma unroll
-                    for (int hi = 0; hi < 2; ++hi) {  // nibbles 0-3, then 4-7
-                        const uint32_t x0 = __byte_perm(vw[0][0][w], vw[0][1][w], hi ? 0x7632 : 0x5410);
-                        const uint32_t x1 = __byte_perm(vw[1][0][w], vw[1][1][w], hi ? 0x7632 : 0x5410);
-                        const uint32_t u0 = x0 >> 8, u1 = x1 >> 8;
-                        const int ct = w * 4 + hi * 2;
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            mma_f16(o[ct][t], x0 & kNib0, x0 & kNib1, x1 & kNib0, x1 & kNib1, pb[h][t][0], pb[h][t][1]);
-                            mma_f16(o[ct + 1][t], u0 & kNib0, u0 & kNib1, u1 & kNib0, u1 & kNib1, pb[h][t][0], pb[h][t][1]);
-                        }
+                    for (int t = 0; t < NT; ++t) {
+                        mma_f16(o[2 * w][t], v0[w] & kNib0, v0[w] & kNib1, v1[w] & kNib0, v1[w] & kNib1, pb[t][0], pb[t][1]);
+                        mma_f16(o[2 * w + 1][t], s0 & kNib0, s0 & kNib1, s1 & kNib0, s1 & kNib1, pb[t][0], pb[t][1]);
                     }
+                }
             }
-            __syncwarp();
+            __syncwarp();  // the slot is read
+            issue(i + S::kStages);
         }
-        copy_async_wait<0>();
 
-        // Join the warps: channel r D/8 + 2 ct in o[ct][.][0..1] (times 2^-24),
-        // the next one in [2..3] (times 2^-20).
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
-                    l[t][j] += __shfl_xor_sync(0xFFFFFFFFu, l[t][j], off);
-                    zs[t][j] += __shfl_xor_sync(0xFFFFFFFFu, zs[t][j], off);
-                }
-        __syncthreads();  // every warp is done with the ring
+        // Join the warps, with the next unit's copies under way.
+        const RowsUnit done = u;
+        at += u.t1 - u.t0;
+        const bool more = !S::kWhole && at < end;
+        if (more) {
+            find();
+            start();
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) l[t][j] += __shfl_xor_sync(0xFFFFFFFFu, l[t][j], off);
                 const int row = t * 8 + c * 2 + j;
                 if (r == 0) {
                     s_m[warp][row] = m[t][j];
                     s_l[warp][row] = l[t][j];
                 }
-                float* dst = merge + (warp * S::kRows + row) * D + r * (D / 8);
+                // channel r D/8 + 2 ct in o[ct][.][0..1] (times 2^-24), the next one in [2..3] (times 2^-20)
+                float* dst = S::part(smem, warp, row) + r * (D / 8);
 #pragma unroll
                 for (int ct = 0; ct < D / 16; ++ct)
                     *reinterpret_cast<float2*>(dst + 2 * ct) =
                         make_float2(fmaf(o[ct][t][j], 16777216.0f, -zs[t][j]), fmaf(o[ct][t][2 + j], 1048576.0f, -zs[t][j]));
             }
+        fence_async_smem();  // the slot's next copy comes after these
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == tiles;
-        const int64_t slot = blockIdx.x * 2LL + (unit_at > range_begin ? 1 : 0);
+        const bool whole = done.t0 == 0 && done.t1 == done.tiles;
+        const int64_t place = blockIdx.x * 2LL + (done.at > range_begin ? 1 : 0);
         for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
             const int row = i / (D / 4), ch = (i - row * (D / 4)) * 4;
-            float big = -INFINITY;
+            float big = kLowest;
 #pragma unroll
             for (int w = 0; w < W; ++w) big = fmaxf(big, s_m[w][row]);
-            const float base = big == -INFINITY ? 0.0f : big;
             float sum = 0.0f;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float f = fast_exp2(s_m[w][row] - base);
-                const float4 x = *reinterpret_cast<const float4*>(merge + (w * S::kRows + row) * D + ch);
+                const float f = fast_exp2(s_m[w][row] - big);
+                const float4 x = *reinterpret_cast<const float4*>(S::part(smem, w, row) + ch);
                 sum = fmaf(s_l[w][row], f, sum);
                 acc.x = fmaf(x.x, f, acc.x);
                 acc.y = fmaf(x.y, f, acc.y);
@@ -518,88 +595,133 @@ __global__ void __launch_bounds__(W * 32) attn_q4_few_kernel(const RowsArgs args
             if (whole) {
                 const float inv = sum == 0.0f ? 0.0f : fast_rcp(sum);
                 const int qi = row / args.group, g = row - qi * args.group;
-                uint16_t* dst = a.out + (first + qi) * a.ldo + (head * args.group + g) * D + ch;
+                uint16_t* dst = a.out + (done.first + qi) * a.ldo + (done.head * args.group + g) * D + ch;
                 store2(dst, narrow2(acc.x * inv, acc.y * inv, a.dtype));
                 store2(dst + 2, narrow2(acc.z * inv, acc.w * inv, a.dtype));
             } else {
-                *reinterpret_cast<float4*>(args.part_o + (slot * S::kRows + row) * D + ch) = acc;
-                if (ch == 0) args.part_ml[slot * S::kRows + row] = make_float2(big, sum);
+                *reinterpret_cast<float4*>(args.part_o + (place * S::kRows + row) * D + ch) = acc;
+                if (ch == 0) args.part_ml[place * S::kRows + row] = make_float2(big, sum);
             }
         }
-        __syncthreads();
-        at += t1 - t0;
+        if (!more) break;
     }
 }
 
-// Adds the parts of the units that span CTAs.  One CTA per (unit, row); its
-// eight warps take the parts in turn.
-template <int D, int NT, int W>
-__global__ void __launch_bounds__(kThreads) attn_q4_join_kernel(const RowsArgs args) {
-    constexpr int kRows = NT * 8, PER = D / 32;
-    __shared__ int s_sum[kThreads / 32];
-    __shared__ float s_m[kThreads / 32], s_l[kThreads / 32];
-    __shared__ float s_o[kThreads / 32][D];
-    griddep_wait();
-    griddep_launch_dependents();
+// Adds the parts of the units that span CTAs, in order.  One CTA per (unit,
+// row): the parts' weights, as many at a time as the CTA has threads, then
+// their sums, a warp (half a warp) a part.
+constexpr int kJoinMax = 512;
+
+template <int D>
+__global__ void __launch_bounds__(kJoinMax) attn_q4_join_kernel(const RowsArgs args, int kRows) {
+    constexpr int LANES = D / 4;  // of a part: four channels each
+    __shared__ int s_a[kJoinMax / 32], s_b[kJoinMax / 32];
+    __shared__ float s_w[kJoinMax];
+    __shared__ float s_big[kJoinMax / 32], s_sum[kJoinMax / 32];
+    __shared__ float4 s_o[kJoinMax];
     const AttnQ4Args& a = args.a;
     const KvView& v = a.v;
+    const int threads = blockDim.x, warps = threads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int seq = blockIdx.x / v.kv_heads, head = blockIdx.x - seq * v.kv_heads, row = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles = seq_tiles(v, seq);
-    int first, n, kv;
-    if (tiles == 0 || !kv_seq(v, seq, &first, &n, &kv) || row >= n * args.group) return;
+    // The call's lengths are older than the kernel whose parts this one waits for
+    // (that kernel lets this one start once it has waited for all before it).
     int all = 0, before = 0;
-    for (int b = threadIdx.x; b < v.seqs; b += kThreads) {
+    for (int b = threadIdx.x; b < v.seqs; b += threads) {
         const int t = seq_tiles(v, b);
         all += t;
         if (b < seq) before += t;
     }
-    const int total = block_sum<kThreads / 32>(all, s_sum) * v.kv_heads;
-    const int unit_at = block_sum<kThreads / 32>(before, s_sum) * v.kv_heads + head * tiles;
-    const int per = tiles_a_cta(total, args.grid, W);
-    const int c0 = unit_at / per, c1 = (unit_at + tiles - 1) / per;
-    if (c0 == c1) return;  // that CTA stored the output
-    float m = -INFINITY, l = 0.0f, o[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) o[j] = 0.0f;
-    for (int p = c0 + warp; p <= c1; p += kThreads / 32) {
-        const int64_t at = (p * 2LL + (unit_at > p * per ? 1 : 0)) * kRows + row;
-        const float2 ml = args.part_ml[at];
-        float x[PER];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) x[j] = args.part_o[at * D + lane * PER + j];
-        const float big = fmaxf(m, ml.x), base = big == -INFINITY ? 0.0f : big;
-        const float f0 = fast_exp2(m - base), f1 = fast_exp2(ml.x - base);
-        l = l * f0 + ml.y * f1;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] = o[j] * f0 + x[j] * f1;
-        m = big;
+    for (int o = 16; o > 0; o >>= 1) {
+        all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
     }
     if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
+        s_a[warp] = all;
+        s_b[warp] = before;
+    }
+    __syncthreads();
+    all = before = 0;
+    for (int w = 0; w < warps; ++w) {
+        all += s_a[w];
+        before += s_b[w];
+    }
+    const int tiles = seq_tiles(v, seq);
+    int first, n, kv;
+    const bool live = kv_seq(v, seq, &first, &n, &kv) && tiles != 0 && row < n * args.group;
+    const int unit_at = before * v.kv_heads + head * tiles;
+    const int per = tiles_a_cta(all * v.kv_heads, args.grid, args.warps);
+    const int c0 = unit_at / per, c1 = (unit_at + tiles - 1) / per;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (!live || c0 == c1) return;  // (the one CTA stored the output)
+    auto place = [&](int p) { return (p * 2LL + (unit_at > p * per ? 1 : 0)) * kRows + row; };
+    float m = kLowest, l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int ch = (threadIdx.x % LANES) * 4, mine = threadIdx.x / LANES, step = threads / LANES;
+    for (int p0 = c0; p0 <= c1; p0 += threads) {
+        const int parts = min(threads, c1 - p0 + 1);
+        float2 ml = make_float2(kLowest, 0.0f);
+        if (threadIdx.x < parts) ml = args.part_ml[place(p0 + threadIdx.x)];
+        float big = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+        if (lane == 0) s_big[warp] = big;
+        __syncthreads();
+        big = m;
+        for (int w = 0; w < warps; ++w) big = fmaxf(big, s_big[w]);
+        const float f = fast_exp2(ml.x - big), fix = fast_exp2(m - big);
+        s_w[threadIdx.x] = f;
+        l = fmaf(l, fix, threadIdx.x < parts ? ml.y * f : 0.0f);
+        acc = make_float4(acc.x * fix, acc.y * fix, acc.z * fix, acc.w * fix);
+        m = big;
+        __syncthreads();
+#pragma unroll 4
+        for (int p = mine; p < parts; p += step) {
+            const float g = s_w[p];
+            const float4 x = *reinterpret_cast<const float4*>(args.part_o + place(p0 + p) * D + ch);
+            acc.x = fmaf(x.x, g, acc.x);
+            acc.y = fmaf(x.y, g, acc.y);
+            acc.z = fmaf(x.z, g, acc.z);
+            acc.w = fmaf(x.w, g, acc.w);
+        }
+        __syncthreads();
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) s_o[warp][lane * PER + j] = o[j];
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+    if (lane == 0) s_sum[warp] = l;
+    s_o[threadIdx.x] = acc;
     __syncthreads();
-    if (threadIdx.x < D) {
-        float big = -INFINITY;
-        for (int w = 0; w < kThreads / 32; ++w) big = fmaxf(big, s_m[w]);
-        const float base = big == -INFINITY ? 0.0f : big;
-        float sum = 0.0f, acc = 0.0f;
-        for (int w = 0; w < kThreads / 32; ++w) {
-            const float f = fast_exp2(s_m[w] - base);
-            sum = fmaf(s_l[w], f, sum);
-            acc = fmaf(s_o[w][threadIdx.x], f, acc);
+    if (threadIdx.x < LANES) {
+        float sum = 0.0f;
+        for (int w = 0; w < warps; ++w) sum += s_sum[w];
+        for (int k = 1; k < step; ++k) {
+            const float4 x = s_o[k * LANES + threadIdx.x];
+            acc = make_float4(acc.x + x.x, acc.y + x.y, acc.z + x.z, acc.w + x.w);
         }
         const float inv = sum == 0.0f ? 0.0f : fast_rcp(sum);
         const int qi = row / args.group, g = row - qi * args.group;
-        a.out[(first + qi) * a.ldo + (head * args.group + g) * D + threadIdx.x] =
-            static_cast<uint16_t>(narrow2(acc * inv, 0.0f, a.dtype));
+        uint16_t* dst = a.out + (first + qi) * a.ldo + (head * args.group + g) * D + ch;
+        store2(dst, narrow2(acc.x * inv, acc.y * inv, a.dtype));
+        store2(dst + 2, narrow2(acc.z * inv, acc.w * inv, a.dtype));
     }
 }
 
 // ------------------------------------------------------------------ many rows
+
+// Sum over the block of one number a thread (every thread gets it).
+template <int W>
+__device__ __forceinline__ int block_sum(int x, int* s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
+    __syncthreads();
+    int t = 0;
+#pragma unroll 1
+    for (int w = 0; w < W; ++w) t += s[w];
+    return t;
+}
 
 // TMEM accesses in MMA-fragment order, 16 lanes (rows) at a time: lane (r, c)
 // of the warp gets, of every eight 32-bit columns, columns 2c and 2c + 1 of
@@ -721,7 +843,6 @@ __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volat
     }
 }
 
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Many rows (prompts, chunks of prompts): tcgen05 flash attention.  A CTA
 // takes 256 rows of a (sequence, kv head) -- new tokens times the query heads
@@ -855,6 +976,11 @@ __device__ __forceinline__ void st_shared_16(uint32_t addr, uint32_t x, uint32_t
 
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
@@ -1309,8 +1435,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                     if ((z[0].y & 0x7C00u) == 0x7C00u) sk = __int_as_float(0x7FFFFFFF);
                     *reinterpret_cast<float*>(cols + st * S::kCols + ((token >> 1) & 3) * S::kColsRow + (token >> 3) * 8 +
                                               (token & 1) * 4) = sk;
-                    const uint32_t zz = (z[0].x >> 16) * 0x10001u;
-                    const uint32_t z1024 = 0x64006400u | zz, z64 = 0xD400D400u | zz << 4, z128 = 0x43004300u | zz;
+                    const uint32_t z1024 = h2_add(__byte_perm(z[0].x, 0, 0x3232), 0x64006400u), zz = z1024 & kNib0;
+                    const uint32_t z64 = 0xD400D400u | zz << 4, z128 = 0x43004300u | zz;
                     const uint32_t kst = k_u32 + st * S::kK;
 #pragma unroll
                     for (int k = 0; k < D / 8; ++k) {
@@ -1337,25 +1463,28 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                     const uint32_t zw[8] = {z[0].x, z[0].y, z[0].z, z[0].w, z[1].x, z[1].y, z[1].z, z[1].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const uint32_t zz = __byte_perm(zw[2 * k], zw[2 * k + 1], 0x7632);
-                        z1024[k] = 0x64006400u | zz;
-                        z64[k] = 0xD400D400u | zz << 4;
+                        z1024[k] = h2_add(__byte_perm(zw[2 * k], zw[2 * k + 1], 0x7632), 0x64006400u);
+                        z64[k] = 0xD400D400u | (z1024[k] & kNib0) << 4;
                         sv[k] = __byte_perm(zw[2 * k], zw[2 * k + 1], 0x5410);
                         if ((sv[k] & 0x7C00u) == 0x7C00u) sv[k] &= 0xFFFF0000u;  // NaN: see above
                         if ((sv[k] & 0x7C000000u) == 0x7C000000u) sv[k] &= 0xFFFFu;
                     }
                     const uint32_t vst = v_u32 + st * S::kV;
 #pragma unroll 1
-                    for (int hw = 0; hw < D / 32; ++hw) {  // word, and nibbles 0-3 or 4-7 of it
-                        const bool second = hw >= 2;
-                        const uint32_t pick = (hw & 1) ? 0x7632 : 0x5410;
+                    for (int hw = 0; hw < D / 32; ++hw) {  // word of a pair
                         uint32_t x[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            if constexpr (D == 128)  // 16 bytes a pair: two words of each token
-                                x[k] = __byte_perm(second ? w[k].y : w[k].x, second ? w[k].w : w[k].z, pick);
-                            else  // 8 bytes a pair
-                                x[k] = __byte_perm((k & 1) ? w[k >> 1].z : w[k >> 1].x, (k & 1) ? w[k >> 1].w : w[k >> 1].y, pick);
+                            if constexpr (D == 128) {  // 16 bytes a pair
+                                x[k] = w[k].x;
+                                w[k].x = w[k].y;
+                                w[k].y = w[k].z;
+                                w[k].z = w[k].w;
+                            } else {  // 8 bytes a pair
+                                x[k] = (k & 1) ? w[k >> 1].z : w[k >> 1].x;
+                                if (k & 1) w[k >> 1].z = w[k >> 1].w;
+                                else w[k >> 1].x = w[k >> 1].y;
+                            }
                         }
                         const int ch = v_r * (D / 8) + hw * 4;
                         auto store = [&](int row, auto&& value) {
@@ -1599,7 +1728,7 @@ Plan make_plan(const KvView& v, int64_t heads, int sms) {
     // Few short units: one CTA of sixteen warps each and no join.
     const int64_t units = static_cast<int64_t>(v.seqs) * v.kv_heads;
     p.split = !(v.max_kv_len <= kWholeWarps * 2 * kTile && units <= sms && p.few <= 2);
-    p.grid = p.split ? sms * (p.few <= 2 ? 3 : 2) : static_cast<int>(units);
+    p.grid = p.split ? sms * (p.few == 1 ? 4 : (p.few == 2 ? 3 : 2)) : static_cast<int>(units);
     if (p.split) {
         p.o_bytes = static_cast<size_t>(p.grid) * 2 * p.few * 8 * v.head_dim * 4;
         p.ml_bytes = static_cast<size_t>(p.grid) * 2 * p.few * 8 * 8;
@@ -1631,7 +1760,9 @@ cudaError_t launch_few_w(const RowsArgs& r, int rows, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(attn_q4_few_kernel<D, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) e = launch_pdl(attn_q4_few_kernel<D, NT, W>, dim3(r.grid), W * 32, smem, s, r);
     if (e == cudaSuccess && r.split)
-        e = launch_pdl(attn_q4_join_kernel<D, NT, W>, dim3(r.a.v.seqs * r.a.v.kv_heads, rows), kThreads, 0, s, r);
+        // A CTA a (unit, row): large ones when they have the device to themselves.
+        e = launch_pdl(attn_q4_join_kernel<D>, dim3(r.a.v.seqs * r.a.v.kv_heads, rows),
+                       static_cast<int64_t>(r.a.v.seqs) * r.a.v.kv_heads * rows <= r.grid / 2 ? kJoinMax : 128, 0, s, r, NT * 8);
     return e;
 }
 
@@ -1710,6 +1841,7 @@ extern "C" int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int 
         r.group = static_cast<int>(heads / kv->kv_heads);
         r.split = plan.split;
         r.grid = plan.grid;
+        r.warps = kSplitWarps;
         r.part_o = static_cast<float*>(ws_dev);
         r.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws_dev) + plan.o_bytes);
         const int rows = r.group * std::max(a.v.max_q_len, 1);
