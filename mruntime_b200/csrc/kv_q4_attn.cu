@@ -73,7 +73,8 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // Split.  The 32-token tiles of all (sequence, kv head) units, in order, are
 // dealt to the CTAs in equal contiguous stretches, whatever the lengths: no
 // CTA waits for a long sequence, and no plan from the host is needed (lengths
-// are read here).  A CTA's warps take a stretch's tiles in turn, each with its
+// are read here).  (Each unit counts kUnitCost tiles more than it has, for the
+// time it takes to begin and to end one.)  A CTA's warps take a stretch's tiles in turn, each with its
 // own ring of bulk copies, and join at the end of the unit, the next unit's
 // first tiles already under way.  A unit that spans CTAs leaves its parts in
 // scratch (two places a CTA: a unit that began earlier, and one that goes on)
@@ -92,12 +93,16 @@ struct RowsArgs {
     int warps;          // of a CTA
 };
 
-// Tiles of sequence b (0: none of its rows is computed).
+// Tiles of sequence b (0: none of its rows is computed), and the places that
+// each of its units has among those that are dealt.
 __device__ __forceinline__ int seq_tiles(const KvView& v, int b) {
     int first, n, kv;
     if (!kv_seq(v, b, &first, &n, &kv) || n == 0) return 0;
     return max(1, (kv + kTile - 1) / kTile);
 }
+
+constexpr int kUnitCost = 4;
+__device__ __forceinline__ int unit_places(int tiles) { return tiles > 0 ? tiles + kUnitCost : 0; }
 
 __device__ __forceinline__ int tiles_a_cta(int total, int grid, int warps) {
     const int per = (total + grid - 1) / grid;
@@ -127,7 +132,7 @@ struct RowsShape {
 
 // A part of a (sequence, kv head) as a CTA works on it.
 struct RowsUnit {
-    int seq, head, tiles, at;  // `at`: number of its first tile among all tiles
+    int seq, head, tiles, at;  // `at`: number of its first tile among all places
     int t0, t1;                // tiles of this CTA
     int first, n, kv;
 };
@@ -166,7 +171,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
     __shared__ __align__(8) uint64_t s_full[W][S::kStages];
     __shared__ int s_sum[W];
     __shared__ int s_seq, s_at;
-    __shared__ float s_fac[S::kRows], s_sumq[S::kRows];
+    __shared__ float s_fac[S::kRows];
     __shared__ int s_limit[S::kRows];
     __shared__ float s_m[W][S::kRows], s_l[W][S::kRows];
     uint4* qf = reinterpret_cast<uint4*>(smem + S::kBytes - S::kQ);
@@ -189,9 +194,9 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
     int at, end, seq_at;  // seq_at: tile number at which the unit's sequence begins
     if constexpr (!S::kWhole) {
         int incl, t, base, chunk;
-        auto scan = [&](int b0) {  // tiles of W * 32 sequences from b0 on
+        auto scan = [&](int b0) {  // places of W * 32 sequences from b0 on
             const int b = b0 + threadIdx.x;
-            t = b < v.seqs ? seq_tiles(v, b) * v.kv_heads : 0;
+            t = b < v.seqs ? unit_places(seq_tiles(v, b)) * v.kv_heads : 0;
             incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -243,24 +248,32 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
         int f, n, kv;
         if (!kv_seq(v, u.seq, &f, &n, &kv) && threadIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
         if (u.tiles == 0) return;
-        seq_at = 0;
-        at = static_cast<int>(blockIdx.x % v.kv_heads) * u.tiles;
-        end = at + u.tiles;
+        at = seq_at = 0;
+        end = u.tiles;
     }
     const int range_begin = at;
 
-    // The unit that `at` lies in.
+    // The unit that place `at` lies in; false: none with a tile before `end`.
     auto find = [&]() {
-        while (at >= seq_at + u.tiles * v.kv_heads) {
-            seq_at += u.tiles * v.kv_heads;
-            ++u.seq;
-            u.tiles = seq_tiles(v, u.seq);
+        if (at >= end) return false;
+        if constexpr (S::kWhole) {
+            u.head = blockIdx.x % v.kv_heads;
+            u.at = 0;
+        } else {
+            int places;
+            while (at >= seq_at + (places = unit_places(u.tiles)) * v.kv_heads) {
+                seq_at += places * v.kv_heads;
+                ++u.seq;
+                u.tiles = seq_tiles(v, u.seq);
+            }
+            u.head = (at - seq_at) / places;
+            u.at = seq_at + u.head * places + kUnitCost;
         }
-        u.head = (at - seq_at) / u.tiles;
-        u.at = seq_at + u.head * u.tiles;
-        u.t0 = at - u.at;
-        u.t1 = min(u.tiles, u.t0 + (end - at));
+        u.t0 = max(at - u.at, 0);
+        u.t1 = min(u.tiles, end - u.at);
+        at = u.at + u.tiles;  // the next unit's first place
         kv_seq(v, u.seq, &u.first, &u.n, &u.kv);
+        return u.t0 < u.t1;
     };
 
     // This warp's tiles of the unit: t0 + warp, + W, ....  Lane l sees to block l of
@@ -319,7 +332,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
 #pragma unroll
         for (int i = 0; i < (S::kWhole ? S::kStages : S::kStages - 1); ++i) issue(i);
     };
-    find();
+    if (!find()) return;
     start();
     uint32_t phases = 0;  // of the ring's slots
     bool late = false;
@@ -340,43 +353,45 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
                 x[j] = widen(static_cast<uint16_t>(qw[k][j >> 1] >> (16 * (j & 1))), a.dtype);
                 big = fmaxf(big, fabsf(x[j]));
             }
+            const int top = static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(big)));  // >= 0: in the order of its bits
+            const int e = top < 0x7F800000 ? max((top >> 23) - 140, -100) : 0;
+            // A lane's channels lie in one half word of the operand: of codes times
+            // 2^-24, or (bits 4-7 of a half) 2^-20.
+            const int ch = lane * PER, word = (ch % (D / 4)) >> 3;
+            const float down = pow2(-e) * ((ch & 4) ? 0.0625f : 1.0f);
+            uint32_t* dst = reinterpret_cast<uint32_t*>(qf + ((row >> 3) * kWords + word) * 32 + (row & 7) * 4 + ch / (D / 4)) + ((ch & 7) >> 1);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-            const int e = big < INFINITY ? max((__float_as_int(big) >> 23) - 140, -100) : 0;
-            const float down = pow2(-e);
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int ch = lane * PER + j, word = (ch % (D / 4)) >> 3, jj = ch & 7;
-                const float y = x[j] * down;
-                const __half h = __float2half_rn((jj & 4) ? y * 0.0625f : y);
-                sum += __half2float(h) * ((jj & 4) ? 16.0f : 1.0f);
-                const int slot = ((row >> 3) * kWords + word) * 32 + (row & 7) * 4 + ch / (D / 4);
-                reinterpret_cast<__half*>(qf + slot)[jj] = h;
+            for (int j = 0; j < PER; j += 2) {
+                const __half2 h = __floats2half2_rn(x[j] * down, x[j + 1] * down);
+                dst[j >> 1] = *reinterpret_cast<const uint32_t*>(&h);
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
             if (lane == 0) {
                 s_fac[row] = a.scale * (1.4426950408889634f * 4096.0f) * pow2(12 + e);
-                s_sumq[row] = sum * 5.9604644775390625e-8f;
                 s_limit[row] = row >= rows ? 0 : (a.causal ? u.kv - u.n + row / args.group + 1 : u.kv);
             }
         }
         __syncthreads();
         if constexpr (!S::kWhole) issue(S::kStages - 1);  // its slot held the last unit's part
-        float fac[NT][2], sq[NT][2];
+        float fac[NT][2], sq[NT][2];  // sq: sum of q over the channels, as a code of one meets it
         int limit_min = 0x7FFFFFFF;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+            float ones[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+                const uint4 q = qf[(t * kWords + w) * 32 + lane];
+                mma_f16(ones, 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, q.x, q.y);
+                mma_f16(ones, 0x00100010u, 0x00100010u, 0x00100010u, 0x00100010u, q.z, q.w);
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int row = t * 8 + c * 2 + j;
                 fac[t][j] = s_fac[row];
-                sq[t][j] = s_sumq[row];
+                sq[t][j] = ones[j];
                 if (row < rows) limit_min = min(limit_min, s_limit[row]);
             }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
+        }
+        limit_min = __reduce_min_sync(0xFFFFFFFFu, limit_min);
         uint4 qr[NT == 1 ? NT : 1][kWords];
         if constexpr (NT == 1) {
 #pragma unroll
@@ -547,12 +562,8 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
 
         // Join the warps, with the next unit's copies under way.
         const RowsUnit done = u;
-        at += u.t1 - u.t0;
-        const bool more = !S::kWhole && at < end;
-        if (more) {
-            find();
-            start();
-        }
+        const bool more = !S::kWhole && find();
+        if (more) start();
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -608,26 +619,27 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
 }
 
 // Adds the parts of the units that span CTAs, in order.  One CTA per (unit,
-// row): the parts' weights, as many at a time as the CTA has threads, then
-// their sums, a warp (half a warp) a part.
-constexpr int kJoinMax = 512;
-
-template <int D>
-__global__ void __launch_bounds__(kJoinMax) attn_q4_join_kernel(const RowsArgs args, int kRows) {
+// row), a warp (half a warp) a part, kJoinParts of each asked for at a time.
+// Of THREADS threads: many parts of few rows, or few of many.
+template <int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) attn_q4_join_kernel(const RowsArgs args, int kRows) {
+    constexpr int kJoinParts = THREADS > 64 ? 10 : 4;
     constexpr int LANES = D / 4;  // of a part: four channels each
-    __shared__ int s_a[kJoinMax / 32], s_b[kJoinMax / 32];
-    __shared__ float s_w[kJoinMax];
-    __shared__ float s_big[kJoinMax / 32], s_sum[kJoinMax / 32];
-    __shared__ float4 s_o[kJoinMax];
+    static_assert(kJoinParts <= LANES, "a thread a part");
+    constexpr int threads = THREADS, warps = THREADS / 32;
+    __shared__ int s_a[warps], s_b[warps];
+    __shared__ float s_w[threads];
+    __shared__ float s_big[warps], s_sum[warps];
+    __shared__ float4 s_o[threads];
     const AttnQ4Args& a = args.a;
     const KvView& v = a.v;
-    const int threads = blockDim.x, warps = threads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int seq = blockIdx.x / v.kv_heads, head = blockIdx.x - seq * v.kv_heads, row = blockIdx.y;
     // The call's lengths are older than the kernel whose parts this one waits for
     // (that kernel lets this one start once it has waited for all before it).
     int all = 0, before = 0;
     for (int b = threadIdx.x; b < v.seqs; b += threads) {
-        const int t = seq_tiles(v, b);
+        const int t = unit_places(seq_tiles(v, b));
         all += t;
         if (b < seq) before += t;
     }
@@ -642,6 +654,7 @@ __global__ void __launch_bounds__(kJoinMax) attn_q4_join_kernel(const RowsArgs a
     }
     __syncthreads();
     all = before = 0;
+#pragma unroll 1
     for (int w = 0; w < warps; ++w) {
         all += s_a[w];
         before += s_b[w];
@@ -649,7 +662,7 @@ __global__ void __launch_bounds__(kJoinMax) attn_q4_join_kernel(const RowsArgs a
     const int tiles = seq_tiles(v, seq);
     int first, n, kv;
     const bool live = kv_seq(v, seq, &first, &n, &kv) && tiles != 0 && row < n * args.group;
-    const int unit_at = before * v.kv_heads + head * tiles;
+    const int unit_at = before * v.kv_heads + head * unit_places(tiles) + kUnitCost;
     const int per = tiles_a_cta(all * v.kv_heads, args.grid, args.warps);
     const int c0 = unit_at / per, c1 = (unit_at + tiles - 1) / per;
     griddep_wait();
@@ -659,8 +672,13 @@ __global__ void __launch_bounds__(kJoinMax) attn_q4_join_kernel(const RowsArgs a
     float m = kLowest, l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int ch = (threadIdx.x % LANES) * 4, mine = threadIdx.x / LANES, step = threads / LANES;
-    for (int p0 = c0; p0 <= c1; p0 += threads) {
-        const int parts = min(threads, c1 - p0 + 1);
+    for (int p0 = c0; p0 <= c1; p0 += kJoinParts * step) {
+        const int parts = min(kJoinParts * step, c1 - p0 + 1);
+        float4 x[kJoinParts];
+#pragma unroll
+        for (int k = 0; k < kJoinParts; ++k)
+            x[k] = mine + k * step < parts ? *reinterpret_cast<const float4*>(args.part_o + place(p0 + mine + k * step) * D + ch)
+                                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float2 ml = make_float2(kLowest, 0.0f);
         if (threadIdx.x < parts) ml = args.part_ml[place(p0 + threadIdx.x)];
         float big = ml.x;
@@ -669,6 +687,7 @@ __global__ void __launch_bounds__(kJoinMax) attn_q4_join_kernel(const RowsArgs a
         if (lane == 0) s_big[warp] = big;
         __syncthreads();
         big = m;
+#pragma unroll
         for (int w = 0; w < warps; ++w) big = fmaxf(big, s_big[w]);
         const float f = fast_exp2(ml.x - big), fix = fast_exp2(m - big);
         s_w[threadIdx.x] = f;
@@ -676,14 +695,14 @@ __global__ void __launch_bounds__(kJoinMax) attn_q4_join_kernel(const RowsArgs a
         acc = make_float4(acc.x * fix, acc.y * fix, acc.z * fix, acc.w * fix);
         m = big;
         __syncthreads();
-#pragma unroll 4
-        for (int p = mine; p < parts; p += step) {
-            const float g = s_w[p];
-            const float4 x = *reinterpret_cast<const float4*>(args.part_o + place(p0 + p) * D + ch);
-            acc.x = fmaf(x.x, g, acc.x);
-            acc.y = fmaf(x.y, g, acc.y);
-            acc.z = fmaf(x.z, g, acc.z);
-            acc.w = fmaf(x.w, g, acc.w);
+#pragma unroll
+        for (int k = 0; k < kJoinParts; ++k) {
+            if (mine + k * step >= parts) break;
+            const float g = s_w[mine + k * step];
+            acc.x = fmaf(x[k].x, g, acc.x);
+            acc.y = fmaf(x[k].y, g, acc.y);
+            acc.z = fmaf(x[k].z, g, acc.z);
+            acc.w = fmaf(x[k].w, g, acc.w);
         }
         __syncthreads();
     }
@@ -1753,16 +1772,28 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem, c
     return e;
 }
 
+// (It runs beside the last CTAs before it and the first ones after it, so it wants
+// the same share of a multiprocessor's memory: a kernel of another share holds
+// CTAs of the next one off it.)
+template <int D, int THREADS>
+cudaError_t launch_join(const RowsArgs& r, int rows, int few, cudaStream_t s) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_q4_join_kernel<D, THREADS>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                               cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(attn_q4_join_kernel<D, THREADS>, dim3(r.a.v.seqs * r.a.v.kv_heads, rows), THREADS, 0, s, r, few * 8);
+}
+
 template <int D, int NT, int W>
 cudaError_t launch_few_w(const RowsArgs& r, int rows, cudaStream_t s) {
     constexpr int smem = RowsShape<D, NT, W>::kBytes;
     // Set at every call: it costs little and holds for whichever device is current.
     cudaError_t e = cudaFuncSetAttribute(attn_q4_few_kernel<D, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attn_q4_few_kernel<D, NT, W>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e == cudaSuccess) e = launch_pdl(attn_q4_few_kernel<D, NT, W>, dim3(r.grid), W * 32, smem, s, r);
     if (e == cudaSuccess && r.split)
-        // A CTA a (unit, row): large ones when they have the device to themselves.
-        e = launch_pdl(attn_q4_join_kernel<D>, dim3(r.a.v.seqs * r.a.v.kv_heads, rows),
-                       static_cast<int64_t>(r.a.v.seqs) * r.a.v.kv_heads * rows <= r.grid / 2 ? kJoinMax : 128, 0, s, r, NT * 8);
+        e = static_cast<int64_t>(r.a.v.seqs) * r.a.v.kv_heads * rows <= r.grid ? launch_join<D, 512>(r, rows, NT, s)
+                                                                             : launch_join<D, 64>(r, rows, NT, s);
     return e;
 }
 
