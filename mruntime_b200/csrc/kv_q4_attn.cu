@@ -73,7 +73,7 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // Split.  The 32-token tiles of all (sequence, kv head) units, in order, are
 // dealt to the CTAs in equal contiguous stretches, whatever the lengths: no
 // CTA waits for a long sequence, and no plan from the host is needed (lengths
-// are read here).  (Each unit counts kUnitCost tiles more than it has, for the
+// are read here).  (Each unit counts unit_cost() tiles more than it has, for the
 // time it takes to begin and to end one.)  A CTA's warps take a stretch's tiles in turn, each with its
 // own ring of bulk copies, and join at the end of the unit, the next unit's
 // first tiles already under way.  A unit that spans CTAs leaves its parts in
@@ -86,6 +86,8 @@ constexpr float kLowest = -3.402823466e38f;  // m before any key: 2^(m - anythin
 struct RowsArgs {
     AttnQ4Args a;
     int group;          // query heads of a kv head
+    uint32_t group_magic;  // row * it >> 16 = row / group for row < 32
+    int vec;            // q's rows can be read 16 bytes at a time
     int split;          // 0: every unit is one CTA's
     float* part_o;      // [2 * grid][8 NT][D]
     float2* part_ml;    // [2 * grid][8 NT]
@@ -101,8 +103,8 @@ __device__ __forceinline__ int seq_tiles(const KvView& v, int b) {
     return max(1, (kv + kTile - 1) / kTile);
 }
 
-constexpr int kUnitCost = 4;
-__device__ __forceinline__ int unit_places(int tiles) { return tiles > 0 ? tiles + kUnitCost : 0; }
+__host__ __device__ constexpr int unit_cost(int rows) { return rows <= 16 ? 8 : 16; }
+__device__ __forceinline__ int unit_places(int tiles, int cost) { return tiles > 0 ? tiles + cost : 0; }
 
 __device__ __forceinline__ int tiles_a_cta(int total, int grid, int warps) {
     const int per = (total + grid - 1) / grid;
@@ -153,6 +155,15 @@ __device__ __forceinline__ void wait_tile(uint64_t* bar, uint32_t parity, int* f
     }
 }
 
+// Eight 16-bit values at any alignment of two bytes.
+__device__ __forceinline__ uint4 load8(const uint16_t* p, bool vec) {
+    if (vec) return *reinterpret_cast<const uint4*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = p[2 * j] | static_cast<uint32_t>(p[2 * j + 1]) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // max that keeps a NaN.
 __device__ __forceinline__ float max_nan(float x, float y) {
     float r;
@@ -166,7 +177,9 @@ template <int D, int NT, int W>
 __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 3 : 2))) attn_q4_few_kernel(const RowsArgs args) {
     using S = RowsShape<D, NT, W>;
     constexpr int kWords = D / 32;               // words of a lane: K row part, and V channel stretch of two tokens
-    constexpr int kMine = (S::kRows + W - 1) / W;  // rows whose q a warp lays out
+    // q is laid out eight channels a lane: lanes of a row, rows of a pass, passes.
+    constexpr int kRowLanes = D / 8, kPass = W * 32 / kRowLanes, kPasses = (S::kRows + kPass - 1) / kPass;
+    constexpr int kCost = unit_cost(S::kRows);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_full[W][S::kStages];
     __shared__ int s_sum[W];
@@ -196,7 +209,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
         int incl, t, base, chunk;
         auto scan = [&](int b0) {  // places of W * 32 sequences from b0 on
             const int b = b0 + threadIdx.x;
-            t = b < v.seqs ? unit_places(seq_tiles(v, b)) * v.kv_heads : 0;
+            t = b < v.seqs ? unit_places(seq_tiles(v, b), kCost) * v.kv_heads : 0;
             incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -261,13 +274,13 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
             u.at = 0;
         } else {
             int places;
-            while (at >= seq_at + (places = unit_places(u.tiles)) * v.kv_heads) {
+            while (at >= seq_at + (places = unit_places(u.tiles, kCost)) * v.kv_heads) {
                 seq_at += places * v.kv_heads;
                 ++u.seq;
                 u.tiles = seq_tiles(v, u.seq);
             }
             u.head = (at - seq_at) / places;
-            u.at = seq_at + u.head * places + kUnitCost;
+            u.at = seq_at + u.head * places + kCost;
         }
         u.t0 = max(at - u.at, 0);
         u.t1 = min(u.tiles, end - u.at);
@@ -290,7 +303,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
             page_next = slot < v.ld_table ? row_table[slot] : -1;
         }
     };
-    auto issue = [&](int i) {
+    auto issue = [&](int i, int slot) {
         if (i >= count) return;
         if ((i & 15) == 0) {
             const int pos = block_pos(i);
@@ -303,34 +316,31 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
             ask(i + 16);
         }
         if ((lane >> 1) == (i & 15)) {
-            uint64_t* bar = &s_full[warp][i % S::kStages];
+            uint64_t* bar = &s_full[warp][slot];
             if (blk != nullptr) {
                 mbar_arrive_expect_tx(bar, S::kBlock);
-                bulk_load(ring + (i % S::kStages) * S::kStage + (lane & 1) * S::kBlock, blk, S::kBlock, bar);
+                bulk_load(ring + slot * S::kStage + (lane & 1) * S::kBlock, blk, S::kBlock, bar);
             } else {
                 mbar_arrive(bar);
             }
         }
     };
-    // q of this warp's rows of the unit, D / 32 neighbouring channels a lane.
-    uint32_t qw[kMine][D / 64];
+    // q of the rows that this thread lays out.
+    uint4 qw[kPasses];
+    const int q_row = threadIdx.x / kRowLanes, q_lane = threadIdx.x & (kRowLanes - 1);
     auto start = [&]() {
         row_table = v.table + static_cast<int64_t>(u.seq) * v.ld_table;
         count = u.t1 - u.t0 > warp ? (u.t1 - u.t0 - warp + W - 1) / W : 0;
         ask(0);
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-            const int row = warp + k * W, i = row / args.group, g = row - i * args.group;
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j) qw[k][j] = 0;
-            if (row < u.n * args.group) {
-                const uint16_t* src = a.q + (u.first + i) * a.ldq + (u.head * args.group + g) * D + lane * (D / 32);
-#pragma unroll
-                for (int j = 0; j < D / 64; ++j) qw[k][j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
-            }
+        for (int k = 0; k < kPasses; ++k) {
+            const int row = q_row + k * kPass, i = row * args.group_magic >> 16, g = row - i * args.group;
+            qw[k] = make_uint4(0, 0, 0, 0);
+            if (row < u.n * args.group)
+                qw[k] = load8(a.q + (u.first + i) * a.ldq + (u.head * args.group + g) * D + q_lane * 8, args.vec);
         }
 #pragma unroll
-        for (int i = 0; i < (S::kWhole ? S::kStages : S::kStages - 1); ++i) issue(i);
+        for (int i = 0; i < (S::kWhole ? S::kStages : S::kStages - 1); ++i) issue(i, i);
     };
     if (!find()) return;
     start();
@@ -343,35 +353,36 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
         // it), in the order of the MMA's B fragments.
         const int rows = u.n * args.group;  // <= 8 NT
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-            const int row = warp + k * W;
-            if (S::kRows % W != 0 && row >= S::kRows) break;
-            constexpr int PER = D / 32;
-            float x[PER], big = 0.0f;
+        for (int k = 0; k < kPasses; ++k) {
+            const int row = q_row + k * kPass;
+            const uint32_t w[4] = {qw[k].x, qw[k].y, qw[k].z, qw[k].w};
+            float x[8], big = 0.0f;
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                x[j] = widen(static_cast<uint16_t>(qw[k][j >> 1] >> (16 * (j & 1))), a.dtype);
+            for (int j = 0; j < 8; ++j) {
+                x[j] = widen(static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1))), a.dtype);
                 big = fmaxf(big, fabsf(x[j]));
             }
-            const int top = static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(big)));  // >= 0: in the order of its bits
-            const int e = top < 0x7F800000 ? max((top >> 23) - 140, -100) : 0;
-            // A lane's channels lie in one half word of the operand: of codes times
-            // 2^-24, or (bits 4-7 of a half) 2^-20.
-            const int ch = lane * PER, word = (ch % (D / 4)) >> 3;
-            const float down = pow2(-e) * ((ch & 4) ? 0.0625f : 1.0f);
-            uint32_t* dst = reinterpret_cast<uint32_t*>(qf + ((row >> 3) * kWords + word) * 32 + (row & 7) * 4 + ch / (D / 4)) + ((ch & 7) >> 1);
 #pragma unroll
-            for (int j = 0; j < PER; j += 2) {
-                const __half2 h = __floats2half2_rn(x[j] * down, x[j + 1] * down);
-                dst[j >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int o = kRowLanes / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+            const int e = big < INFINITY ? max((__float_as_int(big) >> 23) - 140, -100) : 0;
+            // Channels 0-3 of a word meet codes times 2^-24, 4-7 codes times 2^-20.
+            const float down = pow2(-e), down16 = down * 0.0625f;
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float f = j < 2 ? down : down16;
+                const __half2 h = __floats2half2_rn(x[2 * j] * f, x[2 * j + 1] * f);
+                y[j] = *reinterpret_cast<const uint32_t*>(&h);
             }
-            if (lane == 0) {
+            if (S::kRows % kPass != 0 && row >= S::kRows) break;
+            qf[((row >> 3) * kWords + q_lane % kWords) * 32 + (row & 7) * 4 + q_lane / kWords] = make_uint4(y[0], y[1], y[2], y[3]);
+            if (q_lane == 0) {
                 s_fac[row] = a.scale * (1.4426950408889634f * 4096.0f) * pow2(12 + e);
-                s_limit[row] = row >= rows ? 0 : (a.causal ? u.kv - u.n + row / args.group + 1 : u.kv);
+                s_limit[row] = row >= rows ? 0 : (a.causal ? u.kv - u.n + static_cast<int>(row * args.group_magic >> 16) + 1 : u.kv);
             }
         }
         __syncthreads();
-        if constexpr (!S::kWhole) issue(S::kStages - 1);  // its slot held the last unit's part
+        if constexpr (!S::kWhole) issue(S::kStages - 1, S::kStages - 1);  // its slot held the last unit's part
         float fac[NT][2], sq[NT][2];  // sq: sum of q over the channels, as a code of one meets it
         int limit_min = 0x7FFFFFFF;
 #pragma unroll
@@ -415,8 +426,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
         }
 
 #pragma unroll 1
-        for (int i = 0; i < count; ++i) {
-            const int slot = i % S::kStages;
+        for (int i = 0, slot = 0; i < count; ++i) {
             wait_tile(&s_full[warp][slot], (phases >> slot) & 1, v.err_flag, late);
             phases ^= 1u << slot;
             const uint8_t* stage = ring + slot * S::kStage;
@@ -557,7 +567,8 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
                 }
             }
             __syncwarp();  // the slot is read
-            issue(i + S::kStages);
+            issue(i + S::kStages, slot);
+            slot = slot == S::kStages - 1 ? 0 : slot + 1;
         }
 
         // Join the warps, with the next unit's copies under way.
@@ -605,7 +616,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
             }
             if (whole) {
                 const float inv = sum == 0.0f ? 0.0f : fast_rcp(sum);
-                const int qi = row / args.group, g = row - qi * args.group;
+                const int qi = row * args.group_magic >> 16, g = row - qi * args.group;
                 uint16_t* dst = a.out + (done.first + qi) * a.ldo + (done.head * args.group + g) * D + ch;
                 store2(dst, narrow2(acc.x * inv, acc.y * inv, a.dtype));
                 store2(dst + 2, narrow2(acc.z * inv, acc.w * inv, a.dtype));
@@ -623,6 +634,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
 // Of THREADS threads: many parts of few rows, or few of many.
 template <int D, int THREADS>
 __global__ void __launch_bounds__(THREADS) attn_q4_join_kernel(const RowsArgs args, int kRows) {
+    const int kCost = unit_cost(kRows);
     constexpr int kJoinParts = THREADS > 64 ? 10 : 4;
     constexpr int LANES = D / 4;  // of a part: four channels each
     static_assert(kJoinParts <= LANES, "a thread a part");
@@ -639,7 +651,7 @@ __global__ void __launch_bounds__(THREADS) attn_q4_join_kernel(const RowsArgs ar
     // (that kernel lets this one start once it has waited for all before it).
     int all = 0, before = 0;
     for (int b = threadIdx.x; b < v.seqs; b += threads) {
-        const int t = unit_places(seq_tiles(v, b));
+        const int t = unit_places(seq_tiles(v, b), kCost);
         all += t;
         if (b < seq) before += t;
     }
@@ -662,7 +674,7 @@ __global__ void __launch_bounds__(THREADS) attn_q4_join_kernel(const RowsArgs ar
     const int tiles = seq_tiles(v, seq);
     int first, n, kv;
     const bool live = kv_seq(v, seq, &first, &n, &kv) && tiles != 0 && row < n * args.group;
-    const int unit_at = before * v.kv_heads + head * unit_places(tiles) + kUnitCost;
+    const int unit_at = before * v.kv_heads + head * unit_places(tiles, kCost) + kCost;
     const int per = tiles_a_cta(all * v.kv_heads, args.grid, args.warps);
     const int c0 = unit_at / per, c1 = (unit_at + tiles - 1) / per;
     griddep_wait();
@@ -719,7 +731,7 @@ __global__ void __launch_bounds__(THREADS) attn_q4_join_kernel(const RowsArgs ar
             acc = make_float4(acc.x + x.x, acc.y + x.y, acc.z + x.z, acc.w + x.w);
         }
         const float inv = sum == 0.0f ? 0.0f : fast_rcp(sum);
-        const int qi = row / args.group, g = row - qi * args.group;
+        const int qi = row * args.group_magic >> 16, g = row - qi * args.group;
         uint16_t* dst = a.out + (first + qi) * a.ldo + (head * args.group + g) * D + ch;
         store2(dst, narrow2(acc.x * inv, acc.y * inv, a.dtype));
         store2(dst + 2, narrow2(acc.z * inv, acc.w * inv, a.dtype));
@@ -1870,6 +1882,8 @@ extern "C" int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int 
         RowsArgs r{};
         r.a = a;
         r.group = static_cast<int>(heads / kv->kv_heads);
+        r.group_magic = (65536 + r.group - 1) / r.group;
+        r.vec = (reinterpret_cast<uintptr_t>(q_dev) & 15) == 0 && (ldq & 7) == 0;
         r.split = plan.split;
         r.grid = plan.grid;
         r.warps = kSplitWarps;
