@@ -123,7 +123,8 @@ struct RowsShape {
     // behind the rings; of a lone unit, all in its ring.
     static constexpr int kOthers = kWhole ? 0 : W * (kRows - 8) * D * 4;
     static constexpr int kQ = NT * (D / 32) * 32 * 16;
-    static constexpr int kBytes = kRing + kOthers + kQ;
+    static constexpr int kScales = W * kTile * 16;  // of a tile's tokens, a warp's own
+    static constexpr int kBytes = kRing + kOthers + kScales + kQ;
     static_assert((kWhole ? kRows : 8) * D * 4 <= (kWhole ? kStages : 1) * kStage, "parts fit");
     static __device__ __forceinline__ float* part(uint8_t* smem, int w, int row) {
         if (kWhole) return reinterpret_cast<float*>(smem + w * kStages * kStage) + row * D;
@@ -164,6 +165,13 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, bool vec) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// True on one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+
 // max that keeps a NaN.
 __device__ __forceinline__ float max_nan(float x, float y) {
     float r;
@@ -192,10 +200,11 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
     const KvView& v = a.v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     uint8_t* ring = smem + warp * S::kStages * S::kStage;
+    float4* scales = reinterpret_cast<float4*>(smem + S::kRing + S::kOthers) + warp * kTile;
 
     if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < S::kStages; ++i) mbar_init(&s_full[warp][i], kTileBlocks);
+        for (int i = 0; i < S::kStages; ++i) mbar_init(&s_full[warp][i], 1);
         fence_barrier_init();
     }
     __syncwarp();
@@ -290,9 +299,8 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
     };
 
     // This warp's tiles of the unit: t0 + warp, + W, ....  Lane l sees to block l of
-    // sixteen of them: its page's number (asked for sixteen tiles early) and address.
-    int count, page_next;
-    const uint8_t* blk = nullptr;
+    // sixteen of them: its page's number (asked for sixteen tiles early), its own.
+    int count, page_next, blk = -2;
     const int32_t* row_table;
     auto block_pos = [&](int i) { return (u.t0 + warp + (i + (lane >> 1)) * W) * kTile + (lane & 1) * kKvBlock; };
     auto ask = [&](int i) {  // -2: no such block
@@ -307,23 +315,27 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
         if (i >= count) return;
         if ((i & 15) == 0) {
             const int pos = block_pos(i);
-            blk = nullptr;
+            blk = -2;
             if (page_next != -2) {
-                const int n = kv_block_in(v, page_next, kv_slot(v, pos), u.head, pos);
-                if (n < 0) raise_error(v.err_flag, kErrBadPage);
-                else blk = v.data + static_cast<int64_t>(n) * S::kBlock;
+                blk = kv_block_in(v, page_next, kv_slot(v, pos), u.head, pos);
+                if (blk < 0) {
+                    raise_error(v.err_flag, kErrBadPage);
+                    blk = -2;
+                }
             }
             ask(i + 16);
         }
-        if ((lane >> 1) == (i & 15)) {
+        // A tile's two blocks are neighbours where a page holds both.
+        const int n0 = __shfl_sync(0xFFFFFFFFu, blk, (i & 15) * 2), n1 = __shfl_sync(0xFFFFFFFFu, blk, (i & 15) * 2 + 1);
+        if (elect_one()) {
             uint64_t* bar = &s_full[warp][slot];
-            if (blk != nullptr) {
-                mbar_arrive_expect_tx(bar, S::kBlock);
-                bulk_load(ring + slot * S::kStage + (lane & 1) * S::kBlock, blk, S::kBlock, bar);
-            } else {
-                mbar_arrive(bar);
-            }
+            uint8_t* dst = ring + slot * S::kStage;
+            mbar_arrive_expect_tx(bar, (n0 >= 0 ? S::kBlock : 0) + (n1 >= 0 ? S::kBlock : 0));
+            const bool both = n1 == n0 + 1;
+            if (n0 >= 0) bulk_load(dst, v.data + static_cast<int64_t>(n0) * S::kBlock, both ? S::kStage : S::kBlock, bar);
+            if (n1 >= 0 && !both) bulk_load(dst + S::kBlock, v.data + static_cast<int64_t>(n1) * S::kBlock, S::kBlock, bar);
         }
+        __syncwarp();
     };
     // q of the rows that this thread lays out.
     uint4 qw[kPasses];
@@ -432,6 +444,16 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
             const uint8_t* stage = ring + slot * S::kStage;
             const int pos0 = (u.t0 + warp + i * W) * kTile;
 
+            {  // a token a lane: its scales as the sums need them
+                const uint8_t* b = stage + (lane >> 4) * S::kBlock + (lane & 15) * 4;
+                const uint32_t ks = *reinterpret_cast<const uint32_t*>(b + kv_k_scales(D));
+                const float sk = f16_bits_to_f32(static_cast<uint16_t>(ks)), zk = f16_bits_to_f32(static_cast<uint16_t>(ks >> 16));
+                // (never stored: scale 0; it holds zeros whatever its scale)
+                const float sv = max_nan(f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(b + kv_v_scales(D))), 5.9604644775390625e-8f);
+                // A row that sees a NaN scale has a NaN p; the others' sums must not.
+                scales[lane] = make_float4(sk, -zk, fast_log2(sv), fminf(fast_rcp(sv), 16777216.0f));
+                __syncwarp();
+            }
             float y[kTileBlocks][NT][4];
             float rs[kTileBlocks][2];
             uint32_t z[kTileBlocks][2];  // zero points of V: tokens 2c, 2c + 1 and 2c + 8, 2c + 9
@@ -464,20 +486,14 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int token = half * 8 + r;
-                    const uint32_t ks = reinterpret_cast<const uint32_t*>(b + kv_k_scales(D))[token];
-                    const uint16_t vs = *reinterpret_cast<const uint16_t*>(b + kv_v_scales(D) + token * 4);
-                    const float sk = f16_bits_to_f32(static_cast<uint16_t>(ks)), zk = f16_bits_to_f32(static_cast<uint16_t>(ks >> 16));
-                    // (never stored: scale 0; it holds zeros whatever its scale)
-                    const float sv = max_nan(f16_bits_to_f32(vs), 5.9604644775390625e-8f), lv = fast_log2(sv);
-                    // A row that sees a NaN scale has a NaN p; the others' sums must not.
-                    rs[h][half] = fminf(fast_rcp(sv), 16777216.0f);
+                    const float4 sc = scales[h * kKvBlock + half * 8 + r];
+                    rs[h][half] = sc.w;
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             float& e = y[h][t][half * 2 + j];
-                            e = fmaf(fmaf(-zk, sq[t][j], e) * sk, fac[t][j], lv);
+                            e = fmaf(fmaf(sc.y, sq[t][j], e) * sc.x, fac[t][j], sc.z);
                         }
                     const uint2 zw = *reinterpret_cast<const uint2*>(b + kv_v_scales(D) + half * 32 + c * 8);
                     z[h][half] = __byte_perm(zw.x, zw.y, 0x7632);
