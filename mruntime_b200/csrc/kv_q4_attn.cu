@@ -756,20 +756,6 @@ __global__ void __launch_bounds__(THREADS) attn_q4_join_kernel(const RowsArgs ar
 
 // ------------------------------------------------------------------ many rows
 
-// Sum over the block of one number a thread (every thread gets it).
-template <int W>
-__device__ __forceinline__ int block_sum(int x, int* s) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
-    __syncthreads();
-    int t = 0;
-#pragma unroll 1
-    for (int w = 0; w < W; ++w) t += s[w];
-    return t;
-}
-
 // TMEM accesses in MMA-fragment order, 16 lanes (rows) at a time: lane (r, c)
 // of the warp gets, of every eight 32-bit columns, columns 2c and 2c + 1 of
 // rows r and r + 8.  (A thread then meets a quarter of the columns instead of
@@ -926,11 +912,13 @@ __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volat
 // for its instructions.
 //
 // Units' key tiles are dealt to the CTAs in equal contiguous stretches, as in
-// the few-rows kernel, parts of units that span CTAs joined from scratch.
+// the few-rows kernel (each unit at kManyCost tiles more than it has), parts of
+// units that span CTAs joined from scratch.
 constexpr int kManyRows = 256, kManyKeys = 64;
 constexpr int kSoftmaxWarps = 16, kCodesWarps = 8, kManyWarps = kSoftmaxWarps + kCodesWarps + 8;
 constexpr int kManyThreads = kManyWarps * 32;
 constexpr int kLoaders = 96;  // threads that bring Q
+constexpr int kManyCost = 4;  // of a unit's begin and end, in key tiles
 
 struct ManyPart {  // a unit that begins in a CTA's stretch and goes on
     int seq, head, row0;
@@ -941,6 +929,7 @@ struct ManyPart {  // a unit that begins in a CTA's stretch and goes on
 struct ManyArgs {
     AttnQ4Args a;
     int group, grid;
+    uint32_t group_magic;  // high word of x * it = x / group for x < 2^16 (group 1: 0)
     float* part_o;     // [2 * grid][256][D]
     float2* part_ml;   // [2 * grid][256]
     ManyPart* parts;   // [grid]
@@ -982,12 +971,12 @@ __device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a
     return sum;
 }
 
-// Key tiles of row tiles 0 .. x - 1.
+// Places of row tiles 0 .. x - 1: their key tiles, and what the units cost.
 __device__ __forceinline__ int many_before(const ManySeq& s, int x) {
     if (x == 0) return 0;
-    if (!s.causal) return x * s.tiles(0);
+    if (!s.causal) return x * (s.tiles(0) + kManyCost);
     const int y = min(x, s.count - 1);
-    int t = y + static_cast<int>(floor_sum(y, kManyKeys * s.group, kManyRows, kManyRows - 1 + s.past() * s.group));
+    int t = y + x * kManyCost + static_cast<int>(floor_sum(y, kManyKeys * s.group, kManyRows, kManyRows - 1 + s.past() * s.group));
     if (x == s.count) t += s.tiles(s.count - 1);
     return t;
 }
@@ -1064,6 +1053,7 @@ __device__ __forceinline__ uint32_t nib1_f16(uint32_t w, uint32_t z64) {
 struct ManyUnit {
     int seq, head, first, n, kv;  // sequence and kv head, the sequence's first row, new and held tokens
     int row0, rows;               // of the unit's rows
+    int tok0, head0;              // row0's token and query head of the group
     int t0, count;                // its key tiles that are this CTA's; count = 0: no more units
     int whole, place;             // all of them are; where its part goes else
     __device__ __forceinline__ int row_tiles() const { return rows > 128 ? 2 : 1; }
@@ -1072,8 +1062,8 @@ constexpr int kUnits = 4;  // published ahead
 
 // A CTA's stretch of the key tiles, unit by unit.
 struct ManyWalk {
-    int at, end, begin;  // tile numbers: next, end and begin of the stretch
-    int unit_at, tiles;  // where the unit begins, its key tiles
+    int at, end, begin;  // places: next, end and begin of the stretch
+    int unit_at, tiles;  // where the unit begins, its key tiles (kManyCost places on)
     ManySeq sq;
     int seq, head, x;    // the unit: sequence, kv head, row tile
 
@@ -1081,8 +1071,8 @@ struct ManyWalk {
         u->count = 0;
         if (at >= end) return false;
         tiles = sq.tiles(x);
-        if (at >= unit_at + tiles) {
-            unit_at += tiles;
+        if (at >= unit_at + tiles + kManyCost) {
+            unit_at += tiles + kManyCost;
             if (++x == sq.count) {
                 x = 0;
                 if (++head == g.a.v.kv_heads) {
@@ -1100,12 +1090,16 @@ struct ManyWalk {
         u->kv = sq.kv;
         u->row0 = x * kManyRows;
         u->rows = min(kManyRows, sq.n * g.group - u->row0);
-        u->t0 = at - unit_at;
-        u->count = min(unit_at + tiles, end) - at;
+        const int first_at = unit_at + kManyCost;
+        u->t0 = max(at - first_at, 0);
+        u->count = max(min(tiles, end - first_at) - u->t0, 0);
         u->whole = u->count == tiles;
-        u->place = unit_at > begin ? 1 : 0;
-        at += u->count;
-        return true;
+        u->place = first_at > begin ? 1 : 0;
+        const int x = u->row0 / g.group;
+        u->tok0 = x;
+        u->head0 = u->row0 - x * g.group;
+        at = first_at + tiles;
+        return u->count > 0;
     }
 };
 
@@ -1122,6 +1116,7 @@ __device__ __forceinline__ void registers_down() {
 // Registers a thread: at launch, and as the roles share them out (in groups of
 // four warps: four of softmax, two of codes, products, Q).
 constexpr int kManyRegs = 64, kSoftmaxRegs = 72, kCodesRegs = 72, kOtherRegs = 40;
+static_assert(kManyWarps == 32, "a lane a warp in the scan");
 static_assert(4 * kSoftmaxRegs + 2 * kCodesRegs + 2 * kOtherRegs == 8 * kManyRegs, "the roles share what the launch has");
 
 template <int D, bool BF16>
@@ -1178,58 +1173,61 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     griddep_wait();
 
     // This CTA's stretch, and the unit it begins in.
-    int mine = 0, first_tiles = 0;  // of the thread's sequences, of its first
-    for (int b = threadIdx.x; b < v.seqs; b += kManyThreads) {
-        ManySeq q;
-        if (!many_seq(args, b, &q) && blockIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
-        const int t = many_before(q, q.count);
-        mine += t;
-        if (b == threadIdx.x) first_tiles = t;
+    int t, lo, chunk;  // places of the thread's sequence; of those before it and of all in a scan
+    auto scan = [&](int b0) {
+        const int b = b0 + threadIdx.x;
+        t = 0;
+        if (b < v.seqs) {
+            ManySeq q;
+            if (!many_seq(args, b, &q) && blockIdx.x == 0) raise_error(v.err_flag, kErrBadPage);
+            t = many_before(q, q.count) * v.kv_heads;
+        }
+        int incl = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        int warps = s_sum[lane];  // (as many warps as lanes)
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xFFFFFFFFu, warps, o);
+            if (lane >= o) warps += up;
+        }
+        chunk = __shfl_sync(0xFFFFFFFFu, warps, 31);
+        const int before = __shfl_sync(0xFFFFFFFFu, warps, (warp + 31) & 31);
+        lo = (warp > 0 ? before : 0) + incl - t;
+    };
+    int total = 0;
+#pragma unroll 1
+    for (int b0 = (v.seqs - 1) / kManyThreads * kManyThreads; b0 >= 0; b0 -= kManyThreads) {  // the first ones last
+        scan(b0);
+        total += chunk;
     }
-    const int total = block_sum<kManyWarps>(mine, s_sum) * v.kv_heads;
     const int per = (total + args.grid - 1) / args.grid;
     ManyWalk walk;
     walk.at = walk.begin = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(blockIdx.x) * per));
     walk.end = walk.at + min(total - walk.at, per);
-    walk.seq = -1;
     walk.head = walk.x = walk.unit_at = 0;
     if (walk.at < walk.end) {
-        int before = 0;
 #pragma unroll 1
-        for (int b0 = 0; walk.seq < 0; b0 += kManyThreads) {  // ends: walk.at < total
-            const int b = b0 + threadIdx.x;
-            int t = first_tiles;
-            if (b0 > 0 && b < v.seqs) {
-                ManySeq q;
-                many_seq(args, b, &q);
-                t = many_before(q, q.count);
-            }
-            t = b < v.seqs ? t * v.kv_heads : 0;
-            int incl = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            __syncthreads();
-            if (threadIdx.x == 0) s_seq = -1;
-            if (lane == 31) s_sum[warp] = incl;
-            __syncthreads();
-            int base = before;
-#pragma unroll 1
-            for (int w = 0; w < kManyWarps; ++w) {
-                if (w == warp) base = before;
-                before += s_sum[w];
-            }
-            if (walk.at >= base + incl - t && walk.at < base + incl) {
-                s_seq = b;
-                s_at = base + incl - t;
+        for (int b0 = 0, before = 0;;) {  // ends: walk.at < total
+            if (walk.at >= before + lo && walk.at < before + lo + t) {
+                s_seq = b0 + threadIdx.x;
+                s_at = before + lo;
                 s_tiles = t / v.kv_heads;
             }
-            __syncthreads();
-            walk.seq = s_seq;
-            walk.unit_at = s_at;
+            before += chunk;
+            if (walk.at < before) break;
+            b0 += kManyThreads;
+            scan(b0);
         }
+        __syncthreads();
+        walk.seq = s_seq;
+        walk.unit_at = s_at;
         many_seq(args, walk.seq, &walk.sq);
         const int a_head = s_tiles;
         walk.head = (walk.at - walk.unit_at) / a_head;
@@ -1639,22 +1637,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
             if (u.count == 0) break;
             if (n > 0) wait_phase(&s_q_free, (n - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+            const uint16_t* q0 = a.q + (u.first + u.tok0) * a.ldq + u.head * args.group * D + ch * 8;
 #pragma unroll 2
             for (int row = tid / (D / 8); row < u.row_tiles() * 128; row += kLoaders / (D / 8)) {
                 const uint32_t dst = panel_at(q_u32 + ((row >> 7) * kPanels + (ch >> 3)) * S::kPanel, row & 127, ch & 7);
                 const bool live = row < u.rows;
-                const int tok = live ? (u.row0 + row) / args.group : 0, gh = live ? u.row0 + row - tok * args.group : 0;
-                const uint16_t* src = a.q + (u.first + tok) * a.ldq + (u.head * args.group + gh) * D + ch * 8;
+                const int x = live ? u.head0 + row : 0, dt = args.group_magic != 0 ? __umulhi(x, args.group_magic) : x;
+                const uint16_t* src = q0 + dt * a.ldq + (x - dt * args.group) * D;
                 if (vec) {
                     copy_async_16(dst, src, live);
                 } else {
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (live) {
-                        w.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
-                        w.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
-                        w.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
-                        w.w = src[6] | static_cast<uint32_t>(src[7]) << 16;
-                    }
+                    const uint4 w = live ? load8(src, false) : make_uint4(0, 0, 0, 0);
                     st_shared_16(dst, w.x, w.y, w.z, w.w);
                 }
             }
@@ -1677,7 +1670,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 ManyUnit& u = s_unit[n % kUnits];
                 more = walk.next(args, &u);
                 if (more && u.t0 == 0 && !u.whole)
-                    part = ManyPart{u.seq, u.head, u.row0, u.place, (walk.unit_at + walk.tiles - 1) / per};
+                    part = ManyPart{u.seq, u.head, u.row0, u.place, (walk.unit_at + kManyCost + walk.tiles - 1) / per};
                 mbar_arrive(&s_unit_full[n % kUnits]);
             }
             args.parts[blockIdx.x] = part;
@@ -1690,11 +1683,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     if (warp == kSoftmaxWarps + kCodesWarps) tmem_dealloc(tmem, 512);
 }
 
-// Adds the parts of a unit that spans CTAs: one CTA per (CTA it begins in,
-// eight rows), a warp a row.
+// Adds the parts of a unit that spans CTAs: CTAs of 32 rows per CTA it begins
+// in, a quarter of a warp a row.
+constexpr int kJoinRows = kThreads / 8;
+
 template <int D>
 __global__ void __launch_bounds__(kThreads) attn_q4_many_join_kernel(const ManyArgs args) {
-    constexpr int PER = D / 32;
+    constexpr int PER = D / 32;  // float4 of a lane
     griddep_wait();
     griddep_launch_dependents();
     const ManyPart part = args.parts[blockIdx.x];
@@ -1702,29 +1697,38 @@ __global__ void __launch_bounds__(kThreads) attn_q4_many_join_kernel(const ManyA
     const AttnQ4Args& a = args.a;
     int first, n, kv;
     kv_seq(a.v, part.seq, &first, &n, &kv);
-    const int row = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (part.row0 + row >= static_cast<int64_t>(n) * args.group) return;
-    float m = -INFINITY, l = 0.0f, o[PER];
+    const int row = blockIdx.y * kJoinRows + threadIdx.x / 8, lane = threadIdx.x & 7;
+    if (part.row0 + row >= n * args.group) return;
+    float m = -INFINITY, l = 0.0f;
+    float4 o[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) o[j] = 0.0f;
+    for (int j = 0; j < PER; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p = blockIdx.x; p <= part.last_cta; ++p) {
         const int64_t at = (p * 2LL + (p == static_cast<int>(blockIdx.x) ? part.place : 0)) * kManyRows + row;
         const float2 ml = args.part_ml[at];
-        float x[PER];
+        float4 x[PER];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) x[j] = args.part_o[at * D + lane * PER + j];
+        for (int j = 0; j < PER; ++j) x[j] = *reinterpret_cast<const float4*>(args.part_o + at * D + j * 32 + lane * 4);
         const float big = fmaxf(m, ml.x), base = big == -INFINITY ? 0.0f : big;
         const float f0 = fast_exp2(m - base), f1 = fast_exp2(ml.x - base);
         l = l * f0 + ml.y * f1;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] = o[j] * f0 + x[j] * f1;
+        for (int j = 0; j < PER; ++j) {
+            o[j].x = o[j].x * f0 + x[j].x * f1;
+            o[j].y = o[j].y * f0 + x[j].y * f1;
+            o[j].z = o[j].z * f0 + x[j].z * f1;
+            o[j].w = o[j].w * f0 + x[j].w * f1;
+        }
         m = big;
     }
     const float inv = l == 0.0f ? 0.0f : fast_rcp(l);
     const int tok = (part.row0 + row) / args.group, gh = part.row0 + row - tok * args.group;
-    uint16_t* dst = a.out + (first + tok) * a.ldo + (part.head * args.group + gh) * D + lane * PER;
+    uint16_t* dst = a.out + (first + tok) * a.ldo + (part.head * args.group + gh) * D + lane * 4;
 #pragma unroll
-    for (int j = 0; j < PER; j += 2) store2(dst + j, narrow2(o[j] * inv, o[j + 1] * inv, a.dtype));
+    for (int j = 0; j < PER; ++j) {
+        store2(dst + j * 32, narrow2(o[j].x * inv, o[j].y * inv, a.dtype));
+        store2(dst + j * 32 + 2, narrow2(o[j].z * inv, o[j].w * inv, a.dtype));
+    }
 }
 
 }  // namespace
@@ -1740,8 +1744,8 @@ static int check_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int64_t head
     // Rows and tiles are numbered in 31 bits.
     const double group = static_cast<double>(heads / kv->kv_heads), keys = static_cast<double>(batch->max_kv_len) + 128;
     const double rows = static_cast<double>(batch->tokens) * group;
-    if (rows + 512.0 * batch->seqs + keys * group > 2147483647.0 || static_cast<double>(batch->seqs) * kv->kv_heads * keys / 32 > 2147483647.0 ||
-        (rows / 256 + batch->seqs) * kv->kv_heads * keys / 128 > 2147483647.0)
+    if (rows + 512.0 * batch->seqs + keys * group > 2147483647.0 || static_cast<double>(batch->seqs) * kv->kv_heads * (keys / kTile + unit_cost(32)) > 2147483647.0 ||
+        (rows / kManyRows + batch->seqs) * kv->kv_heads * (keys / kManyKeys + kManyCost) > 2147483647.0)
         return set_error(MRT_ERR_SHAPE, "too many rows and keys for one call");
     return MRT_OK;
 }
@@ -1842,7 +1846,9 @@ cudaError_t launch_many(const ManyArgs& m, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(attn_q4_many_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) e = launch_pdl(attn_q4_many_kernel<D, BF16>, dim3(m.grid), kManyThreads, smem, s, m);
     if (e == cudaSuccess)
-        e = launch_pdl(attn_q4_many_join_kernel<D>, dim3(m.grid, kManyRows / (kThreads / 32)), kThreads, 0, s, m);
+        e = cudaFuncSetAttribute(attn_q4_many_join_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess)
+        e = launch_pdl(attn_q4_many_join_kernel<D>, dim3(m.grid, kManyRows / kJoinRows), kThreads, 0, s, m);
     return e;
 }
 
@@ -1911,6 +1917,7 @@ extern "C" int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int 
         ManyArgs m{};
         m.a = a;
         m.group = static_cast<int>(heads / kv->kv_heads);
+        m.group_magic = m.group > 1 ? static_cast<uint32_t>(((1ull << 32) + m.group - 1) / m.group) : 0;
         m.grid = plan.grid;
         m.part_o = static_cast<float*>(ws_dev);
         m.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws_dev) + plan.o_bytes);
