@@ -1040,6 +1040,13 @@ __device__ __forceinline__ uint64_t mask2(uint64_t v, bool lo, bool hi) {
     return pair2(lo ? -INFINITY : low2(v), hi ? -INFINITY : high2(v));
 }
 
+// (A NaN is passed over.)
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
 constexpr uint32_t kSixteenth = 0x2C002C00u;  // FP16 1/16 twice
 
 // Codes at bits 0-3 / 4-7 of each half less the zero points, as FP16: z1024 =
@@ -1267,13 +1274,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             const int count = u.count;
             if (count == 0) break;
             if (i < u.row_tiles()) {
-            float m[2];
+            // Scores are kept relative to m, once a row has seen a key: `far` is what may
+            // not be passed (-inf before: any key).
+            float m[2], far[2];
             uint64_t l[2];  // sums over even and over odd columns
             int limit[2], limit_min = 0x7FFFFFFF;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int row = i * 128 + row_in + b * 8;
-                m[b] = -INFINITY;
+                m[b] = 0.0f;
+                far[b] = -INFINITY;
                 l[b] = 0;
                 limit[b] = 0;
                 if (row < u.rows) {
@@ -1292,47 +1302,47 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 wait_phase(&s_scores[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
                 __syncwarp();
                 tc_fence_after();
-                // y = scale log2(e) s_k S: [column pair][row]
-                uint64_t y[16];
+                // e = scale log2(e) s_k S - m: [column pair][row]
+                uint64_t e[16];
                 {
+                    const uint64_t less[2] = {pair2(-m[0], -m[0]), pair2(-m[1], -m[1])};
                     uint32_t s[32];
                     tmem_ld_frag64(t_s, s);
                     const uint8_t* kl = cols + st * S::kCols + c * S::kColsRow;
 #pragma unroll
                     for (int k = 0; k < 8; k += 2) {
                         const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(kl + k * 8);
-                        y[k * 2] = mul2(pair2(s[k * 4], s[k * 4 + 1]), w.x);
-                        y[k * 2 + 1] = mul2(pair2(s[k * 4 + 2], s[k * 4 + 3]), w.x);
-                        y[k * 2 + 2] = mul2(pair2(s[k * 4 + 4], s[k * 4 + 5]), w.y);
-                        y[k * 2 + 3] = mul2(pair2(s[k * 4 + 6], s[k * 4 + 7]), w.y);
+                        e[k * 2] = fma2(pair2(s[k * 4], s[k * 4 + 1]), w.x, less[0]);
+                        e[k * 2 + 1] = fma2(pair2(s[k * 4 + 2], s[k * 4 + 3]), w.x, less[1]);
+                        e[k * 2 + 2] = fma2(pair2(s[k * 4 + 4], s[k * 4 + 5]), w.y, less[0]);
+                        e[k * 2 + 3] = fma2(pair2(s[k * 4 + 6], s[k * 4 + 7]), w.y, less[1]);
                     }
                 }
                 if (pos0 + kManyKeys > limit_min) {
                     const int left0 = limit[0] - pos0 - c * 2, left1 = limit[1] - pos0 - c * 2;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        y[k * 2] = mask2(y[k * 2], k * 8 >= left0, k * 8 + 1 >= left0);
-                        y[k * 2 + 1] = mask2(y[k * 2 + 1], k * 8 >= left1, k * 8 + 1 >= left1);
+                        e[k * 2] = mask2(e[k * 2], k * 8 >= left0, k * 8 + 1 >= left0);
+                        e[k * 2 + 1] = mask2(e[k * 2 + 1], k * 8 >= left1, k * 8 + 1 >= left1);
                     }
                 }
                 float big[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 16; ++k) big[k & 1] = fmaxf(big[k & 1], fmaxf(low2(y[k]), high2(y[k])));
-                bool grow = false;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
-                    big[b] = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 2));
-                    grow |= big[b] > m[b] + 8.0f;  // from -inf: any
-                }
-                if (__any_sync(0xFFFFFFFFu, grow)) {
+                for (int k = 0; k < 16; ++k) big[k & 1] = max3(big[k & 1], low2(e[k]), high2(e[k]));
+                if (__any_sync(0xFFFFFFFFu, big[0] > far[0] || big[1] > far[1])) {
                     float fix[2];
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
-                        const float to = fmaxf(m[b], big[b]);
-                        fix[b] = to == -INFINITY ? 1.0f : fast_exp2(m[b] - to);
-                        m[b] = to;
+                        float x = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
+                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
+                        const bool seen = far[b] > 0.0f;
+                        const float up = x > (seen ? 0.0f : -INFINITY) ? x : 0.0f;
+                        fix[b] = seen ? fast_exp2(-up) : 1.0f;
+                        if (x > -INFINITY) far[b] = 8.0f;
+                        m[b] += up;
                         l[b] = mul2(l[b], pair2(fix[b], fix[b]));
+#pragma unroll
+                        for (int k = b; k < 16; k += 2) e[k] = add2(e[k], pair2(-up, -up));
                     }
                     if (j > 0) {  // O, once the last product into it has ended
                         wait_phase(&s_done[i][buf ^ 1], ((t - 1) >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
@@ -1348,13 +1358,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                         }
                     }
                 }
-                const float n0 = m[0] == -INFINITY ? 0.0f : -m[0], n1 = m[1] == -INFINITY ? 0.0f : -m[1];
-                const uint64_t less[2] = {pair2(n0, n0), pair2(n1, n1)};
                 uint32_t p[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const uint64_t e = add2(y[k], less[k & 1]);
-                    const float p0 = fast_exp2(low2(e)), p1 = fast_exp2(high2(e));
+                    const float p0 = fast_exp2(low2(e[k])), p1 = fast_exp2(high2(e[k]));
                     l[k & 1] = add2(l[k & 1], pair2(p0, p1));
                     const __half2 hp = __floats2half2_rn(p0, p1);
                     p[k] = *reinterpret_cast<const uint32_t*>(&hp);
@@ -1402,7 +1409,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                         for (int k = 0; k < 4; ++k)
                             *reinterpret_cast<float2*>(dst + k * 8) =
                                 make_float2(__uint_as_float(o[k * 4 + b * 2]), __uint_as_float(o[k * 4 + b * 2 + 1]));
-                        if (ch == 0 && c == 0) args.part_ml[slot * kManyRows + row] = make_float2(m[b], sums[b]);
+                        if (ch == 0 && c == 0) args.part_ml[slot * kManyRows + row] = make_float2(far[b] > 0.0f ? m[b] : -INFINITY, sums[b]);
                     }
                 }
             }
