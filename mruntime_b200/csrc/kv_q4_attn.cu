@@ -1036,10 +1036,6 @@ __device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-__device__ __forceinline__ uint64_t mask2(uint64_t v, bool lo, bool hi) {
-    return pair2(lo ? -INFINITY : low2(v), hi ? -INFINITY : high2(v));
-}
-
 // (A NaN is passed over.)
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float r;
@@ -1302,8 +1298,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 wait_phase(&s_scores[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
                 __syncwarp();
                 tc_fence_after();
-                // e = scale log2(e) s_k S - m: [column pair][row]
-                uint64_t e[16];
+                // e = scale log2(e) s_k S - m: [row][column]
+                float e[2][16];
                 {
                     const uint64_t less[2] = {pair2(-m[0], -m[0]), pair2(-m[1], -m[1])};
                     uint32_t s[32];
@@ -1312,23 +1308,26 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
 #pragma unroll
                     for (int k = 0; k < 8; k += 2) {
                         const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(kl + k * 8);
-                        e[k * 2] = fma2(pair2(s[k * 4], s[k * 4 + 1]), w.x, less[0]);
-                        e[k * 2 + 1] = fma2(pair2(s[k * 4 + 2], s[k * 4 + 3]), w.x, less[1]);
-                        e[k * 2 + 2] = fma2(pair2(s[k * 4 + 4], s[k * 4 + 5]), w.y, less[0]);
-                        e[k * 2 + 3] = fma2(pair2(s[k * 4 + 6], s[k * 4 + 7]), w.y, less[1]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint64_t x = fma2(pair2(s[k * 4 + i * 2], s[k * 4 + i * 2 + 1]), i < 2 ? w.x : w.y, less[i & 1]);
+                            e[i & 1][(k + (i >> 1)) * 2] = low2(x);
+                            e[i & 1][(k + (i >> 1)) * 2 + 1] = high2(x);
+                        }
                     }
                 }
                 if (pos0 + kManyKeys > limit_min) {
-                    const int left0 = limit[0] - pos0 - c * 2, left1 = limit[1] - pos0 - c * 2;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        e[k * 2] = mask2(e[k * 2], k * 8 >= left0, k * 8 + 1 >= left0);
-                        e[k * 2 + 1] = mask2(e[k * 2 + 1], k * 8 >= left1, k * 8 + 1 >= left1);
+                    for (int b = 0; b < 2; ++b) {
+                        const int left = limit[b] - pos0 - c * 2;
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if ((k >> 1) * 8 + (k & 1) >= left) e[b][k] = -INFINITY;
                     }
                 }
                 float big[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 16; ++k) big[k & 1] = max3(big[k & 1], low2(e[k]), high2(e[k]));
+                for (int k = 0; k < 16; ++k) big[k & 1] = max3(big[k & 1], e[k & 1][k & ~1], e[k & 1][k | 1]);
                 if (__any_sync(0xFFFFFFFFu, big[0] > far[0] || big[1] > far[1])) {
                     float fix[2];
 #pragma unroll
@@ -1342,7 +1341,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                         m[b] += up;
                         l[b] = mul2(l[b], pair2(fix[b], fix[b]));
 #pragma unroll
-                        for (int k = b; k < 16; k += 2) e[k] = add2(e[k], pair2(-up, -up));
+                        for (int k = 0; k < 16; ++k) e[b][k] -= up;
                     }
                     if (j > 0) {  // O, once the last product into it has ended
                         wait_phase(&s_done[i][buf ^ 1], ((t - 1) >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
@@ -1361,7 +1360,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 uint32_t p[16];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const float p0 = fast_exp2(low2(e[k])), p1 = fast_exp2(high2(e[k]));
+                    const float p0 = fast_exp2(e[k & 1][k & ~1]), p1 = fast_exp2(e[k & 1][k | 1]);
                     l[k & 1] = add2(l[k & 1], pair2(p0, p1));
                     const __half2 hp = __floats2half2_rn(p0, p1);
                     p[k] = *reinterpret_cast<const uint32_t*>(&hp);
@@ -1522,7 +1521,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                         if ((sv[k] & 0x7C000000u) == 0x7C000000u) sv[k] &= 0xFFFFu;
                     }
                     const uint32_t vst = v_u32 + st * S::kV;
-#pragma unroll 1
+#pragma unroll 2
                     for (int hw = 0; hw < D / 32; ++hw) {  // word of a pair
                         uint32_t x[4];
 #pragma unroll
