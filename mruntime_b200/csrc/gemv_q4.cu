@@ -492,31 +492,41 @@ struct GemvPlan {
     int per_sm;  // CTAs a multiprocessor
 };
 
-// Candidates by time, in microseconds.  A multiprocessor works off a piece in
-// 0.025 us when its warps are many, a warp alone in 0.3 us; x comes into every
-// CTA from L2; larger CTAs start later, and joining sums costs.
+// Candidates by time, in microseconds.  A multiprocessor with all its warps
+// works off a piece in 0.029 us (with four groups in 0.053), a warp alone in
+// 0.38; x comes into every CTA from L2; larger CTAs start later, and joining
+// sums costs.  The numbers are a fit to every candidate's time for twenty
+// weights, 896 x 896 to 152064 x 3584 at 1 to 16 tokens: the times are told
+// within 13% on average, and the choice costs 2% over the best.
+constexpr int kShares[] = {1, 2, 4, 8, 12, 16, 24};  // warps of a tile
+
 GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
     GemvPlan best{0, 0, 0, 0};
     double best_us = 0.0;
     const int nt = M <= 8 ? 1 : 2;
     for (int per_sm = nt == 1 ? 3 : 2; per_sm > 0; --per_sm)
         for (int ks = 1; ks <= 8; ks *= 2)
-            for (int wk : {1, 2, 4, 8, 12, 16, 24}) {
-                const int warps = most_warps(nt) / per_sm, slice = (blocks + ks - 1) / ks;
-                if (warps % wk != 0 || (ks > 1 && (ks - 1) * slice >= blocks) || (wk > 1 && (wk - 1) * kPair >= slice)) continue;
+            for (int c = 0; c < 14; ++c) {
+                // As many warps as fit, or as many as give every CTA one turn's share.
+                // (Clusters of four and eight leave some multiprocessors idle: of 148
+                // they reach 132 and 120.)
+                const int wk = kShares[c >> 1], most = most_warps(nt) / per_sm, slice = (blocks + ks - 1) / ks;
+                const int room_x = std::max(1, sms * per_sm * (ks < 4 ? 16 : (ks == 4 ? 14 : 13)) / (16 * ks));
+                const int warps = (c & 1) ? wk * ((tiles + room_x - 1) / room_x) : most;
+                if (warps > most || warps % wk != 0 || (ks > 1 && (ks - 1) * slice >= blocks) || (wk > 1 && (wk - 1) * kPair >= slice)) continue;
                 if (gemv_smem(M, slice, per, nt, warps, wk * ks > 1, kMinStages, piece) > kSmemMost / per_sm) continue;
                 const int per_cta = warps / wk;
                 const int64_t ctas = static_cast<int64_t>((tiles + per_cta - 1) / per_cta) * ks, room = static_cast<int64_t>(sms) * per_sm;
-                if (ks > 1 && ctas > room) continue;  // slices' CTAs take one turn
+                if (ks > 1 && ctas > room_x * ks) continue;  // slices' CTAs take one turn
                 const int64_t turns = (ctas + room - 1) / room, live = std::min(ctas, room);
                 const int warp_pieces = (slice + wk * kPair - 1) / (wk * kPair) * kPair;
                 // of the busiest multiprocessor, of all of them
-                const double most = static_cast<double>((live + sms - 1) / sms) * turns * per_cta * slice;
+                const double busiest = static_cast<double>((live + sms - 1) / sms) * turns * per_cta * slice;
                 const double mean = static_cast<double>(tiles) * blocks / sms;
-                const double a_piece = (per == 4 ? 0.030 : 0.025) * (nt == 1 ? 1.0 : 1.3);
-                const double work = std::max((0.3 * most + 0.7 * mean) * a_piece, std::max(1.0, mean / (per_sm * per_cta * slice)) * warp_pieces * 0.3);
-                const double x = live * 256.0 / 8.0e6 * M * slice + M * slice * 16.0 / (warps * 32) * 0.1;
-                const double us = work + x + 0.04 * warps + (wk > 1 ? 0.3 * turns : 0.0) + (ks > 1 ? 1.5 : 0.0);
+                const double a_piece = (per == 4 ? 0.053 : 0.029) * (nt == 1 ? 1.0 : 1.4) * (0.86 + 0.14 * most_warps(nt) / (warps * per_sm));
+                const double work = std::max((0.43 * busiest + 0.57 * mean) * a_piece, std::max(1.0, mean / (per_sm * per_cta * slice)) * warp_pieces * 0.38);
+                const double x = live * 256.0 / 7.6e6 * M * slice + M * slice * 16.0 / (warps * 32) * 0.045;
+                const double us = work + x + 0.032 * warps + (wk > 1 ? 0.46 * turns : 0.0) + (ks > 1 ? 1.5 : 0.0);
                 if (best.wk == 0 || us < best_us) {
                     best = GemvPlan{warps, wk, ks, per_sm};
                     best_us = us;
