@@ -31,6 +31,17 @@
 #include "kernels.h"
 #include "q4.cuh"
 
+namespace mrt {
+
+// How a launch runs (plan_gemv()).
+struct GemvPlan {
+    int warps = 0, wk = 0, ks = 0;  // warps of a CTA, of a tile; slices of K.  0: no such launch
+    int per_sm = 0;                 // CTAs a multiprocessor
+};
+constexpr int kMaxTokens = 16;  // of a launch: two token tiles of eight
+
+}  // namespace mrt
+
 // Opaque handle of the public header.
 struct mrt_weight_q4_s {
     int device = -1;
@@ -41,6 +52,7 @@ struct mrt_weight_q4_s {
     int piece = 0;       // bytes of a (tile, block)
     uint8_t* data = nullptr;
     uint16_t* bias = nullptr;    // FP16 [n] or null
+    mrt::GemvPlan plans[mrt::kMaxTokens + 1];  // by tokens
 };
 
 namespace mrt {
@@ -212,8 +224,6 @@ struct GemvQ4Args {
     int* err_flag;
 };
 
-// Two token tiles of eight at most in one launch.
-constexpr int kMaxTokens = 16;
 constexpr int kMaxStages = 4, kMinStages = 2;
 constexpr int kPair = 2;  // neighbouring pieces that a stage holds
 constexpr int kSmemMost = 218 * 1024;  // of a multiprocessor's CTAs together
@@ -487,11 +497,6 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
     }
 }
 
-struct GemvPlan {
-    int warps, wk, ks;
-    int per_sm;  // CTAs a multiprocessor
-};
-
 // Candidates by time, in microseconds.  A multiprocessor with all its warps
 // works off a piece in 0.029 us (with four groups in 0.053), a warp alone in
 // 0.38; x comes into every CTA from L2; larger CTAs start later, and joining
@@ -501,7 +506,7 @@ struct GemvPlan {
 constexpr int kShares[] = {1, 2, 4, 8, 12, 16, 24};  // warps of a tile
 
 GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
-    GemvPlan best{0, 0, 0, 0};
+    GemvPlan best;
     double best_us = 0.0;
     const int nt = M <= 8 ? 1 : 2;
     for (int per_sm = nt == 1 ? 3 : 2; per_sm > 0; --per_sm)
@@ -541,7 +546,7 @@ cudaError_t launch(GemvQ4Args a, const GemvPlan& p, int sms, cudaStream_t s) {
     auto bytes = [&] { return gemv_smem(a.M, a.slice, PER, NT, p.warps, p.wk * p.ks > 1, a.stages, a.piece); };
     while (bytes() > kSmemMost / p.per_sm) --a.stages;
     if (a.stages < kMinStages) return cudaErrorInvalidValue;  // (the plan says that they fit)
-    cudaError_t e = cudaFuncSetAttribute(gemv_q4_kernel<PER, NT, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    cudaError_t e = prepare_kernel<gemv_q4_kernel<PER, NT, ZEROS>>(kSmemMost);
     if (e != cudaSuccess) return e;
     const int per_cta = p.warps / p.wk, ctas = (a.tiles + per_cta - 1) / per_cta;
     cudaLaunchConfig_t cfg{};
@@ -563,14 +568,12 @@ cudaError_t launch(GemvQ4Args a, const GemvPlan& p, int sms, cudaStream_t s) {
     return e;
 }
 
-// Tokens of one launch: sixteen, or as many as leave x room in shared memory
-// (0: not even one does).
-int tokens_at_once(int64_t M, int tiles, int blocks, int per, int piece, int sms, GemvPlan* plan) {
-    for (int m = static_cast<int>(std::min<int64_t>(M, kMaxTokens)); m > 0; m = m > 8 ? 8 : m / 2) {
-        *plan = plan_gemv(m, tiles, blocks, per, piece, sms);
-        if (plan->wk > 0) return m;
-    }
-    return 0;
+// Tokens of the next launch: sixteen, or as many as leave x room in shared
+// memory (0: not even one does).
+int tokens_at_once(const mrt_weight_q4_s* w, int64_t M) {
+    int m = static_cast<int>(std::min<int64_t>(M, kMaxTokens));
+    while (m > 0 && w->plans[m].wk == 0) m = m > 8 ? 8 : m / 2;
+    return m;
 }
 
 cudaError_t launch_gemv_q4(GemvQ4Args a, const GemvPlan& p, int per, int sms, cudaStream_t s) {
@@ -626,6 +629,8 @@ int new_handle(int64_t N, int64_t K, int64_t group, bool zeros, cudaStream_t s, 
     w->blocks = (K + 127) / 128;
     w->zeros = zeros;
     w->piece = piece_bytes(static_cast<int>(128 / group), zeros);
+    for (int m = 1; m <= kMaxTokens; ++m)
+        w->plans[m] = plan_gemv(m, static_cast<int>(w->tiles), static_cast<int>(w->blocks), static_cast<int>(128 / group), w->piece, c->sms);
     const size_t bytes = static_cast<size_t>(w->tiles) * w->blocks * w->piece;
     cudaError_t e = cudaMalloc(&w->data, bytes);
     if (e == cudaSuccess) e = cudaMemsetAsync(w->data, 0, bytes, s);
@@ -811,14 +816,13 @@ extern "C" int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, cons
     a.bias = use_bias ? w->bias : nullptr;
     a.ldr = ldr;
     const int per = static_cast<int>(128 / w->group);
-    GemvPlan plan;
     for (int64_t m = 0; m < M; m += a.M) {
-        a.M = tokens_at_once(M - m, a.tiles, a.blocks, per, a.piece, c->sms, &plan);
+        a.M = tokens_at_once(w, M - m);
         if (a.M == 0) return set_error(MRT_ERR_SHAPE, "K is too large for a token in shared memory");
         a.x = static_cast<const uint16_t*>(x_dev) + m * ldx;
         a.y = static_cast<uint8_t*>(y_dev) + m * ldy * (a.out_f32 ? 4 : 2);
         a.res = res_dev != nullptr ? static_cast<const uint16_t*>(res_dev) + m * ldr : nullptr;
-        const cudaError_t e = launch_gemv_q4(a, plan, per, c->sms, static_cast<cudaStream_t>(stream));
+        const cudaError_t e = launch_gemv_q4(a, w->plans[a.M], per, c->sms, static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) return cuda_error(e, "4-bit gemv launch");
     }
     return MRT_OK;

@@ -377,18 +377,18 @@ int tokens_of(int tokens, int sms) { return std::max(1, std::min(kMaxTokens, tok
 
 bool aligned16(const void* p, int64_t ld) { return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 7) == 0); }
 
-template <typename... P, typename... A>
-cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
+template <auto KERNEL, typename... A>
+cudaError_t launch_pdl(dim3 grid, cudaStream_t s, A... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
+    cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
     if (e == cudaSuccess) note_launches(1);
     return e;
 }
@@ -490,8 +490,7 @@ extern "C" int mrt_kv_q4_append(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dty
     for (int i = 0; i < 64; ++i) f.turn[i] = kv->freq[i];
     const dim3 grid(static_cast<unsigned>((a.v.tokens + a.tokens - 1) / a.tokens), static_cast<unsigned>((rows + a.rows - 1) / a.rows));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = D == 128 ? launch_pdl(kv_append_kernel<128>, grid, kThreads, s, a, f)
-                                   : launch_pdl(kv_append_kernel<64>, grid, kThreads, s, a, f);
+    const cudaError_t e = D == 128 ? launch_pdl<kv_append_kernel<128>>(grid, s, a, f) : launch_pdl<kv_append_kernel<64>>(grid, s, a, f);
     return e == cudaSuccess ? MRT_OK : cuda_error(e, "4-bit cache append launch");
 }
 
@@ -517,7 +516,6 @@ extern "C" int mrt_kv_q4_read(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype
     a.tokens = tokens_of(a.v.tokens, sms);
     const dim3 grid(static_cast<unsigned>((a.v.tokens + a.tokens - 1) / a.tokens));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = D == 128 ? launch_pdl(kv_read_kernel<128>, grid, kThreads, s, a)
-                                   : launch_pdl(kv_read_kernel<64>, grid, kThreads, s, a);
+    const cudaError_t e = D == 128 ? launch_pdl<kv_read_kernel<128>>(grid, s, a) : launch_pdl<kv_read_kernel<64>>(grid, s, a);
     return e == cudaSuccess ? MRT_OK : cuda_error(e, "4-bit cache read launch");
 }

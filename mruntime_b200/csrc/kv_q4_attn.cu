@@ -1793,8 +1793,10 @@ Plan make_plan(const KvView& v, int64_t heads, int sms) {
     return p;
 }
 
-template <typename... P, typename... A>
-cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+template <auto KERNEL, typename... A>
+cudaError_t launch_pdl(dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+    cudaError_t e = prepare_kernel<KERNEL>(smem);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -1805,34 +1807,18 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem, c
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
     if (e == cudaSuccess) note_launches(1);
     return e;
 }
 
-// (It runs beside the last CTAs before it and the first ones after it, so it wants
-// the same share of a multiprocessor's memory: a kernel of another share holds
-// CTAs of the next one off it.)
-template <int D, int THREADS>
-cudaError_t launch_join(const RowsArgs& r, int rows, int few, cudaStream_t s) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_q4_join_kernel<D, THREADS>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                               cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(attn_q4_join_kernel<D, THREADS>, dim3(r.a.v.seqs * r.a.v.kv_heads, rows), THREADS, 0, s, r, few * 8);
-}
-
 template <int D, int NT, int W>
 cudaError_t launch_few_w(const RowsArgs& r, int rows, cudaStream_t s) {
-    constexpr int smem = RowsShape<D, NT, W>::kBytes;
-    // Set at every call: it costs little and holds for whichever device is current.
-    cudaError_t e = cudaFuncSetAttribute(attn_q4_few_kernel<D, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(attn_q4_few_kernel<D, NT, W>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e == cudaSuccess) e = launch_pdl(attn_q4_few_kernel<D, NT, W>, dim3(r.grid), W * 32, smem, s, r);
-    if (e == cudaSuccess && r.split)
-        e = static_cast<int64_t>(r.a.v.seqs) * r.a.v.kv_heads * rows <= r.grid ? launch_join<D, 512>(r, rows, NT, s)
-                                                                             : launch_join<D, 64>(r, rows, NT, s);
-    return e;
+    cudaError_t e = launch_pdl<attn_q4_few_kernel<D, NT, W>>(dim3(r.grid), W * 32, RowsShape<D, NT, W>::kBytes, s, r);
+    if (e != cudaSuccess || !r.split) return e;
+    const dim3 grid(r.a.v.seqs * r.a.v.kv_heads, rows);  // a CTA a (unit, row)
+    return static_cast<int64_t>(grid.x) * rows <= r.grid ? launch_pdl<attn_q4_join_kernel<D, 512>>(grid, 512, 0, s, r, NT * 8)
+                                                         : launch_pdl<attn_q4_join_kernel<D, 64>>(grid, 64, 0, s, r, NT * 8);
 }
 
 template <int D>
@@ -1848,14 +1834,9 @@ cudaError_t launch_few(const RowsArgs& r, int few, int rows, cudaStream_t s) {
 
 template <int D, bool BF16>
 cudaError_t launch_many(const ManyArgs& m, cudaStream_t s) {
-    constexpr int smem = ManyShape<D>::kBytes;
-    cudaError_t e = cudaFuncSetAttribute(attn_q4_many_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = launch_pdl(attn_q4_many_kernel<D, BF16>, dim3(m.grid), kManyThreads, smem, s, m);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(attn_q4_many_join_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e == cudaSuccess)
-        e = launch_pdl(attn_q4_many_join_kernel<D>, dim3(m.grid, kManyRows / kJoinRows), kThreads, 0, s, m);
-    return e;
+    const cudaError_t e = launch_pdl<attn_q4_many_kernel<D, BF16>>(dim3(m.grid), kManyThreads, ManyShape<D>::kBytes, s, m);
+    if (e != cudaSuccess) return e;
+    return launch_pdl<attn_q4_many_join_kernel<D>>(dim3(m.grid, kManyRows / kJoinRows), kThreads, 0, s, m);
 }
 
 }  // namespace

@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace mrt {
 
 constexpr uint32_t kNib0 = 0x000F000Fu;  // codes at bits 0-3 of each half: value c * 2^-24
@@ -82,6 +84,24 @@ __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.com
 template <int N>
 __device__ __forceinline__ void copy_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A kernel's attributes, set once a device: its dynamic shared memory, and all of
+// a multiprocessor's memory as shared memory.  (These kernels run beside the last
+// CTAs of the one before and the first of the next: where one asks for another
+// share, it keeps the next one's CTAs off the multiprocessors that it is on.)
+template <auto KERNEL>
+cudaError_t prepare_kernel(int smem) {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+    return e;
 }
 
 // Two FP32 values in one 64-bit register pair.  (A product of pairs that only a
