@@ -70,6 +70,13 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // The sum is of p' / s_v, and the zero points' part of the output, sum p' z (of
 // the same rounded p'), is one more row of the second product.
 //
+// What bounds it: bytes and instructions alike.  64 sequences of up to 8192
+// tokens (176 MB, 7 of 8 rows used) take 42 us where the bytes would take 27 at
+// the copy's rate: 406 instructions a warp and tile, half of them the masks that
+// make operands of codes, would take 17, and beginning, joining and the CTAs'
+// uneven ends 9.  One of 131071 tokens (70 MB) takes 23 us for 11: 4 until the
+// first tile is there, 13 for the tiles, 5 for the parts.
+//
 // Split.  The 32-token tiles of all (sequence, kv head) units, in order, are
 // dealt to the CTAs in equal contiguous stretches, whatever the lengths: no
 // CTA waits for a long sequence, and no plan from the host is needed (lengths
@@ -103,6 +110,7 @@ __device__ __forceinline__ int seq_tiles(const KvView& v, int b) {
     return max(1, (kv + kTile - 1) / kTile);
 }
 
+// (64 x 8192 tokens 42.1 us, without 43.3; 9 x 3 x 6000 18.9 and 22.8.)
 __host__ __device__ constexpr int unit_cost(int rows) { return rows <= 16 ? 8 : 16; }
 __device__ __forceinline__ int unit_places(int tiles, int cost) { return tiles > 0 ? tiles + cost : 0; }
 
@@ -892,28 +900,36 @@ __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volat
 //   warps 28-30      Q into its panels
 //   warp 31          the walk over the CTA's units, published a few ahead
 //
-// Roles meet only at mbarriers, and units follow one another without a stop.  TMEM: two S (P in
-// its first half) for each row tile, O_0, O_1: the scores of the next keys are
-// there while the softmax works on these, so neither waits for the other's
-// whole chain (with 128 keys and one S a tile, softmax 4000 and products 2600
-// cycles alternated).
+// Roles meet only at mbarriers, and units follow one another without a stop.
+// TMEM: two S (P in its first half) for each row tile, O_0, O_1: the scores of
+// the next keys are there while the softmax works on these, so neither waits
+// for the other's whole chain (with 128 keys and one S a tile, softmax 4000 and
+// products 2600 cycles alternated).
 //
 // A key's scale multiplies its column of S, so scores are as exact as FP32; a
 // value's goes into the operand, at the price of one more rounding (2^-11 of
 // each value, independent from token to token like that of P, and averaged
 // with it), because every number that a column needs in the softmax is a
-// shared-memory read for every pair of rows, and shared memory is what bounds
-// this kernel (Q and K for S, V for O, the codes' stores, the columns'
-// scales); with the value's scale in the exponent, as in the few-rows kernel,
-// a column needed three.  The running maximum m is moved only when a row
-// exceeds it by 2^8 (P then still fits FP16 with all its bits), so O in TMEM is
-// hardly ever rescaled.  All loops are short: with the softmax unrolled over
-// its rows the kernel had 148 KB of code and every step of every role waited
-// for its instructions.
+// shared-memory read for every pair of rows; with the value's scale in the
+// exponent, as in the few-rows kernel, a column needed three.  Scores come out
+// of one fused operation relative to the running maximum m, which moves only
+// when a row exceeds it by 2^8 (P then still fits FP16 with all its bits): rows'
+// maxima are joined, scores moved and O in TMEM rescaled in that case alone.
+// All loops are short: with the softmax unrolled over its rows the kernel had
+// 148 KB of code and every step of every role waited for its instructions.
+//
+// What bounds it: 2048 tokens behind 14000 (28 heads on 4 of 128 channels) take
+// 474 us, 441 GFLOP at 55% of the rate of a large bf16 product.  Issue slots
+// (62% used) and shared memory (two thirds: Q and K for S, V for O, the codes'
+// stores, the columns' scales) come first, the exponentials' unit has 37%, the
+// tensor cores' 36.  Two prompts of 1800 and 965 tokens behind 100 and 54 (14
+// heads on 2 of 64) take 39 us, 9 of them until the first scores are there and 4
+// for the parts.
 //
 // Units' key tiles are dealt to the CTAs in equal contiguous stretches, as in
-// the few-rows kernel (each unit at kManyCost tiles more than it has), parts of
-// units that span CTAs joined from scratch.
+// the few-rows kernel (each unit at kManyCost tiles more than it has: without,
+// the two prompts took 70 us), parts of units that span CTAs joined from
+// scratch.
 constexpr int kManyRows = 256, kManyKeys = 64;
 constexpr int kSoftmaxWarps = 16, kCodesWarps = 8, kManyWarps = kSoftmaxWarps + kCodesWarps + 8;
 constexpr int kManyThreads = kManyWarps * 32;
@@ -1270,152 +1286,152 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             const int count = u.count;
             if (count == 0) break;
             if (i < u.row_tiles()) {
-            // Scores are kept relative to m, once a row has seen a key: `far` is what may
-            // not be passed (-inf before: any key).
-            float m[2], far[2];
-            uint64_t l[2];  // sums over even and over odd columns
-            int limit[2], limit_min = 0x7FFFFFFF;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int row = i * 128 + row_in + b * 8;
-                m[b] = 0.0f;
-                far[b] = -INFINITY;
-                l[b] = 0;
-                limit[b] = 0;
-                if (row < u.rows) {
-                    limit[b] = a.causal ? u.kv - u.n + (u.row0 + row) / args.group + 1 : u.kv;
-                    limit_min = min(limit_min, limit[b]);
-                }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
-#pragma unroll 1
-            for (int j = 0; j < count; ++j) {
-                const uint32_t it = stage_it + j, st = it % S::kStages, t = tile_it + j, buf = t & 1;
-                const uint32_t t_s = t_rows + buf * kManyKeys;
-                const int pos0 = (u.t0 + j) * kManyKeys;
-                wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
-                wait_phase(&s_scores[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
-                __syncwarp();
-                tc_fence_after();
-                // e = scale log2(e) s_k S - m: [row][column]
-                float e[2][16];
-                {
-                    const uint64_t less[2] = {pair2(-m[0], -m[0]), pair2(-m[1], -m[1])};
-                    uint32_t s[32];
-                    tmem_ld_frag64(t_s, s);
-                    const uint8_t* kl = cols + st * S::kCols + c * S::kColsRow;
-#pragma unroll
-                    for (int k = 0; k < 8; k += 2) {
-                        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(kl + k * 8);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint64_t x = fma2(pair2(s[k * 4 + i * 2], s[k * 4 + i * 2 + 1]), i < 2 ? w.x : w.y, less[i & 1]);
-                            e[i & 1][(k + (i >> 1)) * 2] = low2(x);
-                            e[i & 1][(k + (i >> 1)) * 2 + 1] = high2(x);
-                        }
-                    }
-                }
-                if (pos0 + kManyKeys > limit_min) {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const int left = limit[b] - pos0 - c * 2;
-#pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if ((k >> 1) * 8 + (k & 1) >= left) e[b][k] = -INFINITY;
-                    }
-                }
-                float big[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int k = 0; k < 16; ++k) big[k & 1] = max3(big[k & 1], e[k & 1][k & ~1], e[k & 1][k | 1]);
-                if (__any_sync(0xFFFFFFFFu, big[0] > far[0] || big[1] > far[1])) {
-                    float fix[2];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        float x = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
-                        x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
-                        const bool seen = far[b] > 0.0f;
-                        const float up = x > (seen ? 0.0f : -INFINITY) ? x : 0.0f;
-                        fix[b] = seen ? fast_exp2(-up) : 1.0f;
-                        if (x > -INFINITY) far[b] = 8.0f;
-                        m[b] += up;
-                        l[b] = mul2(l[b], pair2(fix[b], fix[b]));
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) e[b][k] -= up;
-                    }
-                    if (j > 0) {  // O, once the last product into it has ended
-                        wait_phase(&s_done[i][buf ^ 1], ((t - 1) >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
-                        __syncwarp();
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int ch = 0; ch < D; ch += 32) {
-                            uint32_t o[16];
-                            tmem_ld_frag32(t_o + ch, o);
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fix[(k >> 1) & 1]);
-                            tmem_st_frag32(t_o + ch, o);
-                        }
-                    }
-                }
-                uint32_t p[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const float p0 = fast_exp2(e[k & 1][k & ~1]), p1 = fast_exp2(e[k & 1][k | 1]);
-                    l[k & 1] = add2(l[k & 1], pair2(p0, p1));
-                    const __half2 hp = __floats2half2_rn(p0, p1);
-                    p[k] = *reinterpret_cast<const uint32_t*>(&hp);
-                }
-                tmem_st_pairs32(t_s, p);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_probs[i][buf]);
-            }
-            // The output, or the unit's part of it.
-            const uint32_t last = tile_it + count - 1;
-            wait_phase(&s_done[i][last & 1], (last >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
-            __syncwarp();
-            tc_fence_after();
-            const bool whole = u.whole;
-            const int64_t slot = blockIdx.x * 2LL + u.place;
-            float sums[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                sums[b] = low2(l[b]) + high2(l[b]);
-                sums[b] += __shfl_xor_sync(0xFFFFFFFFu, sums[b], 1);
-                sums[b] += __shfl_xor_sync(0xFFFFFFFFu, sums[b], 2);
-            }
-#pragma unroll 1
-            for (int ch = 0; ch < D; ch += 32) {
-                uint32_t o[16];
-                __syncwarp();
-                tmem_ld_frag32(t_o + ch, o);
+                // Scores are kept relative to m, once a row has seen a key: `far` is what may
+                // not be passed (-inf before: any key).
+                float m[2], far[2];
+                uint64_t l[2];  // sums over even and over odd columns
+                int limit[2], limit_min = 0x7FFFFFFF;
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const int row = i * 128 + row_in + b * 8;
-                    if (row >= u.rows) continue;
-                    if (whole) {
-                        const float inv = sums[b] == 0.0f ? 0.0f : fast_rcp(sums[b]);
-                        const int tok = (u.row0 + row) / args.group, gh = u.row0 + row - tok * args.group;
-                        uint16_t* dst = a.out + (u.first + tok) * a.ldo + (u.head * args.group + gh) * D + ch + c * 2;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            store2(dst + k * 8, narrow2(__uint_as_float(o[k * 4 + b * 2]) * inv,
-                                                        __uint_as_float(o[k * 4 + b * 2 + 1]) * inv, dtype));
-                    } else {
-                        float* dst = args.part_o + (slot * kManyRows + row) * D + ch + c * 2;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<float2*>(dst + k * 8) =
-                                make_float2(__uint_as_float(o[k * 4 + b * 2]), __uint_as_float(o[k * 4 + b * 2 + 1]));
-                        if (ch == 0 && c == 0) args.part_ml[slot * kManyRows + row] = make_float2(far[b] > 0.0f ? m[b] : -INFINITY, sums[b]);
+                    m[b] = 0.0f;
+                    far[b] = -INFINITY;
+                    l[b] = 0;
+                    limit[b] = 0;
+                    if (row < u.rows) {
+                        limit[b] = a.causal ? u.kv - u.n + (u.row0 + row) / args.group + 1 : u.kv;
+                        limit_min = min(limit_min, limit[b]);
                     }
                 }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[i]);
-            tile_it += count;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) limit_min = min(limit_min, __shfl_xor_sync(0xFFFFFFFFu, limit_min, o));
+#pragma unroll 1
+                for (int j = 0; j < count; ++j) {
+                    const uint32_t it = stage_it + j, st = it % S::kStages, t = tile_it + j, buf = t & 1;
+                    const uint32_t t_s = t_rows + buf * kManyKeys;
+                    const int pos0 = (u.t0 + j) * kManyKeys;
+                    wait_phase(&s_full[st], (it / S::kStages) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                    wait_phase(&s_scores[i][buf], (t >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                    __syncwarp();
+                    tc_fence_after();
+                    // e = scale log2(e) s_k S - m: [row][column]
+                    float e[2][16];
+                    {
+                        const uint64_t less[2] = {pair2(-m[0], -m[0]), pair2(-m[1], -m[1])};
+                        uint32_t s[32];
+                        tmem_ld_frag64(t_s, s);
+                        const uint8_t* kl = cols + st * S::kCols + c * S::kColsRow;
+#pragma unroll
+                        for (int k = 0; k < 8; k += 2) {
+                            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(kl + k * 8);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint64_t x = fma2(pair2(s[k * 4 + i * 2], s[k * 4 + i * 2 + 1]), i < 2 ? w.x : w.y, less[i & 1]);
+                                e[i & 1][(k + (i >> 1)) * 2] = low2(x);
+                                e[i & 1][(k + (i >> 1)) * 2 + 1] = high2(x);
+                            }
+                        }
+                    }
+                    if (pos0 + kManyKeys > limit_min) {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const int left = limit[b] - pos0 - c * 2;
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if ((k >> 1) * 8 + (k & 1) >= left) e[b][k] = -INFINITY;
+                        }
+                    }
+                    float big[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) big[k & 1] = max3(big[k & 1], e[k & 1][k & ~1], e[k & 1][k | 1]);
+                    if (__any_sync(0xFFFFFFFFu, big[0] > far[0] || big[1] > far[1])) {
+                        float fix[2];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            float x = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
+                            x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
+                            const bool seen = far[b] > 0.0f;
+                            const float up = x > (seen ? 0.0f : -INFINITY) ? x : 0.0f;
+                            fix[b] = seen ? fast_exp2(-up) : 1.0f;
+                            if (x > -INFINITY) far[b] = 8.0f;
+                            m[b] += up;
+                            l[b] = mul2(l[b], pair2(fix[b], fix[b]));
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) e[b][k] -= up;
+                        }
+                        if (j > 0) {  // O, once the last product into it has ended
+                            wait_phase(&s_done[i][buf ^ 1], ((t - 1) >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                            __syncwarp();
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int ch = 0; ch < D; ch += 32) {
+                                uint32_t o[16];
+                                tmem_ld_frag32(t_o + ch, o);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fix[(k >> 1) & 1]);
+                                tmem_st_frag32(t_o + ch, o);
+                            }
+                        }
+                    }
+                    uint32_t p[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float p0 = fast_exp2(e[k & 1][k & ~1]), p1 = fast_exp2(e[k & 1][k | 1]);
+                        l[k & 1] = add2(l[k & 1], pair2(p0, p1));
+                        const __half2 hp = __floats2half2_rn(p0, p1);
+                        p[k] = *reinterpret_cast<const uint32_t*>(&hp);
+                    }
+                    tmem_st_pairs32(t_s, p);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_probs[i][buf]);
+                }
+                // The output, or the unit's part of it.
+                const uint32_t last = tile_it + count - 1;
+                wait_phase(&s_done[i][last & 1], (last >> 1) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+                __syncwarp();
+                tc_fence_after();
+                const bool whole = u.whole;
+                const int64_t slot = blockIdx.x * 2LL + u.place;
+                float sums[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    sums[b] = low2(l[b]) + high2(l[b]);
+                    sums[b] += __shfl_xor_sync(0xFFFFFFFFu, sums[b], 1);
+                    sums[b] += __shfl_xor_sync(0xFFFFFFFFu, sums[b], 2);
+                }
+#pragma unroll 1
+                for (int ch = 0; ch < D; ch += 32) {
+                    uint32_t o[16];
+                    __syncwarp();
+                    tmem_ld_frag32(t_o + ch, o);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const int row = i * 128 + row_in + b * 8;
+                        if (row >= u.rows) continue;
+                        if (whole) {
+                            const float inv = sums[b] == 0.0f ? 0.0f : fast_rcp(sums[b]);
+                            const int tok = (u.row0 + row) / args.group, gh = u.row0 + row - tok * args.group;
+                            uint16_t* dst = a.out + (u.first + tok) * a.ldo + (u.head * args.group + gh) * D + ch + c * 2;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                store2(dst + k * 8, narrow2(__uint_as_float(o[k * 4 + b * 2]) * inv,
+                                                            __uint_as_float(o[k * 4 + b * 2 + 1]) * inv, dtype));
+                        } else {
+                            float* dst = args.part_o + (slot * kManyRows + row) * D + ch + c * 2;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                *reinterpret_cast<float2*>(dst + k * 8) =
+                                    make_float2(__uint_as_float(o[k * 4 + b * 2]), __uint_as_float(o[k * 4 + b * 2 + 1]));
+                            if (ch == 0 && c == 0) args.part_ml[slot * kManyRows + row] = make_float2(far[b] > 0.0f ? m[b] : -INFINITY, sums[b]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[i]);
+                tile_it += count;
             }
             stage_it += count;
             __syncwarp();
@@ -1773,6 +1789,9 @@ constexpr int kSplitWarps = 4, kWholeWarps = 16;
 Plan make_plan(const KvView& v, int64_t heads, int sms) {
     Plan p{};
     const int64_t rows = heads / v.kv_heads * std::max(v.max_q_len, 1);
+    // Rows beside the keys' 16 of an MMA while they fill four of its tiles: 9 x 6000
+    // tokens, 28 rows, 24.8 us against 33.0 of the many-rows kernel, 64 x 8192 110
+    // against 164, 1 x 131071 47 against 92.
     if (rows > 32) {
         p.split = 1;
         p.grid = sms;
@@ -1782,9 +1801,12 @@ Plan make_plan(const KvView& v, int64_t heads, int sms) {
         return p;
     }
     p.few = static_cast<int>((rows + 7) / 8);
-    // Few short units: one CTA of sixteen warps each and no join.
+    // Few short units: one CTA of sixteen warps each and no join (1 x 517 tokens 5.4 us
+    // against 6.7 split, 8 x 1000 7.6 against 12.6; but 1 x 2000 10.2 against 7.5).
     const int64_t units = static_cast<int64_t>(v.seqs) * v.kv_heads;
     p.split = !(v.max_kv_len <= kWholeWarps * 2 * kTile && units <= sms && p.few <= 2);
+    // As many CTAs of four warps as registers and shared memory have room for (four:
+    // 64 x 8192 tokens 41.4 us; two of eight warps 43.9).
     p.grid = p.split ? sms * (p.few == 1 ? 4 : (p.few == 2 ? 3 : 2)) : static_cast<int>(units);
     if (p.split) {
         p.o_bytes = static_cast<size_t>(p.grid) * 2 * p.few * 8 * v.head_dim * 4;
@@ -1817,8 +1839,11 @@ cudaError_t launch_few_w(const RowsArgs& r, int rows, cudaStream_t s) {
     cudaError_t e = launch_pdl<attn_q4_few_kernel<D, NT, W>>(dim3(r.grid), W * 32, RowsShape<D, NT, W>::kBytes, s, r);
     if (e != cudaSuccess || !r.split) return e;
     const dim3 grid(r.a.v.seqs * r.a.v.kv_heads, rows);  // a CTA a (unit, row)
-    return static_cast<int64_t>(grid.x) * rows <= r.grid ? launch_pdl<attn_q4_join_kernel<D, 512>>(grid, 512, 0, s, r, NT * 8)
-                                                         : launch_pdl<attn_q4_join_kernel<D, 64>>(grid, 64, 0, s, r, NT * 8);
+    // Units of 24 parts and more are worth a large CTA: 1 x 131071 tokens (148 parts)
+    // 22.8 us against 33.9, 4 x 30000 (37) 18.1 against 23.7; 8 x 4000 (18) 14.0
+    // against 11.5, 16 x 4000 (9) 20.7 against 14.5.
+    return static_cast<int64_t>(grid.x) * 24 <= r.grid ? launch_pdl<attn_q4_join_kernel<D, 512>>(grid, 512, 0, s, r, NT * 8)
+                                                       : launch_pdl<attn_q4_join_kernel<D, 64>>(grid, 64, 0, s, r, NT * 8);
 }
 
 template <int D>

@@ -63,6 +63,36 @@ def test_product(cuda_dev, M, N, K, group, zeros):
     assert torch.equal(run(w, x), got)
 
 
+@pytest.mark.parametrize("M,N,K,group,zeros", [(7, 700, 18944, 32, True), (16, 700, 18944, 128, False),
+                                               (10, 1200, 9600, 64, True), (1, 1700, 9600, 64, False),
+                                               (4, 4608, 512, 64, True), (25, 900, 9600, 128, True)])
+def test_long_sums_cut_into_slices(cuda_dev, M, N, K, group, zeros):
+    """Where x is too much for one CTA, or the rows too few for the device."""
+    w, val, mag = make(N, K, group, zeros, N)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(N)).half()
+    y, tol = bound(x, val, mag, 2.0 ** -11, K)
+    got = run(w, x)
+    assert ((got.double() - y).abs() <= tol).all()
+    assert torch.equal(run(w, x), got)
+
+
+def test_one_weight_on_two_streams(cuda_dev):
+    """Calls that overlap give what they give alone."""
+    w, _, _ = make(700, 4096, 64, True, 4)
+    xs = [torch.randn(m, 4096, generator=torch.Generator().manual_seed(m)).half() for m in (1, 16)]
+    want = [run(w, x) for x in xs]
+    xd, streams = [x.cuda() for x in xs], [torch.cuda.Stream() for _ in xs]
+    ys = [torch.zeros(8, x.shape[0], 700, dtype=torch.float16, device="cuda") for x in xs]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for x, y, s in zip(xd, ys, streams):
+            capi.gemv_q4(w, x.data_ptr(), 4096, y[i].data_ptr(), 700, x.shape[0], stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    capi.sync(stream())
+    for y, o in zip(ys, want):
+        assert (y.cpu() == o).all()
+
+
 @pytest.mark.parametrize("M", [1, 5, 20])
 def test_bias_and_residual(cuda_dev, M):
     N, K = 90, 256

@@ -308,6 +308,93 @@ def test_attention(cuda_dev, case, dtype, causal):
     assert torch.equal(qd[:n], out[:n])
 
 
+def check_attention(c, q, k, v, causal):
+    c.fill(k.cuda(), v.cuda())
+    out = c.attend(q.cuda(), causal)
+    capi.sync(stream())
+    (kx, _), (vx, vs) = quantised(k.float()), quantised(v.float())
+    want, tol = reference(c, q, kx, vx, vs, causal, c.D ** -0.5)
+    bad = (out.cpu().double() - want).abs() > tol
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off"
+    return out
+
+
+@pytest.mark.parametrize("seqs,n_max,H,Hk", [(300, 1, 4, 2), (1100, 20, 2, 1)])
+def test_many_short_sequences(cuda_dev, seqs, n_max, H, Hk):
+    """More sequences than a CTA has threads, some of them without rows or without tokens."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = []
+    for b in range(seqs):
+        kv = int(torch.randint(0, 50, (1,), generator=g))
+        lens.append((min(kv, 0 if b % 5 == 0 else 1), kv))
+    lens[seqs // 2] = (n_max, 90)
+    c = Cache(lens, H, Hk, 64, 16, seed=seqs)
+    check_attention(c, *held_rows(c, seqs), True)
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_random_batches(cuda_dev, seed):
+    """Stretches that begin and end anywhere in sequences of any length."""
+    g = torch.Generator().manual_seed(1000 + seed)
+
+    def pick(lo, hi):
+        return int(torch.randint(lo, hi + 1, (1,), generator=g))
+
+    Hk, group, D = pick(1, 4), [1, 3, 7, 8][pick(0, 3)], [64, 128][pick(0, 1)]
+    n_max = [1, 3, 40, 90][seed % 4]
+    lens = []
+    for _ in range(pick(1, 14)):
+        n = pick(0, n_max)
+        lens.append((n, n + pick(0, [40, 700, 3000][pick(0, 2)])))
+    lens.append((n_max, n_max + pick(0, 5000)))
+    c = Cache(lens, group * Hk, Hk, D, [16, 48, 64][pick(0, 2)], seed=seed)
+    check_attention(c, *held_rows(c, seed), seed % 3 != 0)
+
+
+@pytest.mark.parametrize("n", [1, 50])
+@pytest.mark.parametrize("off,pad", [(1, 3), (4, 8)])
+def test_attention_strides(cuda_dev, n, off, pad):
+    """q and out inside rows of other things, at any alignment of two bytes."""
+    c = Cache([(n, 130), (n, 61)], 6, 2, 64, 16, seed=5)
+    q, k, v = held_rows(c, 5)
+    want = check_attention(c, q, k, v, True)
+    ld = 6 * 64 + pad
+    qb = torch.full((off + 2 * n * ld,), 3.0, dtype=torch.float16, device="cuda")
+    qb[off:].view(2 * n, ld)[:, :384] = q.view(2 * n, 384).cuda()
+    ob = torch.full_like(qb, 9.0)
+    ws = torch.empty(max(16, c.kv.attention_workspace(c.batch, 6)), dtype=torch.uint8, device="cuda")
+    c.kv.attention(c.batch, capi.FP16, qb.data_ptr() + 2 * off, ld, 6, ob.data_ptr() + 2 * off, ld, 0.125, True,
+                   ws.data_ptr(), ws.numel(), stream())
+    capi.sync(stream())
+    got = ob[off:].view(2 * n, ld)
+    assert torch.equal(got[:, :384].reshape(want.shape), want)
+    assert (got[:, 384:] == 9.0).all() and (ob[:off] == 9.0).all()
+
+
+@pytest.mark.parametrize("n", [1, 60])
+def test_two_calls_at_once(cuda_dev, n):
+    """Calls on two streams, each with scratch of its own, give what they give alone."""
+    state = []
+    for i, kv in enumerate((3000, 700)):
+        c = Cache([(n, kv), (1, 200)], 8, 2, 128, 16, seed=i)
+        q, k, v = held_rows(c, i)
+        c.fill(k.cuda(), v.cuda())
+        q = q.cuda()
+        want = c.attend(q, True)
+        capi.sync(stream())
+        ws = torch.empty(max(16, c.kv.attention_workspace(c.batch, 8)), dtype=torch.uint8, device="cuda")
+        state.append((c, q, want, ws, [torch.zeros_like(q) for _ in range(6)], torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for c, q, _, ws, outs, s in state:
+            c.attend(q, True, out=outs[i], st=s.cuda_stream, ws=ws)
+    torch.cuda.synchronize()
+    capi.sync(stream())
+    for _, _, want, _, outs, _ in state:
+        for o in outs:
+            assert torch.equal(o, want)
+
+
 @pytest.mark.parametrize("lens", [[(1, 300), (1, 40)], [(150, 300), (20, 40)]])
 def test_sharp_and_wide_scores(cuda_dev, lens):
     """Scores of hundreds, one key far ahead of the rest, values of tiny and large scales side by side."""
