@@ -379,7 +379,9 @@ int mrt_weight_q4_free(mrt_weight_q4 w);
  * (res_dev FP16 [M, N], row stride ldr, or NULL; y_dev may be res_dev) each
  * added with a rounding, as mrt_gemm and mrt_gemm_residual do.  FP32 y: the
  * sums as they are, without bias or residual.  Any M is right; tokens are
- * taken 16 at a time, each 16 reading the weight once.  No scratch memory.
+ * taken 16 at a time (fewer where K is so long that 16 rows of x leave shared
+ * memory no room), each of these reading the weight once; MRT_ERR_SHAPE where
+ * not even one row fits (K beyond some 400,000).  No scratch memory.
  * An infinity or NaN in a token makes its outputs infinities or NaN. */
 int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, const void* res_dev, int64_t ldr, void* y_dev,
                 int y_dtype, int64_t ldy, int64_t M, unsigned flags, void* stream);
@@ -409,11 +411,13 @@ typedef struct mrt_kv_q4_s* mrt_kv_q4;
  * ld_table + p / page_tokens] holds position p.  The device arrays (INT32) are
  * read when the kernels run, so a captured call can be replayed with other
  * lengths and pages, within the sizes given here.  Rows behind
- * q_start_dev[seqs] and rows at a negative position belong to nobody: they are
- * not read, stored or written.  A sequence with no rows is skipped.  Lengths
- * beyond max_q_len, max_kv_len or tokens, and page numbers outside the cache,
- * are not followed: what needs them is left out, and mrt_sync then returns
- * MRT_ERR_INVALID_ARG.
+ * q_start_dev[seqs] belong to nobody: they are not read, stored or written; nor
+ * does mrt_kv_q4_append or mrt_kv_q4_read touch rows at a negative position
+ * (n > kv_len_dev[b]).  A sequence with no rows is skipped.  Lengths beyond
+ * max_q_len, max_kv_len or tokens, and page numbers outside the cache, are not
+ * followed: such a sequence's rows are left as they were, what needs such a page
+ * is left out (of a sum over it, the result is unspecified), and mrt_sync then
+ * returns MRT_ERR_INVALID_ARG.
  */
 typedef struct mrt_kv_batch {
     int64_t seqs;               /* sequences, at most 65535 */
@@ -455,7 +459,11 @@ int mrt_kv_q4_read(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype, void* k_d
  * kv_len.  q_dev and out_dev [tokens, heads, head_dim] (FP16 or BF16, token
  * strides ldq and ldo; out_dev may be q_dev), heads a multiple of kv_heads,
  * query head h reading kv head h / (heads / kv_heads).  A row that sees no
- * position gives zeros.  ws_dev: scratch of at least the bytes that
+ * position (one at a negative position, when causal) gives zeros.  Sums and
+ * softmax are FP32; probabilities are rounded to FP16 relative to their row's
+ * largest, and where a call has more than 32 rows (max_q_len * heads /
+ * kv_heads) so are the values s (c - z).  MRT_ERR_SHAPE for more rows and keys
+ * than 31 bits number.  ws_dev: scratch of at least the bytes that
  * mrt_kv_q4_attention_workspace says for the same batch sizes (256-byte
  * aligned), the caller's own, so calls with scratch of their own may overlap;
  * its contents need no clearing and mean nothing afterwards.

@@ -263,17 +263,22 @@ __device__ __forceinline__ void store_y(const GemvQ4Args& a, int64_t n, int m, f
 }
 
 // What bounds it: for few tokens the weights' bytes, so every warp keeps up to
-// eight pieces of them under way (two a copy), the first before it waits for the kernel that
-// makes x (with loads into registers, four deep, a warp waited for more than it
-// asked for: 21.5 us for 37888 x 3584 at one token); for 16 tokens, beside them, x
-// from shared memory (eight KB a KB of codes, in FP16).  x is brought in once a
-// CTA, with its group sums, and CTAs stay for all the row tiles they take.
+// eight pieces of them under way (two a copy), the first before it waits for the
+// kernel that makes x (with loads into registers, four deep, a warp waited for
+// more than it asked for: 21.5 us for 37888 x 3584 at one token); and, as much,
+// the instructions that make operands of a piece (about 150 a KB): 16.2 us for
+// 37888 x 3584 at one token (70.5 MB, 4.3 TB/s), 80 for 152064 x 3584 at 16 (286
+// MB, 3.6 TB/s: beside them x from shared memory, eight KB a KB of codes).  Small
+// weights are bound by a launch and x's way into the CTAs: 896 x 896 2.9 us;
+// long sums of several tokens by x in every CTA: 3584 x 18944 at 7, groups of
+// 32, 20 us (40 MB).  x is brought in once a CTA, with its group sums, and CTAs
+// stay for all the row tiles they take.
 //
-// Split.  A multiprocessor holds one CTA of 24 or 16 warps (one or two token
-// tiles), or two or three smaller ones; wk of a CTA's warps share a tile.  Grid x takes the tiles in turn; grid y cuts the columns into
-// slices, one a CTA, whose sums the CTAs of a cluster (1, KS) add through each
-// other's shared memory in slice order, each a part of the rows.  wk and KS by
-// plan_gemv().
+// Split.  A multiprocessor holds one CTA of up to 24 or 16 warps (one or two
+// token tiles), or two or three smaller ones; wk of a CTA's warps share a tile.
+// Grid x takes the tiles in turn; grid y cuts the columns into slices, one a CTA,
+// whose sums the CTAs of a cluster (1, KS) add through each other's shared memory
+// in slice order, each a part of the rows.  Warps, wk and KS by plan_gemv().
 template <int PER, int NT, bool ZEROS>
 __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const GemvQ4Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
