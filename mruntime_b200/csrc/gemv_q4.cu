@@ -35,8 +35,10 @@ namespace mrt {
 
 // How a launch runs (plan_gemv()).
 struct GemvPlan {
-    int warps = 0, wk = 0, ks = 0;  // warps of a CTA, of a tile; slices of K.  0: no such launch
-    int per_sm = 0;                 // CTAs a multiprocessor
+    int warps = 0, tiles = 0, ks = 0;  // warps and tiles of a CTA; slices of K.  0: no such launch
+    int per_sm = 0;                    // CTAs a multiprocessor
+    int share = 0;                     // block pairs of a warp
+    bool joins = false;                // warps share tiles
 };
 constexpr int kMaxTokens = 16;  // of a launch: two token tiles of eight
 
@@ -218,7 +220,8 @@ struct GemvQ4Args {
     const uint16_t* res;
     int64_t ldr;
     int M;
-    int wk;         // warps of a tile (they take its column blocks in turn)
+    int tiles_cta;  // row tiles of a CTA
+    int share;      // block pairs of a warp
     int slice;      // column blocks of a CTA
     int stages;     // pieces that a warp has under way
     int* err_flag;
@@ -230,7 +233,7 @@ constexpr int kSmemMost = 218 * 1024;  // of a multiprocessor's CTAs together
 
 // Shared memory: the warps' rings; x rows of the CTA's columns, 64 bytes apart
 // from a multiple of 128 so that eight rows' reads fall into different banks;
-// their group sums; sums of the warps of a tile.
+// their group sums; two sums a warp of tiles that it shares.
 __host__ __device__ __forceinline__ int x_stride(int slice) { return slice * 256 + 64; }
 __host__ __device__ __forceinline__ int gemv_smem(int M, int slice, int per, int nt, int warps, bool sums, int stages, int piece) {
     return warps * stages * kPair * piece + M * x_stride(slice) + slice * per * nt * 32 + (sums ? 2 * warps * 16 * nt * 32 : 0);
@@ -266,23 +269,28 @@ __device__ __forceinline__ void store_y(const GemvQ4Args& a, int64_t n, int m, f
 // eight pieces of them under way (two a copy), the first before it waits for the
 // kernel that makes x (with loads into registers, four deep, a warp waited for
 // more than it asked for: 21.5 us for 37888 x 3584 at one token); and, as much,
-// the instructions that make operands of a piece (about 150 a KB): 16.2 us for
-// 37888 x 3584 at one token (70.5 MB, 4.3 TB/s), 80 for 152064 x 3584 at 16 (286
-// MB, 3.6 TB/s: beside them x from shared memory, eight KB a KB of codes).  Small
+// the instructions that make operands of a piece (about 150 a KB): 15.9 us for
+// 37888 x 3584 at one token (70.5 MB, 4.4 TB/s), 70 for 152064 x 3584 at 16 (286
+// MB, 4.1 TB/s: beside them x from shared memory, eight KB a KB of codes).  Small
 // weights are bound by a launch and x's way into the CTAs: 896 x 896 2.9 us;
 // long sums of several tokens by x in every CTA: 3584 x 18944 at 7, groups of
-// 32, 20 us (40 MB).  x is brought in once a CTA, with its group sums, and CTAs
+// 32, 18 us (40 MB).  x is brought in once a CTA, with its group sums, and CTAs
 // stay for all the row tiles they take.
 //
-// Split.  A multiprocessor holds one CTA of up to 24 or 16 warps (one or two
-// token tiles), or two or three smaller ones; wk of a CTA's warps share a tile.
-// Grid x takes the tiles in turn; grid y cuts the columns into slices, one a CTA,
-// whose sums the CTAs of a cluster (1, KS) add through each other's shared memory
-// in slice order, each a part of the rows.  Warps, wk and KS by plan_gemv().
+// Split.  A CTA has row tiles next to one another (grid x) and a slice of the
+// columns (grid y); its tiles' block pairs, in order, are dealt to its warps in
+// equal stretches, so that all warps work to the end whatever the shape (with a
+// warp a tile, or a fixed number of warps a tile, 152064 x 3584 took 80 us at 16
+// tokens, 57 at one; now 70 and 50; a small weight's end is 0.2 us longer).  A warp
+// that has a whole tile stores it; the others leave their sums in shared memory
+// (at most two a warp: of the tile it begins in and of the one it ends in),
+// and they are added in order.  Slices' sums the CTAs of a cluster (1, KS) add
+// through each other's shared memory, each a part of the rows.
 template <int PER, int NT, bool ZEROS>
 __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const GemvQ4Args a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t s_full[most_warps(NT)][kMaxStages];
+    __shared__ int2 s_first[32];  // the shared tile that a warp is the first of (-1: none), its pairs of it
     const int warps = blockDim.x >> 5, threads = blockDim.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int stage_bytes = kPair * a.piece;
@@ -290,27 +298,31 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
     uint8_t* xb = smem + warps * a.stages * stage_bytes;
     const int stride = x_stride(a.slice);
     float* xs = reinterpret_cast<float*>(xb + a.M * stride);  // [group of the slice][NT * 8]
-    float* red = xs + a.slice * PER * NT * 8;                 // [2][warp][16][NT * 8]
+    float* red = xs + a.slice * PER * NT * 8;                 // [warp][2][16][NT * 8]
     const int b0 = blockIdx.y * a.slice, nb = min(a.slice, a.blocks - b0);
-    const int wt = warp / a.wk, wi = warp - wt * a.wk, per_cta = warps / a.wk;
-
-    // The warp's pieces, in order: of its tiles the block pairs wi, wi + wk, ..
-    const int pairs = (nb + kPair - 1) / kPair, mine = pairs > wi ? (pairs - wi + a.wk - 1) / a.wk : 0;
-    const int step = gridDim.x * per_cta;
-    // The next pair to fetch (lane 0's).
-    int f_tile = mine > 0 ? blockIdx.x * per_cta + wt : a.tiles, f_block = wi * kPair;
-    const uint8_t* f_src = a.data + (static_cast<int64_t>(f_tile) * a.blocks + b0) * a.piece;
+    // The warp's stretch.  (A last slice that is short counts its tiles' pairs like
+    // the others, so that shares are alike in all CTAs of a cluster.)
+    const int tile_lo = blockIdx.x * a.tiles_cta, here = min(a.tiles_cta, a.tiles - tile_lo);
+    const int pairs = (a.slice + kPair - 1) / kPair, real = (nb + kPair - 1) / kPair;
+    const int total = here * pairs, per = a.share;
+    const int p0 = min(warp * per, total), p1 = min(p0 + per, total);
+    // The next pair to fetch (lane 0's), and its place in its tile.
+    const int t0 = p0 / pairs;
+    int f_p = p0, f_in = p0 - t0 * pairs;
+    const uint8_t* f_src = a.data + (static_cast<int64_t>(tile_lo + t0) * a.blocks + b0) * a.piece;
     auto fetch = [&](int stage) {
-        if (lane != 0 || f_tile >= a.tiles) return;
-        const uint32_t bytes = nb - f_block >= kPair ? stage_bytes : a.piece;
-        mbar_arrive_expect_tx(&s_full[warp][stage], bytes);
-        bulk_load(ring + stage * stage_bytes, f_src + f_block * a.piece, bytes, &s_full[warp][stage]);
-        f_block += a.wk * kPair;
-        if (f_block >= nb) {
-            f_block = wi * kPair;
-            f_tile += step;
-            f_src += static_cast<int64_t>(step) * a.blocks * a.piece;
+        if (lane != 0) return;
+        if (f_in >= real) {
+            f_p += pairs - f_in;
+            f_in = 0;
+            f_src += static_cast<int64_t>(a.blocks) * a.piece;
         }
+        if (f_p >= p1) return;
+        const uint32_t bytes = nb - f_in * kPair >= kPair ? stage_bytes : a.piece;
+        mbar_arrive_expect_tx(&s_full[warp][stage], bytes);
+        bulk_load(ring + stage * stage_bytes, f_src + f_in * stage_bytes, bytes, &s_full[warp][stage]);
+        ++f_p;
+        ++f_in;
     };
     if (lane == 0) {
         for (int i = 0; i < a.stages; ++i) mbar_init(&s_full[warp][i], 1);
@@ -365,20 +377,22 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
     }
     __syncthreads();
 
-    int turn = 0, stage = 0;
+    int stage = 0;
     uint32_t phase = 0;
     bool late = false;
     // Columns past M of a token tile repeat its last token: never stored.
     const uint8_t* x_row[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) x_row[t] = xb + min(t * 8 + r, a.M - 1) * stride + c * 16;
-    for (int tile0 = blockIdx.x * per_cta; tile0 < a.tiles; tile0 += step, turn ^= 1) {
+    int in = p0 - t0 * pairs, tile = tile_lo + t0;
+    int2 first = make_int2(-1, 0);
+    for (int p = p0; p < p1; in = 0, ++tile) {
+        const int count = min(p1 - p, pairs - in);  // of this tile
         uint64_t tot[NT][2];  // rows r and r + 8: tokens 2c, 2c + 1 of a token tile
 #pragma unroll
         for (int t = 0; t < NT; ++t) tot[t][0] = tot[t][1] = 0;
-        const int tile = tile0 + wt;
 #pragma unroll 1
-        for (int b = tile < a.tiles ? wi * kPair : nb; b < nb; b += a.wk * kPair) {
+        for (int b = in * kPair, b1 = min((in + count) * kPair, nb); b < b1; b += kPair) {
             wait_piece(&s_full[warp][stage], phase, a.err_flag, late);
             const uint8_t* piece = ring + stage * stage_bytes;
             uint4 lo[kPair], hi[kPair];
@@ -446,7 +460,7 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
                 }
             }
         }
-        if (a.wk == 1 && gridDim.y == 1) {  // the warp has whole sums
+        if (count == pairs && gridDim.y == 1) {  // the warp has whole sums
             const int64_t n = tile * 16LL + r;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -454,61 +468,74 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
                 for (int j = 0; j < 4; ++j) {
                     const int m = t * 8 + c * 2 + (j & 1);
                     const int64_t row = n + (j >> 1) * 8;
-                    if (tile < a.tiles && m < a.M && row < a.n) store_y(a, row, m, (j & 1) ? high2(tot[t][j >> 1]) : low2(tot[t][j >> 1]));
+                    if (m < a.M && row < a.n) store_y(a, row, m, (j & 1) ? high2(tot[t][j >> 1]) : low2(tot[t][j >> 1]));
                 }
-            continue;
-        }
-        float* part = red + turn * warps * 16 * NT * 8;  // the other turn's may still be read
-        float* p = part + warp * 16 * NT * 8;
+        } else {
+            const int place = p == p0 ? 0 : 1;
+            if (in == 0) first = make_int2(tile * 2 + place, count);
+            float* part = red + (warp * 2 + place) * 16 * NT * 8;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            *reinterpret_cast<uint64_t*>(p + r * NT * 8 + t * 8 + c * 2) = tot[t][0];
-            *reinterpret_cast<uint64_t*>(p + (r + 8) * NT * 8 + t * 8 + c * 2) = tot[t][1];
+            for (int t = 0; t < NT; ++t) {
+                *reinterpret_cast<uint64_t*>(part + r * NT * 8 + t * 8 + c * 2) = tot[t][0];
+                *reinterpret_cast<uint64_t*>(part + (r + 8) * NT * 8 + t * 8 + c * 2) = tot[t][1];
+            }
         }
-        const int rows = per_cta * 16;
-        if (gridDim.y == 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < rows * NT * 8; i += threads) {
-                const int m = i / rows, row = i - m * rows;  // neighbouring threads, neighbouring rows
-                const int64_t n = tile0 * 16LL + row;
-                if (m >= a.M || n >= a.n) continue;
-                const float* q = part + ((row >> 4) * a.wk * 16 + (row & 15)) * NT * 8 + m;
-                float s = 0.0f;
-                for (int w = 0; w < a.wk; ++w) s += q[w * 16 * NT * 8];
-                store_y(a, n, m, s);
+        p += count;
+    }
+    if (gridDim.y == 1 && a.share % pairs == 0) return;  // no tile is shared
+    if (lane == 0) s_first[warp] = first;
+    const int ranks = gridDim.y, rank = blockIdx.y, halves = threads >> 4, row = threadIdx.x & 15;
+    if (ranks == 1) __syncthreads();
+    else cluster_barrier();
+    // Half a warp a (tile, token): the first warp's part, then those of the warps
+    // that begin inside the tile.
+    const uint32_t firsts = __ballot_sync(0xFFFFFFFFu, lane < warps && s_first[lane].x >= 0);
+    constexpr int kPart = 16 * NT * 8;
+    for (int q = rank * halves + (threadIdx.x >> 4);; q += ranks * halves) {
+        uint32_t rest = firsts;
+        int m = q;
+        for (; rest != 0 && m >= a.M; m -= a.M) rest &= rest - 1;
+        if (rest == 0) break;
+        const int w = __ffs(rest) - 1;
+        const int2 f = s_first[w];
+        const int64_t n = (f.x >> 1) * 16LL + row;
+        if (n >= a.n) continue;
+        const float* part = red + (w * 2 + (f.x & 1)) * kPart + row * NT * 8 + m;
+        float s = 0.0f;
+        if (ranks == 1) {
+            s = *part;
+            part = red + (w * 2 + 2) * kPart + row * NT * 8 + m;
+            for (int have = f.y; have < pairs; part += 8 * kPart) {  // four asked for, then added
+                float x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k, have += a.share) x[k] = have < pairs ? part[k * 2 * kPart] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += x[k];
             }
         } else {
-            // Slices of a cluster: this launch has one turn, so nothing is written again.
-            cluster_barrier();
-            const int rank = blockIdx.y, ranks = gridDim.y;
-            for (int i = threadIdx.x + rank * threads; i < rows * NT * 8; i += threads * ranks) {
-                const int m = i / rows, row = i - m * rows;
-                const int64_t n = tile0 * 16LL + row;
-                if (m >= a.M || n >= a.n) continue;
-                const uint32_t at = smem_u32(part + ((row >> 4) * a.wk * 16 + (row & 15)) * NT * 8 + m);
-                float s = 0.0f;
-                for (int w = 0; w < a.wk; ++w) {
-                    float v[8];  // all asked for, then added
+            for (int v = w, have = f.y;; have += a.share) {
+                const uint32_t at = smem_u32(part);
+                float x[8];  // all asked for, then added
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        v[k] = k < ranks ? ld_cluster_f32(cluster_address(at, k) + w * 16 * NT * 8 * 4) : 0.0f;
+                for (int k = 0; k < 8; ++k) x[k] = k < ranks ? ld_cluster_f32(cluster_address(at, k)) : 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) s += v[k];
-                }
-                store_y(a, n, m, s);
+                for (int k = 0; k < 8; ++k) s += x[k];
+                if (have >= pairs) break;
+                part = red + ++v * 2 * kPart + row * NT * 8 + m;
             }
-            cluster_barrier();  // the others have read this CTA's sums
         }
+        store_y(a, n, m, s);
     }
+    if (ranks > 1) cluster_barrier();  // the others have read this CTA's sums
 }
 
 // Candidates by time, in microseconds.  A multiprocessor with all its warps
-// works off a piece in 0.029 us (with four groups in 0.053), a warp alone in
-// 0.38; x comes into every CTA from L2; larger CTAs start later, and joining
+// works off a piece in 0.041 us (with four groups in 0.046), a warp alone in
+// 0.445; x comes into every CTA from L2; larger CTAs start later, and joining
 // sums costs.  The numbers are a fit to every candidate's time for twenty
-// weights, 896 x 896 to 152064 x 3584 at 1 to 16 tokens: the times are told
-// within 13% on average, and the choice costs 2% over the best.
-constexpr int kShares[] = {1, 2, 4, 8, 12, 16, 24};  // warps of a tile
+// weights, 896 x 896 to 152064 x 3584 at 1 to 16 tokens: times are told within
+// 12% on average, and the choice costs 2% over the best.
+constexpr int kWarps[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 20, 24};
 
 GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
     GemvPlan best;
@@ -516,29 +543,28 @@ GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
     const int nt = M <= 8 ? 1 : 2;
     for (int per_sm = nt == 1 ? 3 : 2; per_sm > 0; --per_sm)
         for (int ks = 1; ks <= 8; ks *= 2)
-            for (int c = 0; c < 14; ++c) {
-                // As many warps as fit, or as many as give every CTA one turn's share.
+            for (int warps : kWarps) {
+                const int slice = (blocks + ks - 1) / ks, pairs = (slice + kPair - 1) / kPair;
+                if (warps * per_sm > most_warps(nt) || (ks > 1 && (ks - 1) * slice >= blocks)) continue;
                 // (Clusters of four and eight leave some multiprocessors idle: of 148
                 // they reach 132 and 120.)
-                const int wk = kShares[c >> 1], most = most_warps(nt) / per_sm, slice = (blocks + ks - 1) / ks;
-                const int room_x = std::max(1, sms * per_sm * (ks < 4 ? 16 : (ks == 4 ? 14 : 13)) / (16 * ks));
-                const int warps = (c & 1) ? wk * ((tiles + room_x - 1) / room_x) : most;
-                if (warps > most || warps % wk != 0 || (ks > 1 && (ks - 1) * slice >= blocks) || (wk > 1 && (wk - 1) * kPair >= slice)) continue;
-                if (gemv_smem(M, slice, per, nt, warps, wk * ks > 1, kMinStages, piece) > kSmemMost / per_sm) continue;
-                const int per_cta = warps / wk;
-                const int64_t ctas = static_cast<int64_t>((tiles + per_cta - 1) / per_cta) * ks, room = static_cast<int64_t>(sms) * per_sm;
-                if (ks > 1 && ctas > room_x * ks) continue;  // slices' CTAs take one turn
-                const int64_t turns = (ctas + room - 1) / room, live = std::min(ctas, room);
-                const int warp_pieces = (slice + wk * kPair - 1) / (wk * kPair) * kPair;
+                const int room = std::max(1, sms * per_sm * (ks < 4 ? 16 : (ks == 4 ? 14 : 13)) / (16 * ks));
+                const int64_t tiles_cta = (tiles + room - 1) / room, share = (tiles_cta * pairs + warps - 1) / warps;
+                if (ks > 1 && tiles_cta > warps) continue;  // (a warp keeps two sums)
+                if (tiles_cta * pairs < warps) continue;
+                const bool joins = ks > 1 || share % pairs != 0;
+                if (gemv_smem(M, slice, per, nt, warps, joins, kMinStages, piece) > kSmemMost / per_sm) continue;
+                const int64_t ctas = (tiles + tiles_cta - 1) / tiles_cta * ks;
                 // of the busiest multiprocessor, of all of them
-                const double busiest = static_cast<double>((live + sms - 1) / sms) * turns * per_cta * slice;
+                const double busiest = static_cast<double>((ctas + sms - 1) / sms) * tiles_cta * slice;
                 const double mean = static_cast<double>(tiles) * blocks / sms;
-                const double a_piece = (per == 4 ? 0.053 : 0.029) * (nt == 1 ? 1.0 : 1.4) * (0.86 + 0.14 * most_warps(nt) / (warps * per_sm));
-                const double work = std::max((0.43 * busiest + 0.57 * mean) * a_piece, std::max(1.0, mean / (per_sm * per_cta * slice)) * warp_pieces * 0.38);
-                const double x = live * 256.0 / 7.6e6 * M * slice + M * slice * 16.0 / (warps * 32) * 0.045;
-                const double us = work + x + 0.032 * warps + (wk > 1 ? 0.46 * turns : 0.0) + (ks > 1 ? 1.5 : 0.0);
-                if (best.wk == 0 || us < best_us) {
-                    best = GemvPlan{warps, wk, ks, per_sm};
+                const double a_piece = (per == 4 ? 0.0463 : 0.0407) * (nt == 1 ? 1.0 : 1.73) * (0.942 + 0.058 * most_warps(nt) / (warps * per_sm));
+                const double work = std::max((0.797 * busiest + 0.203 * mean) * a_piece, share * kPair * 0.445);
+                const double x = ctas * 256.0 / 11.8e6 * M * slice + M * slice * 16.0 / (warps * 32) * 0.0843;
+                const double parts = share < pairs ? std::min<double>(warps, static_cast<double>(pairs) / share) : 1.0;  // of a tile
+                const double us = work + x + 0.0574 * warps + (joins ? 0.3 + 0.04 * parts : 0.0) + (ks > 1 ? 2.05 + 0.029 * ks : 0.0);
+                if (best.warps == 0 || us < best_us) {
+                    best = GemvPlan{warps, static_cast<int>(tiles_cta), ks, per_sm, static_cast<int>(share), joins};
                     best_us = us;
                 }
             }
@@ -546,16 +572,15 @@ GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
 }
 
 template <int PER, int NT, bool ZEROS>
-cudaError_t launch(GemvQ4Args a, const GemvPlan& p, int sms, cudaStream_t s) {
+cudaError_t launch(GemvQ4Args a, const GemvPlan& p, cudaStream_t s) {
     a.stages = kMaxStages;
-    auto bytes = [&] { return gemv_smem(a.M, a.slice, PER, NT, p.warps, p.wk * p.ks > 1, a.stages, a.piece); };
+    auto bytes = [&] { return gemv_smem(a.M, a.slice, PER, NT, p.warps, p.joins, a.stages, a.piece); };
     while (bytes() > kSmemMost / p.per_sm) --a.stages;
     if (a.stages < kMinStages) return cudaErrorInvalidValue;  // (the plan says that they fit)
     cudaError_t e = prepare_kernel<gemv_q4_kernel<PER, NT, ZEROS>>(kSmemMost);
     if (e != cudaSuccess) return e;
-    const int per_cta = p.warps / p.wk, ctas = (a.tiles + per_cta - 1) / per_cta;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.ks > 1 ? ctas : std::min(ctas, sms * p.per_sm)), static_cast<unsigned>(p.ks));
+    cfg.gridDim = dim3(static_cast<unsigned>((a.tiles + p.tiles - 1) / p.tiles), static_cast<unsigned>(p.ks));
     cfg.blockDim = dim3(static_cast<unsigned>(p.warps) * 32);
     cfg.dynamicSmemBytes = static_cast<size_t>(bytes());
     cfg.stream = s;
@@ -577,21 +602,22 @@ cudaError_t launch(GemvQ4Args a, const GemvPlan& p, int sms, cudaStream_t s) {
 // memory (0: not even one does).
 int tokens_at_once(const mrt_weight_q4_s* w, int64_t M) {
     int m = static_cast<int>(std::min<int64_t>(M, kMaxTokens));
-    while (m > 0 && w->plans[m].wk == 0) m = m > 8 ? 8 : m / 2;
+    while (m > 0 && w->plans[m].warps == 0) m = m > 8 ? 8 : m / 2;
     return m;
 }
 
-cudaError_t launch_gemv_q4(GemvQ4Args a, const GemvPlan& p, int per, int sms, cudaStream_t s) {
-    a.wk = p.wk;
+cudaError_t launch_gemv_q4(GemvQ4Args a, const GemvPlan& p, int per, cudaStream_t s) {
+    a.tiles_cta = p.tiles;
+    a.share = p.share;
     a.slice = (a.blocks + p.ks - 1) / p.ks;
     const bool z = a.zeros != 0;
     switch (per * 2 + (a.M > 8)) {
-        case 2: return z ? launch<1, 1, true>(a, p, sms, s) : launch<1, 1, false>(a, p, sms, s);
-        case 3: return z ? launch<1, 2, true>(a, p, sms, s) : launch<1, 2, false>(a, p, sms, s);
-        case 4: return z ? launch<2, 1, true>(a, p, sms, s) : launch<2, 1, false>(a, p, sms, s);
-        case 5: return z ? launch<2, 2, true>(a, p, sms, s) : launch<2, 2, false>(a, p, sms, s);
-        case 8: return z ? launch<4, 1, true>(a, p, sms, s) : launch<4, 1, false>(a, p, sms, s);
-        default: return z ? launch<4, 2, true>(a, p, sms, s) : launch<4, 2, false>(a, p, sms, s);
+        case 2: return z ? launch<1, 1, true>(a, p, s) : launch<1, 1, false>(a, p, s);
+        case 3: return z ? launch<1, 2, true>(a, p, s) : launch<1, 2, false>(a, p, s);
+        case 4: return z ? launch<2, 1, true>(a, p, s) : launch<2, 1, false>(a, p, s);
+        case 5: return z ? launch<2, 2, true>(a, p, s) : launch<2, 2, false>(a, p, s);
+        case 8: return z ? launch<4, 1, true>(a, p, s) : launch<4, 1, false>(a, p, s);
+        default: return z ? launch<4, 2, true>(a, p, s) : launch<4, 2, false>(a, p, s);
     }
 }
 
@@ -827,7 +853,7 @@ extern "C" int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, cons
         a.x = static_cast<const uint16_t*>(x_dev) + m * ldx;
         a.y = static_cast<uint8_t*>(y_dev) + m * ldy * (a.out_f32 ? 4 : 2);
         a.res = res_dev != nullptr ? static_cast<const uint16_t*>(res_dev) + m * ldr : nullptr;
-        const cudaError_t e = launch_gemv_q4(a, w->plans[a.M], per, c->sms, static_cast<cudaStream_t>(stream));
+        const cudaError_t e = launch_gemv_q4(a, w->plans[a.M], per, static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) return cuda_error(e, "4-bit gemv launch");
     }
     return MRT_OK;

@@ -257,20 +257,23 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
         at = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(blockIdx.x) * per));
         end = min(total - at, per) + at;
         if (at >= end) return;
-        for (int b0 = 0, before = 0;;) {  // ends: at < total
+        if (threadIdx.x == 0) s_seq = -1;
+        __syncthreads();
+        for (int b0 = 0, before = 0;;) {
             const int lo = before + base + incl - t;
             if (at >= lo && at < lo + t) {
                 s_seq = b0 + threadIdx.x;
                 s_at = lo;
             }
             before += chunk;
-            if (at < before) break;
             b0 += W * 32;
+            if (at < before || b0 >= v.seqs) break;
             scan(b0);
         }
         __syncthreads();
         u.seq = s_seq;
         seq_at = s_at;
+        if (u.seq < 0) return;  // (never, unless the lengths are written meanwhile)
         u.tiles = seq_tiles(v, u.seq);
     } else {
         u.seq = blockIdx.x / v.kv_heads;
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
             int places;
             while (at >= seq_at + (places = unit_places(u.tiles, kCost)) * v.kv_heads) {
                 seq_at += places * v.kv_heads;
-                ++u.seq;
+                if (++u.seq >= v.seqs) return false;
                 u.tiles = seq_tiles(v, u.seq);
             }
             u.head = (at - seq_at) / places;
@@ -518,9 +521,10 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 
 #pragma unroll
                             for (int j = 0; j < 2; ++j)
                                 if (pos + r >= s_limit[t * 8 + c * 2 + j]) y[h][t][half * 2 + j] = -INFINITY;
-                        // nobody's: bytes of any kind
-                        if (pos + 2 * c >= u.kv) z[h][half] &= 0xFFFF0000u;
-                        if (pos + 2 * c + 1 >= u.kv) z[h][half] &= 0x0000FFFFu;
+                        // (of tokens and pages that are nobody's: bytes of any kind)
+                        const __half2 zz = __hmin2(__hmax2(*reinterpret_cast<const __half2*>(&z[h][half]), __float2half2_rn(0.0f)),
+                                                   __float2half2_rn(15.0f));
+                        z[h][half] = *reinterpret_cast<const uint32_t*>(&zz);
                     }
             }
             bool far = false;
@@ -1096,8 +1100,10 @@ struct ManyWalk {
                 x = 0;
                 if (++head == g.a.v.kv_heads) {
                     head = 0;
-                    do many_seq(g, ++seq, &sq);
-                    while (sq.count == 0);
+                    do {
+                        if (++seq >= g.a.v.seqs) return false;
+                        many_seq(g, seq, &sq);
+                    } while (sq.count == 0);
                 }
             }
             tiles = sq.tiles(x);
@@ -1232,16 +1238,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     walk.end = walk.at + min(total - walk.at, per);
     walk.head = walk.x = walk.unit_at = 0;
     if (walk.at < walk.end) {
+        if (threadIdx.x == 0) s_seq = 0;
+        __syncthreads();
 #pragma unroll 1
-        for (int b0 = 0, before = 0;;) {  // ends: walk.at < total
+        for (int b0 = 0, before = 0;;) {
             if (walk.at >= before + lo && walk.at < before + lo + t) {
                 s_seq = b0 + threadIdx.x;
                 s_at = before + lo;
                 s_tiles = t / v.kv_heads;
             }
             before += chunk;
-            if (walk.at < before) break;
             b0 += kManyThreads;
+            if (walk.at < before || b0 >= v.seqs) break;
             scan(b0);
         }
         __syncthreads();

@@ -590,6 +590,20 @@ def test_bad_pages_and_lengths_are_reported(cuda_dev):
     assert torch.equal(again, good)
 
 
+@pytest.mark.parametrize("n,kv,H", [(3, 33, 4), (3, 33, 8), (40, 49, 4)])
+def test_a_bad_page_spoils_no_row_that_does_not_need_it(cuda_dev, n, kv, H):
+    """The newest token's page is none of the cache: earlier rows do not see it."""
+    c = Cache([(n, kv)], H, 2, 64, 16, seed=4)
+    q, k, v = held_rows(c, 4)
+    good = check_attention(c, q, k, v, True)
+    c.table[0, kv // 16] = 10 ** 6
+    out = c.attend(q.cuda(), True)
+    with pytest.raises(capi.MrtError):
+        capi.sync(stream())
+    sees = torch.arange(kv - n, kv) >= kv // 16 * 16
+    assert torch.equal(out[~sees.cuda()], good[~sees.cuda()])
+
+
 def test_refusals(cuda_dev):
     c = Cache([(1, 20)], 4, 2, 64, 16)
     t = torch.zeros(4096, dtype=torch.float16, device="cuda")
