@@ -269,7 +269,7 @@ __device__ __forceinline__ void store_y(const GemvQ4Args& a, int64_t n, int m, f
 // eight pieces of them under way (two a copy), the first before it waits for the
 // kernel that makes x (with loads into registers, four deep, a warp waited for
 // more than it asked for: 21.5 us for 37888 x 3584 at one token); and, as much,
-// the instructions that make operands of a piece (about 150 a KB): 15.9 us for
+// the instructions that make operands of a piece (about 140 a KB): 15.9 us for
 // 37888 x 3584 at one token (70.5 MB, 4.4 TB/s), 70 for 152064 x 3584 at 16 (286
 // MB, 4.1 TB/s: beside them x from shared memory, eight KB a KB of codes).  Small
 // weights are bound by a launch and x's way into the CTAs: 896 x 896 2.9 us;
