@@ -371,6 +371,19 @@ def test_attention_strides(cuda_dev, n, off, pad):
     assert (got[:, 384:] == 9.0).all() and (ob[:off] == 9.0).all()
 
 
+@pytest.mark.parametrize("n", [1, 24])
+def test_sequences_share_a_prefix(cuda_dev, n):
+    """Two sequences whose first pages are the same ones read what each held alone."""
+    c = Cache([(n, 100), (n, 80)], 8, 2, 64, 16, seed=6)
+    q, k, v = held_rows(c, 6)
+    k[100:148], v[100:148] = k[:48], v[:48]
+    want = check_attention(c, q, k, v, True)
+    c.table[1, :3] = c.table[0, :3]
+    out = c.attend(q.cuda(), True)
+    capi.sync(stream())
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("n", [1, 60])
 def test_two_calls_at_once(cuda_dev, n):
     """Calls on two streams, each with scratch of its own, give what they give alone."""
