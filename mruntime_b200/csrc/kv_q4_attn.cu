@@ -71,10 +71,10 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // the same rounded p'), is one more row of the second product.
 //
 // What bounds it: bytes and instructions alike.  64 sequences of up to 8192
-// tokens (176 MB, 7 of 8 rows used) take 42 us where the bytes would take 27 at
+// tokens (176 MB, 7 of 8 rows used) take 41 us where the bytes would take 27 at
 // the copy's rate: 406 instructions a warp and tile, half of them the masks that
 // make operands of codes, would take 17, and beginning, joining and the CTAs'
-// uneven ends 9.  One of 131071 tokens (70 MB) takes 23 us for 11: 4 until the
+// uneven ends 9.  One of 131071 tokens (70 MB) takes 22 us for 11: 4 until the
 // first tile is there, 13 for the tiles, 5 for the parts.
 //
 // Split.  The 32-token tiles of all (sequence, kv head) units, in order, are
@@ -190,7 +190,7 @@ __device__ __forceinline__ float max_nan(float x, float y) {
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 template <int D, int NT, int W>
-__global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 4 : (NT == 2 ? 3 : 2))) attn_q4_few_kernel(const RowsArgs args) {
+__global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 3 : 2)) attn_q4_few_kernel(const RowsArgs args) {
     using S = RowsShape<D, NT, W>;
     constexpr int kWords = D / 32;               // words of a lane: K row part, and V channel stretch of two tokens
     // q is laid out eight channels a lane: lanes of a row, rows of a pass, passes.
@@ -1813,9 +1813,11 @@ Plan make_plan(const KvView& v, int64_t heads, int sms) {
     // against 6.7 split, 8 x 1000 7.6 against 12.6; but 1 x 2000 10.2 against 7.5).
     const int64_t units = static_cast<int64_t>(v.seqs) * v.kv_heads;
     p.split = !(v.max_kv_len <= kWholeWarps * 2 * kTile && units <= sms && p.few <= 2);
-    // As many CTAs of four warps as registers and shared memory have room for (four:
-    // 64 x 8192 tokens 41.4 us; two of eight warps 43.9).
-    p.grid = p.split ? sms * (p.few == 1 ? 4 : (p.few == 2 ? 3 : 2)) : static_cast<int>(units);
+    // Three CTAs of four warps a multiprocessor (64 x 8192 tokens 41.0 us, 1 x 131071
+    // 21.6; four, 41.3 and 22.9; two of eight warps 43.9 and 22.4), two where rows take
+    // the registers (14 rows, 64 x 8192 58.6 us and 9 x 6000 15.6; three, which spill,
+    // 61.9 and 19.1).
+    p.grid = p.split ? sms * (p.few == 1 ? 3 : 2) : static_cast<int>(units);
     if (p.split) {
         p.o_bytes = static_cast<size_t>(p.grid) * 2 * p.few * 8 * v.head_dim * 4;
         p.ml_bytes = static_cast<size_t>(p.grid) * 2 * p.few * 8 * 8;
@@ -1847,7 +1849,7 @@ cudaError_t launch_few_w(const RowsArgs& r, int rows, cudaStream_t s) {
     cudaError_t e = launch_pdl<attn_q4_few_kernel<D, NT, W>>(dim3(r.grid), W * 32, RowsShape<D, NT, W>::kBytes, s, r);
     if (e != cudaSuccess || !r.split) return e;
     const dim3 grid(r.a.v.seqs * r.a.v.kv_heads, rows);  // a CTA a (unit, row)
-    // Units of 24 parts and more are worth a large CTA: 1 x 131071 tokens (148 parts)
+    // Units of 24 parts and more are worth a large CTA (of 592 parts in all): 1 x 131071 tokens (148 parts)
     // 22.8 us against 33.9, 4 x 30000 (37) 18.1 against 23.7; 8 x 4000 (18) 14.0
     // against 11.5, 16 x 4000 (9) 20.7 against 14.5.
     return static_cast<int64_t>(grid.x) * 24 <= r.grid ? launch_pdl<attn_q4_join_kernel<D, 512>>(grid, 512, 0, s, r, NT * 8)
