@@ -1578,6 +1578,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 if (j + 2 < count) fetch(j + 2);
             }
             stage_it += count;
+            __syncwarp();  // (no tile of the unit may be this group's: every lane has read it all the same)
             if (lane == 0) mbar_arrive(&s_unit_empty[n % kUnits]);
         }
     } else if (warp < kSoftmaxWarps + kCodesWarps + 4) {

@@ -332,6 +332,25 @@ def test_many_short_sequences(cuda_dev, seqs, n_max, H, Hk):
     check_attention(c, *held_rows(c, seqs), True)
 
 
+@pytest.mark.parametrize("D,causal", [(64, True), (128, False)])
+def test_many_units_of_one_key_tile(cuda_dev, D, causal):
+    """More units a CTA than are published ahead, each of one key tile: half of the operand warps have no tile of
+    a unit and meet the next one at once.  More than 32 rows, so that no other kernel takes them."""
+    g = torch.Generator().manual_seed(D)
+    lens = []
+    for b in range(400):
+        kv = int(torch.randint(1, 65, (1,), generator=g))
+        lens.append((min(kv, 1 + b % 7 * 5), kv))
+    c = Cache(lens, 6, 3, D, 16, seed=D)
+    q, k, v = held_rows(c, D)
+    out = check_attention(c, q, k, v, causal)
+    qd = q.cuda()
+    for _ in range(20):
+        again = c.attend(qd, causal)
+        capi.sync(stream())
+        assert torch.equal(again, out)
+
+
 @pytest.mark.parametrize("seed", range(10))
 def test_random_batches(cuda_dev, seed):
     """Stretches that begin and end anywhere in sequences of any length."""
