@@ -1658,55 +1658,57 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             }
         }
         __syncwarp();
-    } else if (warp < kManyWarps - 1) {
-        // -------------------------------------------------------------- Q, as it is
-        registers_down<kOtherRegs>();
-        const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.ldq & 7) == 0;
-        const int tid = threadIdx.x - (kManyThreads - 128), ch = tid & (D / 8 - 1);
-        for (uint32_t n = 0;; ++n) {
-            const ManyUnit& u = s_unit[n % kUnits];
-            wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
-            if (u.count == 0) break;
-            if (n > 0) wait_phase(&s_q_free, (n - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
-            const uint16_t* q0 = a.q + (u.first + u.tok0) * a.ldq + u.head * args.group * D + ch * 8;
-#pragma unroll 2
-            for (int row = tid / (D / 8); row < u.row_tiles() * 128; row += kLoaders / (D / 8)) {
-                const uint32_t dst = panel_at(q_u32 + ((row >> 7) * kPanels + (ch >> 3)) * S::kPanel, row & 127, ch & 7);
-                const bool live = row < u.rows;
-                const int x = live ? u.head0 + row : 0, dt = args.group_magic != 0 ? __umulhi(x, args.group_magic) : x;
-                const uint16_t* src = q0 + dt * a.ldq + (x - dt * args.group) * D;
-                if (vec) {
-                    copy_async_16(dst, src, live);
-                } else {
-                    const uint4 w = live ? load8(src, false) : make_uint4(0, 0, 0, 0);
-                    st_shared_16(dst, w.x, w.y, w.z, w.w);
-                }
-            }
-            copy_async_commit();
-            copy_async_wait<0>();
-            fence_async_smem();
-            mbar_arrive(&s_q);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_unit_empty[n % kUnits]);
-        }
     } else {
-        // -------------------------------------------------------------- the walk
+        // (Before the roles part: the four warps of a group give up registers with one instruction.)
         registers_down<kOtherRegs>();
-        if (lane == 0) {
-            ManyPart part{0, 0, 0, 0, -1};
-            bool more = true;
-            for (uint32_t n = 0; more; ++n) {
-                if (n >= kUnits)
-                    wait_phase(&s_unit_empty[n % kUnits], (n / kUnits - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
-                ManyUnit& u = s_unit[n % kUnits];
-                more = walk.next(args, &u);
-                if (more && u.t0 == 0 && !u.whole)
-                    part = ManyPart{u.seq, u.head, u.row0, u.place, (walk.unit_at + kManyCost + walk.tiles - 1) / per};
-                mbar_arrive(&s_unit_full[n % kUnits]);
+        if (warp < kManyWarps - 1) {
+            // ---------------------------------------------------------- Q, as it is
+            const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.ldq & 7) == 0;
+            const int tid = threadIdx.x - (kManyThreads - 128), ch = tid & (D / 8 - 1);
+            for (uint32_t n = 0;; ++n) {
+                const ManyUnit& u = s_unit[n % kUnits];
+                wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+                if (u.count == 0) break;
+                if (n > 0) wait_phase(&s_q_free, (n - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+                const uint16_t* q0 = a.q + (u.first + u.tok0) * a.ldq + u.head * args.group * D + ch * 8;
+#pragma unroll 2
+                for (int row = tid / (D / 8); row < u.row_tiles() * 128; row += kLoaders / (D / 8)) {
+                    const uint32_t dst = panel_at(q_u32 + ((row >> 7) * kPanels + (ch >> 3)) * S::kPanel, row & 127, ch & 7);
+                    const bool live = row < u.rows;
+                    const int x = live ? u.head0 + row : 0, dt = args.group_magic != 0 ? __umulhi(x, args.group_magic) : x;
+                    const uint16_t* src = q0 + dt * a.ldq + (x - dt * args.group) * D;
+                    if (vec) {
+                        copy_async_16(dst, src, live);
+                    } else {
+                        const uint4 w = live ? load8(src, false) : make_uint4(0, 0, 0, 0);
+                        st_shared_16(dst, w.x, w.y, w.z, w.w);
+                    }
+                }
+                copy_async_commit();
+                copy_async_wait<0>();
+                fence_async_smem();
+                mbar_arrive(&s_q);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_unit_empty[n % kUnits]);
             }
-            args.parts[blockIdx.x] = part;
+        } else {
+            // ---------------------------------------------------------- the walk
+            if (lane == 0) {
+                ManyPart part{0, 0, 0, 0, -1};
+                bool more = true;
+                for (uint32_t n = 0; more; ++n) {
+                    if (n >= kUnits)
+                        wait_phase(&s_unit_empty[n % kUnits], (n / kUnits - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+                    ManyUnit& u = s_unit[n % kUnits];
+                    more = walk.next(args, &u);
+                    if (more && u.t0 == 0 && !u.whole)
+                        part = ManyPart{u.seq, u.head, u.row0, u.place, (walk.unit_at + kManyCost + walk.tiles - 1) / per};
+                    mbar_arrive(&s_unit_full[n % kUnits]);
+                }
+                args.parts[blockIdx.x] = part;
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
     // Every product has ended: each softmax waited for the last one of its tile.
     tc_fence_before();
