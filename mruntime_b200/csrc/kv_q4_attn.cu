@@ -869,10 +869,11 @@ __device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
 }
 
 // Wait for a phase, bounded: after kWaitLimitNs, or once another thread of the
-// CTA has given up, the wait ends, and the kernel runs on to its end without
-// waiting (every access stays in bounds whatever was computed).  Unlike
-// mbar_wait it does not look at the device's error flag: a bad page of one
-// sequence must not end another's waits.
+// CTA has given up, the wait ends.  The unit under way is then run through
+// without waiting (every access stays in bounds whatever was computed), and each
+// role leaves where it would begin the next one: a unit that was not waited for
+// may be anything.  Unlike mbar_wait it does not look at the device's error flag:
+// a bad page of one sequence must not end another's waits.
 __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volatile int* gave_up, int* flag, int code) {
     uint64_t t0 = 0;
 #pragma unroll 1
@@ -888,6 +889,9 @@ __device__ __forceinline__ void wait_phase(uint64_t* bar, uint32_t parity, volat
     }
 }
 
+__device__ __forceinline__ bool gave_up(const volatile int* flag) { return *flag != 0; }
+// The same answer for all lanes.
+__device__ __forceinline__ bool warp_gave_up(const volatile int* flag) { return __any_sync(0xFFFFFFFFu, *flag != 0); }
 
 // Many rows (prompts, chunks of prompts): tcgen05 flash attention.  A CTA
 // takes 256 rows of a (sequence, kv head) -- new tokens times the query heads
@@ -1153,7 +1157,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
     // s_scores: S; s_probs: P; s_done: the product that used it.  s_free: O has
     // been read.  s_q, s_q_free: Q.
     __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_scores[2][2], s_probs[2][2], s_done[2][2], s_free[2], s_q, s_q_free;
-    __shared__ uint64_t s_unit_full[kUnits], s_unit_empty[kUnits];
+    __shared__ uint64_t s_unit_full[kUnits], s_unit_empty[kUnits], s_drain[4];
     __shared__ ManyUnit s_unit[kUnits];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up, s_seq, s_at, s_tiles, s_sum[kManyWarps];
@@ -1177,6 +1181,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             }
             mbar_init(&s_free[i], 8);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(&s_drain[i], 1);
         for (int i = 0; i < kUnits; ++i) {
             mbar_init(&s_unit_full[i], 1);
             mbar_init(&s_unit_empty[i], kManyWarps - 1);  // each warp but the walker's
@@ -1291,6 +1296,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
         for (uint32_t n = 0;; ++n) {
             const ManyUnit& u = s_unit[n % kUnits];
             wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+            if (warp_gave_up(&s_gave_up)) break;
             const int count = u.count;
             if (count == 0) break;
             if (i < u.row_tiles()) {
@@ -1461,6 +1467,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
         for (uint32_t n = 0;; ++n) {
             const ManyUnit& u = s_unit[n % kUnits];
             wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrEpiWait);
+            if (warp_gave_up(&s_gave_up)) break;
             const int count = u.count;
             if (count == 0) break;
             const int32_t* row_table = v.table + static_cast<int64_t>(u.seq) * v.ld_table;
@@ -1591,6 +1598,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             for (uint32_t n = 0;; ++n) {
                 const ManyUnit& u = s_unit[n % kUnits];
                 wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                if (gave_up(&s_gave_up)) break;
                 const int count = u.count, row_tiles = u.row_tiles();
                 mbar_arrive(&s_unit_empty[n % kUnits]);
                 if (count == 0) break;
@@ -1625,6 +1633,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             for (uint32_t n = 0;; ++n) {
                 const ManyUnit& u = s_unit[n % kUnits];
                 wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrMmaWait);
+                if (gave_up(&s_gave_up)) break;
                 const int count = u.count, row_tiles = u.row_tiles();
                 mbar_arrive(&s_unit_empty[n % kUnits]);
                 if (count == 0) break;
@@ -1657,6 +1666,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 stage_it += count;
             }
         }
+        if (lane == 0) {  // TMEM is freed and shared memory given up once all that this thread asked for has ended
+            tc_commit(&s_drain[warp & 3]);
+            mbar_wait(&s_drain[warp & 3], 0, nullptr, kErrDrainWait);
+        }
         __syncwarp();
     } else {
         // (Before the roles part: the four warps of a group give up registers with one instruction.)
@@ -1668,7 +1681,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             for (uint32_t n = 0;; ++n) {
                 const ManyUnit& u = s_unit[n % kUnits];
                 wait_phase(&s_unit_full[n % kUnits], (n / kUnits) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
-                if (u.count == 0) break;
+                if (warp_gave_up(&s_gave_up) || u.count == 0) break;
                 if (n > 0) wait_phase(&s_q_free, (n - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
                 const uint16_t* q0 = a.q + (u.first + u.tok0) * a.ldq + u.head * args.group * D + ch * 8;
 #pragma unroll 2
@@ -1699,6 +1712,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                 for (uint32_t n = 0; more; ++n) {
                     if (n >= kUnits)
                         wait_phase(&s_unit_empty[n % kUnits], (n / kUnits - 1) & 1, &s_gave_up, v.err_flag, kErrTmaWait);
+                    if (gave_up(&s_gave_up)) break;
                     ManyUnit& u = s_unit[n % kUnits];
                     more = walk.next(args, &u);
                     if (more && u.t0 == 0 && !u.whole)
@@ -1710,7 +1724,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
             __syncwarp();
         }
     }
-    // Every product has ended: each softmax waited for the last one of its tile.
     tc_fence_before();
     __syncthreads();
     if (warp == kSoftmaxWarps + kCodesWarps) tmem_dealloc(tmem, 512);
