@@ -393,8 +393,10 @@ int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, const void* res
  * any order.  A (token, kv head) row of head_dim channels (64 or 128) has one
  * FP16 scale s and one zero point z: with lo = min(0, min x) and hi = max(0,
  * max x), s = max(fp16((hi - lo) / 15), 2^-24), z = rint(-lo / s), c =
- * rint(x / s) + z (both kept in 0..15); the row holds s (c - z).  A row with a
- * NaN, or a magnitude above 65504 once rotated, reads back as NaN.  The
+ * rint(x / s) + z (both kept in 0..15); the row holds s (c - z).  Where s
+ * max(z, 15 - z) would exceed 65504, s is lowered to the largest FP16 with which
+ * it does not (before c is found), so every held value is finite in FP16.  A row
+ * with a NaN, or a magnitude above 65504 once rotated, reads back as NaN.  The
  * handle owns the pages (pages * page_tokens * kv_heads * (head_dim + 8)
  * bytes, zero at first); page_tokens is a multiple of 16.  rope_theta is that
  * of the position rotation (pairs i, i + head_dim / 2 turned by position *

@@ -5,7 +5,10 @@
 // Every (token, head) row of D channels has one scale and one zero point:
 //   lo = min(0, min x), hi = max(0, max x)
 //   s  = max(fp16((hi - lo) / 15), 2^-24),  z = rint(-lo / s),  c = rint(x / s) + z
-// (both clamped to 0..15), and holds the values s (c - z).  One scale a row
+// (both clamped to 0..15), and holds the values s (c - z).  Where codes could so
+// mean more than FP16 holds (s max(z, 15 - z) > 65504: a row that reaches beyond
+// 60000), s is then lowered until they do not: all held values are finite as
+// FP16 operands, and a token that a row does not see adds 0 times a number.  One scale a row
 // rather than one for every 32 channels: the attention kernel then multiplies
 // a key's scale into one score and a value's into one probability, and the
 // codes go to the tensor cores untouched.
@@ -281,8 +284,13 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a,
             continue;
         }
         uint16_t sb = __half_as_ushort(__float2half_rn(fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), 5.9604644775390625e-8f)));
-        const float inv = __frcp_rn(__half2float(__ushort_as_half(sb)));
+        float inv = __frcp_rn(__half2float(__ushort_as_half(sb)));
         float zero = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
+        const float most = fmaxf(zero, 15.0f - zero);  // a code's distance from the zero point
+        if (__half2float(__ushort_as_half(sb)) * most > 65504.0f) {
+            sb = __half_as_ushort(__float2half_rd(__fdiv_rd(65504.0f, most)));
+            inv = __frcp_rn(__half2float(__ushort_as_half(sb)));
+        }
         uint32_t w0 = codes8(x0, inv, static_cast<int>(zero), is_v), w1 = codes8(x1, inv, static_cast<int>(zero), is_v);
         if (odd) {  // no scale says what the row holds: it reads back as NaN
             w0 = w1 = 0;

@@ -206,6 +206,89 @@ def test_append_strides_in_place(cuda_dev, ldq, off):
         assert torch.equal(x, y)
 
 
+# (lowest, highest) channel of rows whose codes could mean more than FP16 holds
+WIDE = [(-2000.0, 65504.0), (-60000.0, 65504.0), (-65504.0, 60000.0), (-60000.0, 63000.0), (0.0, 65504.0),
+        (-65504.0, 0.0), (-65504.0, 65504.0), (-500.0, 65504.0)]
+
+
+def wide_rows(n, heads, D, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.zeros(n, heads, D)
+    for i in range(n):
+        lo, hi = WIDE[i % len(WIDE)]
+        x[i] = lo + (hi - lo) * torch.rand(heads, D, generator=g)
+        x[i, :, i % D], x[i, :, (i + 7) % D] = lo, hi
+    return x.half()
+
+
+def held_finite(x):
+    """quantised() with the scale lowered until every code's value is a finite FP16."""
+    lo, hi = x.amin(-1, keepdim=True).clamp(max=0), x.amax(-1, keepdim=True).clamp(min=0)
+    s = ((hi - lo) * torch.tensor(1.0 / 15.0)).half().float().clamp(min=2.0 ** -24)
+    z = torch.round(-lo * (1.0 / s)).clamp(0, 15)
+    most = torch.maximum(z, 15 - z)
+    low = (65504.0 / most).half()  # the largest FP16 below: one less where this rounded up
+    low = torch.where(low.double() * most.double() > 65504, torch.nextafter(low, torch.zeros_like(low)), low).float()
+    s = torch.where(s * most > 65504, low, s)
+    c = (torch.round(x * (1.0 / s)) + z).clamp(0, 15)
+    return (c - z).double() * s.double(), s.double()
+
+
+def test_wide_rows_in_the_oracle_are_finite_and_near():
+    x = wide_rows(64, 2, 64, 1).float()
+    v, _ = held_finite(x)
+    assert float(v.abs().max()) <= 65504
+    # In steps s before it is lowered, to s': the near end n = 15 - z steps away, n s > 65504 >= hi, n >= 8 > z (s < 8736).
+    # The far end is off by z's rounding, 1/2, and z (s - s').  n s - hi = n s - range - lo <= (1/2 + 15 2^-11) s, as
+    # range >= 15 s (1 - 2^-11) and -lo <= (z + 1/2) s; s' is FP16, 2^-10 of itself less at most; z / n <= 7 / 8.
+    old, s = quantised(x)
+    assert ((v - x).abs() / s).max() <= 0.5 + 7 / 8 * (0.5 + 15 * 2.0 ** -11) + 7 * 2.0 ** -10
+    assert float(old.abs().max()) > 65520  # without it they are not
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_wide_rows_are_held_in_fp16(cuda_dev, D):
+    """Magnitudes up to 65504 are taken; what they read back as is finite and within a step."""
+    c = Cache([(40, 40)], 2, 2, D, 16, seed=2)
+    k, v = wide_rows(40, 2, D, 1), wide_rows(40, 2, D, 2)
+    c.append(c.batch, k.cuda(), v.cuda())
+    for x, got in zip((k, v), c.read(c.batch)):
+        assert torch.isfinite(got).all()
+        assert torch.equal(got, held_finite(x.float())[0].half())
+
+
+@pytest.mark.parametrize("n,kv", [(3, 40), (140, 150)])
+def test_wide_values_reach_no_row_that_does_not_see_them(cuda_dev, n, kv):
+    """Values near the largest FP16 at a position that earlier rows do not see, and in the last page's tail where
+    an earlier owner left them."""
+    H, Hk, D = 4, 2, 64
+    c = Cache([(n, kv)], H, Hk, D, 16, seed=1)
+    q, k, v = held_rows(c, 2)
+    c.fill(k.cuda(), v.cuda())
+    clean = c.attend(q.cuda(), True)
+    capi.sync(stream())
+    tail = -(-kv // 16) * 16
+    assert tail > kv
+    t = Cache([(tail, tail)], H, Hk, D, 16, seed=1)
+    t.kv, t.table, t.ld = c.kv, c.table, c.ld
+    wide = wide_rows(tail, Hk, D, 5).cuda()
+    t.fill(wide, wide)
+    c.fill(k.cuda(), v.cuda())
+    out = c.attend(q.cuda(), True)
+    capi.sync(stream())
+    assert torch.equal(out, clean)
+    v2 = v.clone()
+    v2[kv - 2:] = wide[:2].cpu()
+    c.fill(k.cuda(), v2.cuda())
+    out = c.attend(q.cuda(), True)
+    capi.sync(stream())
+    sees = torch.arange(kv - n, kv) >= kv - 2
+    assert torch.equal(out[~sees.cuda()], clean[~sees.cuda()])
+    (kx, _), (vx, vs) = quantised(k.float()), held_finite(v2.float())
+    want, tol = reference(c, q, kx, vx, vs, True, D ** -0.5)
+    assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
 def test_non_finite_rows_read_back_as_nan(cuda_dev):
     c = Cache([(6, 6)], 1, 1, 128, 16)
     x = torch.ones(6, 1, 128, dtype=torch.bfloat16)
