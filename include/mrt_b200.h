@@ -415,8 +415,9 @@ typedef struct mrt_kv_q4_s* mrt_kv_q4;
  * lengths and pages, within the sizes given here.  Rows behind
  * q_start_dev[seqs] belong to nobody: they are not read, stored or written; nor
  * does mrt_kv_q4_append or mrt_kv_q4_read touch rows at a negative position
- * (n > kv_len_dev[b]).  A sequence with no rows is skipped.  Lengths beyond
- * max_q_len, max_kv_len or tokens, and page numbers outside the cache, are not
+ * (n > kv_len_dev[b]).  A sequence with no rows is skipped.  Lengths below 0 or
+ * beyond max_q_len, max_kv_len or tokens (of a sequence with no rows too), a
+ * q_start_dev that decreases, and page numbers outside the cache are not
  * followed: such a sequence's rows are left as they were, what needs such a page
  * is left out (of a sum over it, the result is unspecified), and mrt_sync then
  * returns MRT_ERR_INVALID_ARG.

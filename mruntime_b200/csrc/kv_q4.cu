@@ -139,13 +139,15 @@ __device__ __forceinline__ void store8(uint16_t* p, uint4 v, bool vec) {
 }
 
 // Sequence and position of `count` rows from t0 on (block-wide): seq[i] < 0 for
-// a row that is nobody's or breaks the call's bounds (which is reported).
+// a row that is nobody's or breaks the call's bounds.  The first block looks at
+// every sequence, so that one whose rows no block has is reported too.
 __device__ __forceinline__ void find_rows(const KvView& v, int t0, int count, int* seq, int* pos) {
     if (threadIdx.x < count) seq[threadIdx.x] = -1;
     __syncthreads();
+    const bool every = blockIdx.x == 0 && blockIdx.y == 0;
     for (int b = threadIdx.x; b < v.seqs; b += blockDim.x) {
         const int f = v.q_start[b], e = v.q_start[b + 1];
-        if (e <= t0 || f >= t0 + count || e <= f) continue;
+        if (!every && (e <= t0 || f >= t0 + count || e <= f)) continue;
         int first, n, kv;
         if (!kv_seq(v, b, &first, &n, &kv)) {
             raise_error(v.err_flag, kErrBadPage);

@@ -705,6 +705,48 @@ def test_bad_pages_and_lengths_are_reported(cuda_dev):
     assert torch.equal(again, good)
 
 
+# q_start and kv_len of two sequences, of calls with 4 rows, at most 4 a sequence and 32 tokens held; the rows that are good
+BAD_LENGTHS = [([0, 4, 8], [20, 30], [0, 1, 2, 3]), ([0, 2, 5], [20, 30], [0, 1]), ([4, 4, 5], [20, 30], []),
+               ([0, 3, 2], [20, 30], [0, 1, 2]), ([0, 4, 4], [20, 33], [0, 1, 2, 3]), ([0, 0, 4], [-1, 30], [0, 1, 2, 3]),
+               ([0, 1, 4], [33, 30], [1, 2, 3]), ([-1, 2, 4], [20, 30], [2, 3])]
+
+
+@pytest.mark.parametrize("case", range(len(BAD_LENGTHS)))
+@pytest.mark.parametrize("heads", [2, 16])
+def test_every_call_reports_bad_lengths(cuda_dev, case, heads):
+    """Append, read and attention (of few rows and of many) leave a bad sequence's rows as they were, serve the
+    other, and say so: a sequence behind the call's rows, one without rows and one that ends before it begins too."""
+    start, held, good = BAD_LENGTHS[case]
+    D = 64
+    c = Cache([(4, 32), (4, 32)], heads, 1, D, 16, 10000.0, seed=case)
+    g = torch.Generator().manual_seed(case)
+    k, v = rows(g, 64, 1, D), rows(g, 64, 1, D)
+    c.fill(k.cuda(), v.cuda())
+    b = c.make_batch([0, 0], tokens=4, max_q=4, max_kv=32)
+    b.keep[0].copy_(torch.tensor(start, dtype=torch.int32))
+    b.keep[1].copy_(torch.tensor(held, dtype=torch.int32))
+    q = rows(g, 4, heads, D).cuda()
+    qo, kn, vn = torch.full_like(q, 9.0), rows(g, 4, 1, D).cuda(), rows(g, 4, 1, D).cuda()
+    rest = [i for i in range(4) if i not in good]
+
+    def reported():
+        with pytest.raises(capi.MrtError) as e:
+            capi.sync(stream())
+        assert e.value.code == 1
+
+    c.append(b, kn, vn, q, qo)
+    reported()
+    assert (qo[rest] == 9.0).all() and all((qo[i] != 9.0).any() for i in good)
+    kr, vr = (torch.full((4, 1, D), 9.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    c.kv.read(b, capi.FP16, kr.data_ptr(), D, vr.data_ptr(), D, stream())
+    reported()
+    assert (vr[rest] == 9.0).all()
+    assert torch.equal(vr[good].cpu(), quantised(vn[good].cpu().float())[0].half())
+    out = c.attend(q, True, batch=b)
+    reported()
+    assert (out[rest] == 9.0).all() and all((out[i] != 9.0).any() for i in good)
+
+
 @pytest.mark.parametrize("n,kv,H", [(3, 33, 4), (3, 33, 8), (40, 49, 4)])
 def test_a_bad_page_spoils_no_row_that_does_not_need_it(cuda_dev, n, kv, H):
     """The newest token's page is none of the cache: earlier rows do not see it."""
