@@ -378,10 +378,12 @@ int mrt_weight_q4_free(mrt_weight_q4 w);
  * FP32 sums.  FP16 y: rounded once, then bias (MRT_GEMM_BIAS) and residual
  * (res_dev FP16 [M, N], row stride ldr, or NULL; y_dev may be res_dev) each
  * added with a rounding, as mrt_gemm and mrt_gemm_residual do.  FP32 y: the
- * sums as they are, without bias or residual.  Any M is right; tokens are
- * taken 16 at a time (fewer where K is so long that 16 rows of x leave shared
- * memory no room), each of these reading the weight once; MRT_ERR_SHAPE where
- * not even one row fits (K beyond some 400,000).  No scratch memory.
+ * sums as they are, without bias or residual.  Any M and N are right; tokens
+ * are taken 16 at a time (fewer where K is so long that 16 rows of x leave
+ * shared memory no room), each of these reading the weight once (in several
+ * launches, over parts of the rows, where both N and K are large);
+ * MRT_ERR_SHAPE where not even one token fits: K beyond 570,000 to 770,000, by
+ * the group.  No scratch memory.
  * An infinity or NaN in a token makes its outputs infinities or NaN. */
 int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, const void* res_dev, int64_t ldr, void* y_dev,
                 int y_dtype, int64_t ldy, int64_t M, unsigned flags, void* stream);

@@ -39,6 +39,8 @@ struct GemvPlan {
     int per_sm = 0;                    // CTAs a multiprocessor
     int share = 0;                     // block pairs of a warp
     bool joins = false;                // warps share tiles
+    int at_once = 0;                   // row tiles of a launch
+    double us = 0.0;                   // of all launches, as told
 };
 constexpr int kMaxTokens = 16;  // of a launch: two token tiles of eight
 
@@ -537,9 +539,11 @@ __global__ void __launch_bounds__(most_warps(NT) * 32, 1) gemv_q4_kernel(const G
 // 12% on average, and the choice costs 2% over the best.
 constexpr int kWarps[] = {1, 2, 3, 4, 6, 8, 10, 12, 14, 16, 20, 24};
 
-GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
+// `parts`: also launches over a part of the row tiles after one another.  (A
+// warp of a CTA with a slice of K keeps two sums, so such a CTA takes no more
+// tiles than it has warps.)
+GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms, bool parts) {
     GemvPlan best;
-    double best_us = 0.0;
     const int nt = M <= 8 ? 1 : 2;
     for (int per_sm = nt == 1 ? 3 : 2; per_sm > 0; --per_sm)
         for (int ks = 1; ks <= 8; ks *= 2)
@@ -549,24 +553,29 @@ GemvPlan plan_gemv(int M, int tiles, int blocks, int per, int piece, int sms) {
                 // (Clusters of four and eight leave some multiprocessors idle: of 148
                 // they reach 132 and 120.)
                 const int room = std::max(1, sms * per_sm * (ks < 4 ? 16 : (ks == 4 ? 14 : 13)) / (16 * ks));
-                const int64_t tiles_cta = (tiles + room - 1) / room, share = (tiles_cta * pairs + warps - 1) / warps;
-                if (ks > 1 && tiles_cta > warps) continue;  // (a warp keeps two sums)
+                int64_t tiles_cta = (tiles + room - 1) / room;
+                int launches = 1, at_once = tiles;
+                if (ks > 1 && tiles_cta > warps) {
+                    if (!parts) continue;
+                    launches = static_cast<int>((tiles_cta + warps - 1) / warps);
+                    tiles_cta = (tiles_cta + launches - 1) / launches;
+                    at_once = static_cast<int>(room * tiles_cta);
+                }
+                const int64_t share = (tiles_cta * pairs + warps - 1) / warps;
                 if (tiles_cta * pairs < warps) continue;
                 const bool joins = ks > 1 || share % pairs != 0;
                 if (gemv_smem(M, slice, per, nt, warps, joins, kMinStages, piece) > kSmemMost / per_sm) continue;
-                const int64_t ctas = (tiles + tiles_cta - 1) / tiles_cta * ks;
+                const int64_t ctas = (std::min(at_once, tiles) + tiles_cta - 1) / tiles_cta * ks;
                 // of the busiest multiprocessor, of all of them
                 const double busiest = static_cast<double>((ctas + sms - 1) / sms) * tiles_cta * slice;
-                const double mean = static_cast<double>(tiles) * blocks / sms;
+                const double mean = static_cast<double>(std::min(at_once, tiles)) * blocks / sms;
                 const double a_piece = (per == 4 ? 0.0463 : 0.0407) * (nt == 1 ? 1.0 : 1.73) * (0.942 + 0.058 * most_warps(nt) / (warps * per_sm));
                 const double work = std::max((0.797 * busiest + 0.203 * mean) * a_piece, share * kPair * 0.445);
                 const double x = ctas * 256.0 / 11.8e6 * M * slice + M * slice * 16.0 / (warps * 32) * 0.0843;
-                const double parts = share < pairs ? std::min<double>(warps, static_cast<double>(pairs) / share) : 1.0;  // of a tile
-                const double us = work + x + 0.0574 * warps + (joins ? 0.3 + 0.04 * parts : 0.0) + (ks > 1 ? 2.05 + 0.029 * ks : 0.0);
-                if (best.warps == 0 || us < best_us) {
-                    best = GemvPlan{warps, static_cast<int>(tiles_cta), ks, per_sm, static_cast<int>(share), joins};
-                    best_us = us;
-                }
+                const double shares = share < pairs ? std::min<double>(warps, static_cast<double>(pairs) / share) : 1.0;  // of a tile
+                const double us = work + x + 0.0574 * warps + (joins ? 0.3 + 0.04 * shares : 0.0) + (ks > 1 ? 2.05 + 0.029 * ks : 0.0);
+                if (best.warps == 0 || us * launches < best.us)
+                    best = GemvPlan{warps, static_cast<int>(tiles_cta), ks, per_sm, static_cast<int>(share), joins, at_once, us * launches};
             }
     return best;
 }
@@ -600,10 +609,28 @@ cudaError_t launch(GemvQ4Args a, const GemvPlan& p, cudaStream_t s) {
 
 // Tokens of the next launch: sixteen, or as many as leave x room in shared
 // memory (0: not even one does).
-int tokens_at_once(const mrt_weight_q4_s* w, int64_t M) {
+int tokens_at_once(const GemvPlan* plans, int64_t M) {
     int m = static_cast<int>(std::min<int64_t>(M, kMaxTokens));
-    while (m > 0 && w->plans[m].warps == 0) m = m > 8 ? 8 : m / 2;
+    while (m > 0 && plans[m].warps == 0) m = m > 8 ? 8 : m / 2;
     return m;
+}
+
+// Plans of a weight by tokens.  Where no launch can take all of it, launches over
+// parts of its rows, unless fewer tokens at a time are quicker (16 tokens on 28768
+// x 18944, groups of 32: eight launches, against four over the whole weight).
+void plan_weight(GemvPlan* plans, int tiles, int blocks, int per, int piece, int sms) {
+    for (int m = 1; m <= kMaxTokens; ++m) {
+        plans[m] = plan_gemv(m, tiles, blocks, per, piece, sms, false);
+        if (plans[m].warps > 0) continue;
+        double us = 0.0;  // of fewer at a time
+        for (int left = m, t; left > 0; left -= t) {
+            t = tokens_at_once(plans, left);
+            if (t == 0) break;
+            us += plans[t].us;
+        }
+        const GemvPlan p = plan_gemv(m, tiles, blocks, per, piece, sms, true);
+        if (p.warps > 0 && (us == 0.0 || p.us < us)) plans[m] = p;
+    }
 }
 
 cudaError_t launch_gemv_q4(GemvQ4Args a, const GemvPlan& p, int per, cudaStream_t s) {
@@ -660,8 +687,7 @@ int new_handle(int64_t N, int64_t K, int64_t group, bool zeros, cudaStream_t s, 
     w->blocks = (K + 127) / 128;
     w->zeros = zeros;
     w->piece = piece_bytes(static_cast<int>(128 / group), zeros);
-    for (int m = 1; m <= kMaxTokens; ++m)
-        w->plans[m] = plan_gemv(m, static_cast<int>(w->tiles), static_cast<int>(w->blocks), static_cast<int>(128 / group), w->piece, c->sms);
+    plan_weight(w->plans, static_cast<int>(w->tiles), static_cast<int>(w->blocks), static_cast<int>(128 / group), w->piece, c->sms);
     const size_t bytes = static_cast<size_t>(w->tiles) * w->blocks * w->piece;
     cudaError_t e = cudaMalloc(&w->data, bytes);
     if (e == cudaSuccess) e = cudaMemsetAsync(w->data, 0, bytes, s);
@@ -832,29 +858,33 @@ extern "C" int mrt_gemv_q4(mrt_weight_q4 w, const void* x_dev, int64_t ldx, cons
     if (!c) return MRT_ERR_CUDA;
     if (c->device != w->device) return set_error(MRT_ERR_INVALID_ARG, "weight lives on another device");
     GemvQ4Args a{};
-    a.data = w->data;
     a.piece = w->piece;
     a.zeros = w->zeros ? 1 : 0;
     a.err_flag = c->d_err;
-    a.n = static_cast<int>(w->n);
     a.k = static_cast<int>(w->k);
     a.blocks = static_cast<int>(w->blocks);
-    a.tiles = static_cast<int>(w->tiles);
     a.ldx = ldx;
     a.x_vec = (reinterpret_cast<uintptr_t>(x_dev) & 15) == 0 && (ldx & 7) == 0;
     a.ldy = ldy;
     a.out_f32 = y_dtype == MRT_FP32;
-    a.bias = use_bias ? w->bias : nullptr;
     a.ldr = ldr;
     const int per = static_cast<int>(128 / w->group);
     for (int64_t m = 0; m < M; m += a.M) {
-        a.M = tokens_at_once(w, M - m);
+        a.M = tokens_at_once(w->plans, M - m);
         if (a.M == 0) return set_error(MRT_ERR_SHAPE, "K is too large for a token in shared memory");
+        const GemvPlan& plan = w->plans[a.M];
         a.x = static_cast<const uint16_t*>(x_dev) + m * ldx;
-        a.y = static_cast<uint8_t*>(y_dev) + m * ldy * (a.out_f32 ? 4 : 2);
-        a.res = res_dev != nullptr ? static_cast<const uint16_t*>(res_dev) + m * ldr : nullptr;
-        const cudaError_t e = launch_gemv_q4(a, w->plans[a.M], per, static_cast<cudaStream_t>(stream));
-        if (e != cudaSuccess) return cuda_error(e, "4-bit gemv launch");
+        for (int64_t t = 0; t < w->tiles; t += plan.at_once) {
+            const int64_t row = t * 16;
+            a.tiles = static_cast<int>(std::min<int64_t>(w->tiles - t, plan.at_once));
+            a.n = static_cast<int>(w->n - row);
+            a.data = w->data + t * w->blocks * w->piece;
+            a.y = static_cast<uint8_t*>(y_dev) + (m * ldy + row) * (a.out_f32 ? 4 : 2);
+            a.bias = use_bias ? w->bias + row : nullptr;
+            a.res = res_dev != nullptr ? static_cast<const uint16_t*>(res_dev) + m * ldr + row : nullptr;
+            const cudaError_t e = launch_gemv_q4(a, plan, per, static_cast<cudaStream_t>(stream));
+            if (e != cudaSuccess) return cuda_error(e, "4-bit gemv launch");
+        }
     }
     return MRT_OK;
 }

@@ -76,6 +76,71 @@ def test_long_sums_cut_into_slices(cuda_dev, M, N, K, group, zeros):
     assert torch.equal(run(w, x), got)
 
 
+def make_large(N, K, group, zeros, seed):
+    """make() for weights that are told by slices of rows: the weight, and its values and magnitudes of rows a..b."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8, device="cuda")
+    scales = (0.001 + 0.02 * torch.rand(N, K // group, generator=g, device="cuda")).half()
+    z = torch.randint(0, 16, (N, K // group), generator=g, dtype=torch.uint8, device="cuda") if zeros else None
+    w = capi.WeightQ4.from_codes(codes.data_ptr(), scales.data_ptr(), capi.FP16, z.data_ptr() if zeros else None, True,
+                                 N, K, group, stream())
+
+    def values(a, b):
+        c = torch.stack((codes[a:b] & 15, codes[a:b] >> 4), -1).view(-1, K // group, group).double()
+        s = scales[a:b].double()[:, :, None]
+        zz = z[a:b].double()[:, :, None] if zeros else 8.0
+        return (s * (c - zz)).view(-1, K), (s * (c + zz)).view(-1, K)
+
+    return w, values
+
+
+def check_large(w, values, x, got, out_eps, added=0.0):
+    """Every output against 64-bit sums, a slice of rows at a time; `added`: to the product, once it is rounded."""
+    step = max(16, (1 << 27) // w.k)
+    xd = x.cuda()
+    for a in range(0, w.n, step):
+        val, mag = values(a, min(a + step, w.n))
+        y, tol = bound(xd, val, mag, out_eps, w.k)
+        extra = added[:, a:a + step].double().cuda() if torch.is_tensor(added) else 0.0
+        tol = tol + (2.0 ** -11 * ((y + extra).abs() + tol) if torch.is_tensor(added) else 0.0)
+        assert ((got[:, a:a + step].cuda().double() - y - extra).abs() <= tol).all(), f"rows from {a} on"
+
+
+# No launch takes all of these: x is too long for a CTA without slices of K, and clusters have too few warps for the rows.
+@pytest.mark.parametrize("N,K,group,zeros,Ms", [(28771, 18944, 32, True, (5, 7, 16)), (6100, 131072, 128, False, (4, 9)),
+                                                (32000, 98304, 128, True, (1, 3))])
+def test_long_rows_of_large_weights(cuda_dev, N, K, group, zeros, Ms):
+    w, values = make_large(N, K, group, zeros, K)
+    for M in Ms:
+        g = torch.Generator().manual_seed(M)
+        x = torch.randn(M, K, generator=g).half()
+        got = run(w, x)
+        check_large(w, values, x, got, 2.0 ** -11)
+        assert torch.equal(run(w, x), got)
+        check_large(w, values, x, run(w, x, y_dtype=capi.FP32), 2.0 ** -24)
+        res = torch.randn(M, N, generator=g).half()
+        rd = res.cuda()
+        check_large(w, values, x, run(w, x, res_ptr=rd.data_ptr(), ldr=N), 2.0 ** -11, res)
+
+
+def test_bias_of_a_weight_in_parts(cuda_dev):
+    N, K = 6100, 131072
+    w, values = make_large(N, K, 128, False, 3)
+    b = torch.randn(N, generator=torch.Generator().manual_seed(1)).half()
+    bd = b.cuda()
+    w.attach_bias(bd.data_ptr(), capi.FP16, True, stream())
+    x = torch.randn(4, K, generator=torch.Generator().manual_seed(2)).half()
+    check_large(w, values, x, run(w, x, bias=True), 2.0 ** -11, b[None].expand(4, N))
+
+
+def test_k_beyond_shared_memory_is_refused(cuda_dev):
+    K = 1 << 20
+    w = make_large(16, K, 128, False, 1)[0]
+    t = torch.zeros(K, dtype=torch.float16, device="cuda")
+    assert capi.lib().mrt_gemv_q4(w.h, t.data_ptr(), K, None, 0, t.data_ptr(), 0, 16, 1, 0, stream()) == 2
+    capi.sync(stream())
+
+
 def test_one_weight_on_two_streams(cuda_dev):
     """Calls that overlap give what they give alone."""
     w, _, _ = make(700, 4096, 64, True, 4)
