@@ -123,6 +123,26 @@ def test_long_rows_of_large_weights(cuda_dev, N, K, group, zeros, Ms):
         check_large(w, values, x, run(w, x, res_ptr=rd.data_ptr(), ldr=N), 2.0 ** -11, res)
 
 
+# Stretches of several tiles a warp, with a piece of a tile at each end; the last CTA short, the last tile not whole.
+@pytest.mark.parametrize("N,K,group,zeros", [(152064, 3584, 128, False), (152057, 3584, 64, True), (150003, 512, 64, True),
+                                             (149993, 640, 32, False), (60010, 896, 128, True)])
+@pytest.mark.parametrize("M", [1, 7, 16])
+def test_warps_with_many_tiles(cuda_dev, N, K, group, zeros, M):
+    w, values = make_large(N, K, group, zeros, N + M)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).half()
+    got = run(w, x)
+    check_large(w, values, x, got, 2.0 ** -11)
+    assert torch.equal(run(w, x), got)
+    check_large(w, values, x, run(w, x, y_dtype=capi.FP32), 2.0 ** -24)
+
+
+@pytest.mark.parametrize("M", [14, 30])
+def test_fewer_tokens_at_a_time_where_more_have_no_plan(cuda_dev, M):
+    w, values = make_large(28771, 18944, 32, True, M)
+    x = torch.randn(M, 18944, generator=torch.Generator().manual_seed(M)).half()
+    check_large(w, values, x, run(w, x), 2.0 ** -11)
+
+
 def test_bias_of_a_weight_in_parts(cuda_dev):
     N, K = 6100, 131072
     w, values = make_large(N, K, 128, False, 3)
