@@ -391,6 +391,50 @@ def test_attention(cuda_dev, case, dtype, causal):
     assert torch.equal(qd[:n], out[:n])
 
 
+def attention64(c, q, kx, vx, causal, rounded=None):
+    """64-bit attention of whole sequences; `rounded`: the type that probabilities (relative to their row's largest)
+    and, of many rows, values are rounded to on the way."""
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    many = max(n for n, _ in c.lens) * c.H // c.Hk > 32
+    row = tok = 0
+    for n, kv in c.lens:
+        s = torch.einsum("nhgd,thd->hgnt", q[row:row + n].double().view(n, c.Hk, -1, c.D), kx[tok:tok + kv]) * c.D ** -0.5
+        if causal:
+            s = s.masked_fill(torch.ones(n, kv, dtype=torch.bool).triu(kv - n + 1), -math.inf)
+        p = (s - s.amax(-1, keepdim=True)).exp()
+        w, v = p, vx[tok:tok + kv]
+        if rounded is not None:
+            w, v = p.to(rounded).double(), v.to(rounded).double() if many else v
+        out[row:row + n] = torch.einsum("hgnt,thd->nhgd", w / p.sum(-1, keepdim=True), v).reshape(n, c.H, c.D)
+        row, tok = row + n, tok + kv
+    return out
+
+
+@pytest.mark.parametrize("lens,H,Hk,D", [([(1, 517), (1, 1200), (1, 90)], 28, 4, 128), ([(1, 700), (1, 350)], 14, 2, 64),
+                                         ([(3, 400), (2, 1500)], 28, 4, 128), ([(64, 300), (40, 700)], 14, 2, 64),
+                                         ([(90, 500)], 28, 4, 128), ([(130, 130), (7, 900)], 12, 4, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_rounds_to_fp16_and_no_further(cuda_dev, lens, H, Hk, D, causal):
+    """The error of a whole call.  Of numbers whose mantissas are spread evenly over the logarithm, rounding to FP16
+    is off by 2^-11 sqrt(1/3 . 3/4 / (2 ln 2)) = 0.425 2^-11 in the root mean square.  There are three: of the outputs,
+    and of probabilities and (of many rows) values, whose terms p v, of either sign, add up as their errors do; so
+    sqrt(3) 0.425 = 0.74 of 2^-11 in all, FP32 sums being 2^-20 of it.  Rounded to BF16 instead, at 8 times that, the
+    same inputs are beyond the bound."""
+    c = Cache(lens, H, Hk, D, 16, seed=D + H)
+    g = torch.Generator().manual_seed(H)
+    total = sum(kv for _, kv in lens)
+    q, k, v = (torch.randn(n, h, D, generator=g).half() for n, h in ((c.T, H), (total, Hk), (total, Hk)))
+    c.fill(k.cuda(), v.cuda())
+    out = c.attend(q.cuda(), causal)
+    capi.sync(stream())
+    kx, vx = quantised(k.float())[0], quantised(v.float())[0]
+    want = attention64(c, q, kx, vx, causal)
+    err = lambda x: float((x.double() - want).norm() / want.norm())  # noqa: E731
+    assert err(attention64(c, q, kx, vx, causal, torch.float16).half()) <= 2.0 ** -11
+    assert err(attention64(c, q, kx, vx, causal, torch.bfloat16).half()) > 2.0 ** -11
+    assert err(out.cpu()) <= 2.0 ** -11
+
+
 def check_attention(c, q, k, v, causal):
     c.fill(k.cuda(), v.cuda())
     out = c.attend(q.cuda(), causal)
