@@ -1865,10 +1865,11 @@ cudaError_t launch_few_w(const RowsArgs& r, int rows, cudaStream_t s) {
     cudaError_t e = launch_pdl<attn_q4_few_kernel<D, NT, W>>(dim3(r.grid), W * 32, RowsShape<D, NT, W>::kBytes, s, r);
     if (e != cudaSuccess || !r.split) return e;
     const dim3 grid(r.a.v.seqs * r.a.v.kv_heads, rows);  // a CTA a (unit, row)
-    // Units of 24 parts and more are worth a large CTA (of 592 parts in all): 1 x 131071 tokens (148 parts)
-    // 22.8 us against 33.9, 4 x 30000 (37) 18.1 against 23.7; 8 x 4000 (18) 14.0
-    // against 11.5, 16 x 4000 (9) 20.7 against 14.5.
-    return static_cast<int64_t>(grid.x) * 24 <= r.grid ? launch_pdl<attn_q4_join_kernel<D, 512>>(grid, 512, 0, s, r, NT * 8)
+    // Units of 20 parts and more are worth a large CTA.  7 rows (444 parts in all): 1 x 131071 tokens (111 parts) 20.5 us
+    // against 27.7, 4 x 30000 (28) 16.2 against 20.0, 5 x 30000 (22) 17.8 against 21.6, 6 x 30000 (18) 23.1 against 23.5;
+    // 8 x 30000 (14) 26.8 against 26.4, 16 x 4000 (7) 20.9 against 13.7.  14 rows (296): 1 x 131071 (74) 26.7 against 31.1,
+    // 3 x 30000 (25) 21.5 both ways, 4 x 30000 (18) 24.0 against 22.2.
+    return static_cast<int64_t>(grid.x) * 20 <= r.grid ? launch_pdl<attn_q4_join_kernel<D, 512>>(grid, 512, 0, s, r, NT * 8)
                                                        : launch_pdl<attn_q4_join_kernel<D, 64>>(grid, 64, 0, s, r, NT * 8);
 }
 
