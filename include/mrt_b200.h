@@ -377,7 +377,8 @@ int mrt_weight_q4_free(mrt_weight_q4 w);
  * y_dev[M, N] (row stride ldy) = x_dev[M, K] (FP16, row stride ldx) * W^T in
  * FP32 sums.  FP16 y: rounded once, then bias (MRT_GEMM_BIAS) and residual
  * (res_dev FP16 [M, N], row stride ldr, or NULL; y_dev may be res_dev) each
- * added with a rounding, as mrt_gemm and mrt_gemm_residual do.  FP32 y: the
+ * added with a rounding, as mrt_gemm and mrt_gemm_residual do; y_dev does not
+ * overlap x_dev.  FP32 y: the
  * sums as they are, without bias or residual.  Any M and N are right; tokens
  * are taken 16 at a time (fewer where K is so long that 16 rows of x leave
  * shared memory no room), each of these reading the weight once (in several
@@ -464,11 +465,19 @@ int mrt_kv_q4_read(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype, void* k_d
  * kv_len.  q_dev and out_dev [tokens, heads, head_dim] (FP16 or BF16, token
  * strides ldq and ldo; out_dev may be q_dev), heads a multiple of kv_heads,
  * query head h reading kv head h / (heads / kv_heads).  A row that sees no
- * position (one at a negative position, when causal) gives zeros.  Sums and
- * softmax are FP32; probabilities are rounded to FP16 relative to their row's
- * largest, and where a call has more than 32 rows (max_q_len * heads /
- * kv_heads) so are the values s (c - z).  MRT_ERR_SHAPE for more rows and keys
- * than 31 bits number.  ws_dev: scratch of at least the bytes that
+ * position (one at a negative position, when causal) gives zeros.
+ *
+ * Sums and softmax are FP32, with the hardware's exponential, logarithm and
+ * reciprocal (off by some 2^-22).  Two forms, by the call's sizes alone: up to 32
+ * rows (max_q_len * heads / kv_heads) q goes in as FP16 times a power of two of
+ * its row (no rounding but of channels below 2^-23 of the largest), and a
+ * probability times its value's scale s is rounded to FP16, relative to the row's
+ * largest; with more, q goes in as it is, and probabilities, relative to the
+ * largest, and values s (c - z) are rounded to FP16.  One sequence of many rows
+ * takes all of its call to the second form, where a sequence of few rows is
+ * worked on as if it had 128: prompts and single tokens are better two calls.
+ *
+ * MRT_ERR_SHAPE for more rows and keys than 31 bits number.  ws_dev: scratch of at least the bytes that
  * mrt_kv_q4_attention_workspace says for the same batch sizes (256-byte
  * aligned), the caller's own, so calls with scratch of their own may overlap;
  * its contents need no clearing and mean nothing afterwards.

@@ -270,11 +270,14 @@ __device__ __forceinline__ void store_y(const GemvQ4Args& a, int64_t n, int m, f
 // What bounds it: for few tokens the weights' bytes, so every warp keeps up to
 // eight pieces of them under way (two a copy), the first before it waits for the
 // kernel that makes x (with loads into registers, four deep, a warp waited for
-// more than it asked for: 21.5 us for 37888 x 3584 at one token); and, as much,
-// the instructions that make operands of a piece (about 140 a KB): 15.9 us for
-// 37888 x 3584 at one token (70.5 MB, 4.4 TB/s), 70 for 152064 x 3584 at 16 (286
-// MB, 4.1 TB/s: beside them x from shared memory, eight KB a KB of codes).  Small
-// weights are bound by a launch and x's way into the CTAs: 896 x 896 2.9 us;
+// more than it asked for: 21.5 us for 37888 x 3584 at one token); and the chain of
+// instructions that make operands of a piece (about 140 a KB): 15.4 us for 37888 x
+// 3584 at one token (70.6 MB, 4.6 TB/s), 70 for 152064 x 3584 at 16 (286 MB, 4.1
+// TB/s: beside them x from shared memory, eight KB a KB of codes).  No unit is full
+// there: at one token issue slots are at 50%, the ALU at 48, four warps a scheduler
+// that issue every 7.5 cycles, 1.9 of them the instructions' own latency, 1.2 pieces
+// and 1.0 the ALU.  Small
+// weights are bound by a launch and x's way into the CTAs: 896 x 896 3.2 us;
 // long sums of several tokens by x in every CTA: 3584 x 18944 at 7, groups of
 // 32, 18 us (40 MB).  x is brought in once a CTA, with its group sums, and CTAs
 // stay for all the row tiles they take.

@@ -193,9 +193,12 @@ __device__ __forceinline__ uint32_t codes8(const float (&x)[8], float inv, int z
 // changes lanes and every lane packs whole words.  CTAs take tokens (prompts:
 // eight, so that the angles' sines, in 64 bits, and the search for the sequence
 // are shared by many rows) and all their rows, or, when tokens are few, a stretch
-// of them.  Bound by instructions: five prompts of up to 2900 tokens (9060 tokens,
-// 36 rows of 128) take 39 us where their bytes would take 20 (reading them back
-// 13 us); 33 tokens take 3.3 us, a launch and four loads that wait for one another.
+// of them.  Five prompts of up to 2900 tokens (9758 tokens, 36 rows of 128) take
+// 38.5 us where their bytes (165 MB) would take 25, and 9.6 to be read back (25
+// MB, 3.8).  No unit is full there (issue slots 42%, ALU 28%): of the ten cycles
+// between a warp's instructions 3.6 wait for global loads, as no row is under way
+// before the token's place and sines are known, and 1.6 for shared memory and the
+// sines.  33 tokens take 3.7 us, a launch and four loads that wait for one another.
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a, const Freqs f) {
     constexpr int LANES = D / 16, HALF = D / 2;
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const ReadArgs a) {
 uint64_t magic_of(int rows) { return ((1ull << 40) + rows - 1) / rows; }
 
 // Tokens of a CTA: as many as leave every multiprocessor two CTAs (append and
-// read of 9060 tokens 50 us, with one token a CTA 114; of 33 6.6 us, with eight a
+// read of 9758 tokens 50 us, with one token a CTA 114; of 33 6.6 us, with eight a
 // CTA 13.3; of 700 9.1, against 12.6 and 13.5).
 int tokens_of(int tokens, int sms) { return std::max(1, std::min(kMaxTokens, tokens / (2 * sms))); }
 

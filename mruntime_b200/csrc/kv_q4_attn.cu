@@ -20,7 +20,7 @@ constexpr int kThreads = 256;
 
 struct AttnQ4Args {
     KvView v;
-    int dtype, heads, causal;
+    int dtype, causal;
     float scale;
     const uint16_t* q;
     int64_t ldq;
@@ -70,12 +70,20 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // The sum is of p' / s_v, and the zero points' part of the output, sum p' z (of
 // the same rounded p'), is one more row of the second product.
 //
-// What bounds it: bytes and instructions alike.  64 sequences of up to 8192
-// tokens (176 MB, 7 of 8 rows used) take 41 us where the bytes would take 27 at
-// the copy's rate: 406 instructions a warp and tile, half of them the masks that
-// make operands of codes, would take 17, and beginning, joining and the CTAs'
-// uneven ends 9.  One of 131071 tokens (70 MB) takes 22 us for 11: 4 until the
-// first tile is there, 13 for the tiles, 5 for the parts.
+// What bounds it: latency.  64 sequences of up to 8192 tokens (175 MB, 7 of 8 rows
+// used) take 41 us where the bytes would take 27 at the copy's rate and the 406
+// instructions a warp and tile, half of them the masks that make operands of codes,
+// 17; beginning, joining and the CTAs' uneven ends are 9.  168 registers leave a
+// scheduler three warps, each of which issues every six cycles (1.6 of them the
+// instructions' own latency, 0.6 each pages, shared memory, the ALU): issue slots
+// 46%, ALU 44.  One of 131071 tokens (70 MB) takes 20 us for 11 (of 22, with
+// four CTAs a multiprocessor, 4 passed until the first tile was there, 13 with the
+// tiles, 5 with the parts).
+//
+// More rows cost registers first: from nine on there are two CTAs a multiprocessor,
+// and with 24 rows 16 bytes a thread are spilled, with 32 rows 624, of 16 rows of
+// a lone unit's sixteen warps 280 (9 x 3 x 6000 tokens, 21 rows: 19 us for 3, four
+// tiles a warp and eight warps a multiprocessor, issue slots 31%).
 //
 // Split.  The 32-token tiles of all (sequence, kv head) units, in order, are
 // dealt to the CTAs in equal contiguous stretches, whatever the lengths: no
@@ -901,8 +909,8 @@ __device__ __forceinline__ bool warp_gave_up(const volatile int* flag) { return 
 //                    P back into its place
 //   warps 16-23      codes from the pages into the tensor cores' swizzled
 //                    layout, K as the integers c - z (exact), V as values
-//                    s (c - z) rounded to FP16; four warps the even key tiles,
-//                    four the odd ones
+//                    s (c - z) rounded to FP16 (finite: append sees to it); four
+//                    warps the even key tiles, four the odd ones
 //   warps 24, 25     S_i = Q_i K^T
 //   warps 26, 27     O_i += P_i V (P from TMEM)
 //   warps 28-30      Q into its panels
@@ -919,7 +927,11 @@ __device__ __forceinline__ bool warp_gave_up(const volatile int* flag) { return 
 // each value, independent from token to token like that of P, and averaged
 // with it), because every number that a column needs in the softmax is a
 // shared-memory read for every pair of rows; with the value's scale in the
-// exponent, as in the few-rows kernel, a column needed three.  Scores come out
+// exponent, as in the few-rows kernel, a column needed three.  (With V as c - z
+// times a power of two, exact, and the rest of its scale multiplied into the
+// probability, a call's error against 64 bits is 2.9e-4 of its norm instead of
+// 3.5e-4, 2.1e-4 being the FP16 output's, but the 2048 tokens below take 523 to 531
+// us instead of 471.)  Scores come out
 // of one fused operation relative to the running maximum m, which moves only
 // when a row exceeds it by 2^8 (P then still fits FP16 with all its bits): rows'
 // maxima are joined, scores moved and O in TMEM rescaled in that case alone.
@@ -927,11 +939,12 @@ __device__ __forceinline__ bool warp_gave_up(const volatile int* flag) { return 
 // 148 KB of code and every step of every role waited for its instructions.
 //
 // What bounds it: 2048 tokens behind 14000 (28 heads on 4 of 128 channels) take
-// 474 us, 441 GFLOP at 55% of the rate of a large bf16 product.  Issue slots
+// 471 us in a short run, 441 GFLOP at 56% of the rate of a large bf16 product, and
+// 520 to 530 at the clocks of a long one (50%).  Issue slots
 // (62% used) and shared memory (two thirds: Q and K for S, V for O, the codes'
-// stores, the columns' scales) come first, the exponentials' unit has 37%, the
-// tensor cores' 36.  Two prompts of 1800 and 965 tokens behind 100 and 54 (14
-// heads on 2 of 64) take 39 us, 9 of them until the first scores are there and 4
+// stores, the columns' scales) come first, the exponentials' unit has 38%, the
+// tensor cores' 38.  Two prompts of 1800 and 966 tokens behind 100 and 54 (14
+// heads on 2 of 64) take 40 us, 9 of them until the first scores are there and 4
 // for the parts.
 //
 // Units' key tiles are dealt to the CTAs in equal contiguous stretches, as in
@@ -973,8 +986,9 @@ struct ManySeq {
     }
 };
 
-// sum_{i < n} floor((a i + b) / m), the lattice points under a line, counted by
-// exchanging the axes until the line is flat.  a n + b fits in 32 bits (checked
+// sum_{i < n} floor((a i + b) / m), the lattice points under a line, by the known
+// Euclid-like method (reciprocity of sums of floors; Graham, Knuth and Patashnik,
+// Concrete Mathematics, 3.5): the axes are exchanged until the line is flat.  a n + b fits in 32 bits (checked
 // on the host); so does the sum, whose parts may wrap.
 __device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     uint32_t sum = 0;
@@ -1143,7 +1157,8 @@ __device__ __forceinline__ void registers_down() {
 }
 
 // Registers a thread: at launch, and as the roles share them out (in groups of
-// four warps: four of softmax, two of codes, products, Q).
+// four warps: four of softmax, two of codes, products, Q).  (4 to 12 bytes a thread
+// are spilled.)
 constexpr int kManyRegs = 64, kSoftmaxRegs = 72, kCodesRegs = 72, kOtherRegs = 40;
 static_assert(kManyWarps == 32, "a lane a warp in the scan");
 static_assert(4 * kSoftmaxRegs + 2 * kCodesRegs + 2 * kOtherRegs == 8 * kManyRegs, "the roles share what the launch has");
@@ -1930,7 +1945,6 @@ extern "C" int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int 
             return set_error(MRT_ERR_INVALID_ARG, "scratch must be 256-byte aligned");
     }
     a.dtype = dtype;
-    a.heads = static_cast<int>(heads);
     a.causal = causal != 0;
     a.scale = scale;
     a.q = static_cast<const uint16_t*>(q_dev);

@@ -55,6 +55,8 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     return d;
 }
 
+// The hardware's own forms, off by some 2^-22: far below the roundings to 16 bits
+// that follow wherever they are used.  (They take a denormal for zero.)
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
