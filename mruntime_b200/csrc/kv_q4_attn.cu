@@ -63,10 +63,11 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // the M operands straight from their bytes (q4.cuh).
 //
 // Softmax.  In powers of two, with a value's scale taken into the exponent:
-// y = scale log2(e) q.k + log2 s_v, p' = 2^(y - m), m at most eight below the
+// y = scale log2(e) q.k + log2 s_v, p' = 2^(y - m), m seven to fifteen below the
 // running maximum of y (so it seldom has to be moved).  So p' is the probability
-// times its value's scale, relative to the largest such product within 2^8: FP16
-// operands keep eleven bits of whatever matters, however unlike the scales are.
+// times its value's scale, relative to the largest such product: FP16 operands keep
+// eleven bits of whatever matters, down to 2^-21 of the largest, however unlike the
+// scales are.
 // The sum is of p' / s_v, and the zero points' part of the output, sum p' z (of
 // the same rounded p'), is one more row of the second product.
 //
@@ -97,6 +98,9 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 constexpr int kTile = 32;
 constexpr int kTileBlocks = kTile / kKvBlock;
 constexpr float kLowest = -3.402823466e38f;  // m before any key: 2^(m - anything seen) is 0
+// Exponents of a row's probabilities as FP16 operands: the largest's when m is set,
+// and what is not passed before m is moved (2^16 is infinity there).
+constexpr float kTop = 7.0f, kFar = 15.0f;
 
 struct RowsArgs {
     AttnQ4Args a;
@@ -542,14 +546,14 @@ __global__ void __launch_bounds__(W * 32, W > 8 ? 1 : (NT == 1 ? 3 : 2)) attn_q4
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     big[t][j] = fmaxf(fmaxf(y[0][t][j], y[0][t][2 + j]), fmaxf(y[1][t][j], y[1][t][2 + j]));
-                    far |= big[t][j] > m[t][j] + 8.0f;
+                    far |= big[t][j] > m[t][j] + kFar;
                 }
             if (__any_sync(0xFFFFFFFFu, far)) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float x = fmaxf(big[t][j], m[t][j]);
+                        float x = fmaxf(big[t][j] - kTop, m[t][j]);
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, off));
                         const float fix = fast_exp2(m[t][j] - x);
@@ -932,9 +936,14 @@ __device__ __forceinline__ bool warp_gave_up(const volatile int* flag) { return 
 // probability, a call's error against 64 bits is 2.9e-4 of its norm instead of
 // 3.5e-4, 2.1e-4 being the FP16 output's, but the 2048 tokens below take 523 to 531
 // us instead of 471.)  Scores come out
-// of one fused operation relative to the running maximum m, which moves only
-// when a row exceeds it by 2^8 (P then still fits FP16 with all its bits): rows'
-// maxima are joined, scores moved and O in TMEM rescaled in that case alone.
+// of one fused operation relative to m, which lies 2^7 below the largest
+// probability when it is set and moves only when a row exceeds it by 2^15 (P then
+// still fits FP16): rows' maxima are joined, scores moved and O in TMEM rescaled in
+// that case alone.  (From the upper end of FP16's range down, P keeps its bits to
+// 2^-21 of the row's largest: where one key without a value takes most of a row, as
+// a first token often does, the output is made of probabilities that small.  With m
+// at the largest, 2^-14, a call whose first key had e^12 times the others'
+// probability and a value of zeros was off by 3.6e-3 of its norm, now by 3.5e-4.)
 // All loops are short: with the softmax unrolled over its rows the kernel had
 // 148 KB of code and every step of every role waited for its instructions.
 //
@@ -1380,9 +1389,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attn_q4_many_kernel(const Man
                             float x = fmaxf(big[b], __shfl_xor_sync(0xFFFFFFFFu, big[b], 1));
                             x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
                             const bool seen = far[b] > 0.0f;
-                            const float up = x > (seen ? 0.0f : -INFINITY) ? x : 0.0f;
+                            const float up = x > (seen ? kTop : -INFINITY) ? x - kTop : 0.0f;
                             fix[b] = seen ? fast_exp2(-up) : 1.0f;
-                            if (x > -INFINITY) far[b] = 8.0f;
+                            if (x > -INFINITY) far[b] = kFar;
                             m[b] += up;
                             l[b] = mul2(l[b], pair2(fix[b], fix[b]));
 #pragma unroll

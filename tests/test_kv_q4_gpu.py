@@ -435,6 +435,33 @@ def test_attention_rounds_to_fp16_and_no_further(cuda_dev, lens, H, Hk, D, causa
     assert err(out.cpu()) <= 2.0 ** -11
 
 
+@pytest.mark.parametrize("lens,H,Hk,D", [([(300, 6000)], 28, 4, 128), ([(400, 2000), (30, 3000)], 14, 2, 64),
+                                         ([(3, 800), (2, 900)] * 3, 4, 2, 64), ([(2, 1000)] * 40, 14, 2, 128)])
+@pytest.mark.parametrize("ahead", [8.0, 14.0])
+def test_a_first_key_that_takes_most_of_every_row(cuda_dev, lens, H, Hk, D, ahead):
+    """Its value is next to nothing, so that the outputs are made of probabilities that are e^-8 and e^-14 of their row's
+    largest.  e^-14 is 2^-20.2, and 2^-13.2 where the largest is 2^7: FP16's normal numbers end at 2^-14.  Below, each is
+    off by 2^-24 / sqrt(12) in the root mean square, where probabilities e^s, s of a variance of one, are 2^-13.2 e
+    in theirs: 2^-14, an eighth of 2^-11, which the three roundings' 0.74 (above) leaves room for."""
+    c = Cache(lens, H, Hk, D, 16, seed=D + H)
+    g = torch.Generator().manual_seed(H)
+    total = sum(kv for _, kv in lens)
+    q, k, v = (torch.randn(n, h, D, generator=g).half() for n, h in ((c.T, H), (total, Hk), (total, Hk)))
+    q[:, :, 0] = 4.0  # a channel that all rows share and only first keys have
+    k[:, :, 0] = 0.0
+    at = 0
+    for _, kv in lens:
+        k[at] = 0.0
+        k[at, :, 0] = ahead * D ** 0.5 / 4.0
+        v[at] *= 2.0 ** -12
+        at += kv
+    c.fill(k.cuda(), v.cuda())
+    out = c.attend(q.cuda(), True)
+    capi.sync(stream())
+    want = attention64(c, q, quantised(k.float())[0], quantised(v.float())[0], True)
+    assert float((out.cpu().double() - want).norm() / want.norm()) <= 2.0 ** -11
+
+
 def check_attention(c, q, k, v, causal):
     c.fill(k.cuda(), v.cuda())
     out = c.attend(q.cuda(), causal)
