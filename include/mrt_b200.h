@@ -471,16 +471,16 @@ int mrt_kv_q4_read(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype, void* k_d
  * reciprocal (off by some 2^-22).  Two forms, by the call's sizes alone: up to 32
  * rows (max_q_len * heads / kv_heads) q goes in as FP16 times a power of two of
  * its row (no rounding but of channels below 2^-23 of the largest), and a
- * probability times its value's scale s is rounded to FP16, relative to the row's
- * largest; with more, q goes in as it is, and probabilities, relative to the
- * largest, and values s (c - z) are rounded to FP16.  One sequence of many rows
- * takes all of its call to the second form, where a sequence of few rows is
+ * probability times its value's scale s is rounded to FP16, with all its bits down
+ * to 2^-21 of the row's largest; with more, q goes in as it is, and probabilities,
+ * as far down, and values s (c - z) are rounded to FP16.  One sequence of many
+ * rows takes all of its call to the second form, where a sequence of few rows is
  * worked on as if it had 128: prompts and single tokens are better two calls.
  *
- * MRT_ERR_SHAPE for more rows and keys than 31 bits number.  ws_dev: scratch of at least the bytes that
- * mrt_kv_q4_attention_workspace says for the same batch sizes (256-byte
- * aligned), the caller's own, so calls with scratch of their own may overlap;
- * its contents need no clearing and mean nothing afterwards.
+ * MRT_ERR_SHAPE for more rows and keys than 31 bits number.  ws_dev: scratch of at
+ * least the bytes that mrt_kv_q4_attention_workspace says for the same batch sizes
+ * (256-byte aligned), the caller's own, so calls with scratch of their own may
+ * overlap; its contents need no clearing and mean nothing afterwards.
  */
 int mrt_kv_q4_attention_workspace(mrt_kv_q4 kv, const mrt_kv_batch* batch, int64_t heads, size_t* bytes);
 int mrt_kv_q4_attention(mrt_kv_q4 kv, const mrt_kv_batch* batch, int dtype, const void* q_dev, int64_t ldq,
